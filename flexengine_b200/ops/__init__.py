@@ -1752,6 +1752,147 @@ def sample_listed(logits, temperature, top_k, seed, draw):
     return out
 
 
+# ---- keys and values held in 4 bits (csrc/kv4.cuh has their form) -------------------------------------------------------
+KV4_TILE = 16            # tokens of a tile: page sizes of a 4-bit cache are multiples of it
+KV4_MAX_DIM = 256
+KV4_MAX_SPLITS = 64      # what the merge kernel takes (fe_kv4_attention_max_splits)
+
+
+def kv4_row_bytes(d: int) -> int:
+    """Bytes of one token's key and value of one head: 5 bits a number, groups of 32 with a scale and a centre each."""
+    if d % 16 or not 16 <= d <= KV4_MAX_DIM:
+        raise ValueError(f"head size {d}: a 4-bit cache takes multiples of 16 from 16 to {KV4_MAX_DIM}")
+    return 40 * -(-d // 32)
+
+
+def kv4_shape(pages: int, nkv: int, page_size: int, d: int) -> tuple:
+    """The shape of a 4-bit cache of ``pages`` pages, a uint8 tensor: [pages, nkv, page_size / 16, bytes of a tile of 16 tokens]."""
+    if page_size < KV4_TILE or page_size % KV4_TILE:
+        raise ValueError(f"page size {page_size}: a 4-bit cache takes multiples of {KV4_TILE}")
+    return (pages, nkv, page_size // KV4_TILE, KV4_TILE * kv4_row_bytes(d))
+
+
+def _kv4():
+    return library.load("kv4")
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def _on(what, *tensors):
+    """A context in which the device of the tensors (which all lie on one) is the current one; refuses others."""
+    _need_cuda(*tensors)
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _index_ok(what, name, t, shape) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} is a contiguous int32 {list(shape)}, not {t.dtype} {list(t.shape)}")
+
+
+def _kv4_cache_ok(what, cache, nkv, d, page_size) -> None:
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or tuple(cache.shape) != kv4_shape(cache.shape[0], nkv, page_size, d) \
+            or not cache.is_contiguous() or cache.data_ptr() % 16:
+        raise ValueError(f"{what}: the cache is a contiguous uint8 {list(kv4_shape(cache.shape[0], nkv, page_size, d))} on a 16-byte boundary, "
+                         f"not {cache.dtype} {list(cache.shape)}")
+
+
+def qkv_rope_kv4(projected, bias, positions, inv_freq, rot, slot_mapping, cache, nq, nkv, d, page_size, pairs="halves", rot_gain=1.0,
+                 out_dtype=None):
+    """What ``qkv_bias_rope_cache`` does, for a 4-bit cache: ``projected`` [T, >= (nq + 2 nkv) d] (float32 or bfloat16, any row stride) +
+    ``bias`` (float32 or None), the first ``rot`` entries of query and key heads turned by position * ``inv_freq`` (float32 [rot / 2]) and
+    multiplied by ``rot_gain``; keys and values to their slots, rounded to 4 bits once, from 32 bits.  Returns the
+    queries [T, nq d] in ``out_dtype`` (the projection's where None).  ``pairs`` "halves": entry j turns with j + rot / 2, "interleaved": 2j with 2j + 1.
+    ``slot_mapping`` (int32 [T], None: no write): page * page_size + offset, distinct in one call; below 0: not written.  Angles are
+    taken in 64 bits: far positions turn as exactly as near ones."""
+    what = "qkv_rope_kv4"
+    with _on(what, projected, bias, positions, inv_freq if rot else None, slot_mapping, cache):
+        if projected.dim() != 2 or projected.shape[1] < (nq + 2 * nkv) * d or projected.stride(1) != 1:
+            raise ValueError(f"{what}: the projection is [T, >= (nq + 2 nkv) d] with unit column stride")
+        if pairs not in ("halves", "interleaved"):
+            raise ValueError(f"{what}: pairs {pairs!r}; 'halves' or 'interleaved'")
+        T, out_dtype = projected.shape[0], out_dtype or projected.dtype
+        _kv4_cache_ok(what, cache, nkv, d, page_size)
+        _index_ok(what, "positions", positions, (T,))
+        if slot_mapping is not None:
+            _index_ok(what, "slot_mapping", slot_mapping, (T,))
+        if bias is not None and (bias.dtype != torch.float32 or bias.numel() != (nq + 2 * nkv) * d or not bias.is_contiguous()):
+            raise ValueError(f"{what}: the bias is contiguous float32 [(nq + 2 nkv) d]")
+        if rot and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2 or not inv_freq.is_contiguous()):
+            raise ValueError(f"{what}: inv_freq is contiguous float32 [rot / 2]")
+        queries = torch.empty((T, nq * d), dtype=out_dtype, device=projected.device)
+        _run(_kv4(), "fe_qkv_rope_kv4", _ptr(projected), _code(projected.dtype), projected.stride(0) if T > 1 else projected.shape[1], _ptr(bias),
+             _ptr(positions), _ptr(inv_freq) if rot else None, rot, 1 if pairs == "interleaved" else 0, float(rot_gain), _ptr(slot_mapping), _ptr(cache),
+             _ptr(queries), _code(out_dtype), T, nq, nkv, d, page_size, cache.shape[0] * page_size, _ptr(status_word(projected.device)), _stream())
+    return queries
+
+
+def kv4_rows(cache, slots, nkv, d, page_size, dtype=torch.bfloat16):
+    """The keys and the values [N, nkv, d] that a 4-bit cache holds at ``slots`` (int32 [N], page * page_size + offset; below 0: zeros)."""
+    what = "kv4_rows"
+    with _on(what, cache, slots):
+        _kv4_cache_ok(what, cache, nkv, d, page_size)
+        n = slots.numel()
+        _index_ok(what, "slots", slots, (n,))
+        keys, values = (torch.empty((n, nkv, d), dtype=dtype, device=cache.device) for _ in range(2))
+        _run(_kv4(), "fe_kv4_rows", _ptr(cache), _ptr(slots), _ptr(keys), _ptr(values), _code(dtype), n, nkv, d, page_size, cache.shape[0] * page_size,
+             _ptr(status_word(cache.device)), _stream())
+    return keys, values
+
+
+def kv4_splits(blocks: int, keys: int, sms: int | None = None) -> int:
+    """Into how many blocks the keys of a row are shared out over a 4-bit cache; ``blocks``: column tiles x key/value heads."""
+    sms = sms or sm_count()
+    tiles = -(-keys // KV4_TILE)
+    return int(max(1, min(4 * sms // max(1, blocks), tiles // 8, KV4_MAX_SPLITS)))
+
+
+def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale, window=0, keep_first=0, sink=False):
+    """``paged_attention`` over a 4-bit cache: causal grouped-query attention of the step's tokens over their requests' pages.  q [T, >= nq d],
+    bfloat16 or float32, holds the turned queries in its first nq d columns; returns [T, nq d] of its type.  ``ctx``: the step
+    (``cu_q``, ``q_start``, ``max_q_len``, ``max_ctx_len``).  ``window`` > 0: the last so many keys are seen, and with ``keep_first`` the sequence's first
+    so many too; ``sink``: 1 is added to the softmax's denominator.  Codes are multiplied as they are, scales and centres applied in 32
+    bits (csrc/attention_kv4.cu); float32 queries keep 22 bits through the products."""
+    what = "paged_attention_kv4"
+    with _on(what, q, cache, block_table, ctx.cu_q, ctx.q_start):
+        T, requests = q.shape[0], ctx.cu_q.numel() - 1
+        if q.dim() != 2 or q.shape[1] < nq * d or q.stride(1) != 1 or (T > 1 and q.stride(0) % 8) or q.data_ptr() % 16:
+            raise ValueError(f"{what}: q is [T, >= nq d] with unit column stride, rows on 16-byte boundaries")
+        _kv4_cache_ok(what, cache, nkv, d, page_size)
+        _index_ok(what, "cu_q", ctx.cu_q, (requests + 1,))
+        _index_ok(what, "q_start", ctx.q_start, (requests,))
+        _index_ok(what, "block_table", block_table, (requests, block_table.shape[-1]))
+        if window < 0 or keep_first < 0 or (keep_first and not window):
+            raise ValueError(f"{what}: a window is not negative, and kept first keys go with one")
+        if ctx.max_ctx_len > block_table.shape[1] * page_size:
+            raise ValueError(f"{what}: {ctx.max_ctx_len} tokens in {block_table.shape[1]} pages of {page_size}")
+        columns = -(-ctx.max_q_len * (nq // nkv) // 8)
+        span = ctx.max_ctx_len if window == 0 else min(ctx.max_ctx_len, window + ctx.max_q_len + KV4_TILE + keep_first)
+        out = torch.empty((T, nq * d), dtype=q.dtype, device=q.device)
+        lengths = getattr(ctx, "host_lengths", None)
+        tiles = sum(-(-n * (nq // nkv) // 8) for n in lengths) if lengths else columns * requests
+        splits = kv4_splits(tiles * nkv, span)
+        # of its own for every call: two streams, or two captured graphs, may be at it at once
+        nbytes = _kv4().fe_kv4_attention_scratch_bytes(T, nq, d, splits)
+        part = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        _run(_kv4(), "fe_paged_attention_kv4", _ptr(q), q.stride(0) if T > 1 else nq * d, _ptr(out), nq * d, _ptr(cache), _ptr(block_table), block_table.shape[1],
+             _ptr(ctx.cu_q), _ptr(ctx.q_start), requests, T, ctx.max_q_len, nq, nkv, d, page_size, cache.shape[0], float(scale), window, keep_first,
+             1 if sink else 0, splits, _ptr(part), _code(q.dtype), _ptr(status_word(q.device)), _stream())
+    return out
+
+
 # ---- a whole decoder layer as one call --------------------------------------------------------------------------
 import ctypes as _ct
 

@@ -35,6 +35,8 @@ GROUPS = {
     # elementwise.cu once more: the layer executor launches its kernels from inside this library
     "bf16": ["errors.cu", "attention_mma.cu", "attention_tcgen05.cu", "gemm_skinny.cu", "gemm_tcgen05.cu", "elementwise.cu",
              "layer_executor.cu"],
+    # keys and values held in 4 bits
+    "kv4": ["errors.cu", "kv4_store.cu", "attention_kv4.cu"],
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}
