@@ -26,6 +26,8 @@
 // A weight p s has to keep its place in half precision whatever the scale of the values, so the reference point m is a maximum of score +
 // exponent of the token's largest value scale: 2^(score - m) s is then at most 2, and the sum of 2^(score - m) is kept in 32 bits, where
 // small scales may make it large.  The reference moves only when it has grown by more than 2^8.
+#include <type_traits>
+
 #define FE_PDL_CLASS 2      // FE_PDL_DECODE_ATTENTION
 #include "kv4.cuh"
 #include "tcgen05.cuh"
@@ -35,7 +37,7 @@ using namespace fe;
 namespace {
 
 constexpr int WARPS = 4;
-constexpr int STAGES = 4;
+constexpr int PAIR = 2;              // tiles that a warp takes at once
 constexpr long long WAIT_LIMIT = 1000000000LL;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float MOVE_STEP = 8.f;
@@ -49,10 +51,10 @@ __device__ __forceinline__ void mma(float* c, unsigned a0, unsigned a1, unsigned
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// the same with nothing added to
-__device__ __forceinline__ void mma_fresh(float* c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+// the same, added to ``even`` and ``odd`` in every row's two columns
+__device__ __forceinline__ void mma_from(float* c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1, float even, float odd) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};\n"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(even), "f"(odd));
 }
 __device__ __forceinline__ unsigned transposed(unsigned a) {
     unsigned d;
@@ -103,18 +105,33 @@ template <int NG> __device__ __forceinline__ void pieces(const unsigned char* p,
     }
 }
 
-// false when the wait ran out
-__device__ __forceinline__ bool wait_for(unsigned long long* bar, unsigned parity) { return mbar_wait(bar, parity, WAIT_LIMIT); }
+// false when the wait ran out; the test itself waits a while, so the clock is asked rarely
+__device__ __forceinline__ bool wait_for(unsigned long long* bar, unsigned parity) {
+    if (mbar_test(bar, parity)) return true;
+    return mbar_wait(bar, parity, WAIT_LIMIT);
+}
 
-__device__ __forceinline__ void copy_tile(void* dst, const unsigned char* src, int bytes, unsigned long long* bar) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy_tile(unsigned to, const unsigned char* from, int bytes, unsigned bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
-                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+                 ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
 }
 
 template <typename T> __device__ __forceinline__ void put(T* p, float v);
 template <> __device__ __forceinline__ void put<float>(float* p, float v) { *p = v; }
 template <> __device__ __forceinline__ void put<bf16>(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// the same variable in the shared memory of block ``rank`` of this cluster
+__device__ __forceinline__ float ld_cluster(const float* own, unsigned rank) {
+    unsigned remote;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(smem_u32(own)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(remote) : "memory");
+    return v;
+}
 
 struct Problem {
     const void* q;
@@ -126,25 +143,63 @@ struct Problem {
     int bt_stride;
     const int* cu_q;
     const int* q_start;
-    int nq, nkv, d, ps, num_pages;
+    int requests, nq, nkv, d, ps, num_pages;
     float scale_log2;
     int window, keep, sink, splits;
-    float* part;            // [token, head, split, d] float32, then [token, head, split] maxima and sums
+    float* part;            // partial results of the blocks: see the kernel
     long long tokens;       // rows of q
     int* status;
 };
 
-// dynamic shared memory: every warp's ring, and later the warps' results
-template <int NG, int NT> __host__ __device__ constexpr int ring_bytes() { return WARPS * STAGES * kv4_tile_bytes(NG); }
-template <int NG, int NT> __host__ __device__ constexpr int result_bytes() { return WARPS * 8 * NT * (32 * NG + 4) * 4; }
-template <int NG, int NT> __host__ __device__ constexpr int smem_bytes() {
-    return ring_bytes<NG, NT>() > result_bytes<NG, NT>() ? ring_bytes<NG, NT>() : result_bytes<NG, NT>();
+// dynamic shared memory: every warp's ring (two places of a pair of tiles each), then the warps' results
+constexpr int STAGES = 2;
+template <int NG> __host__ __device__ constexpr int ring_bytes() { return WARPS * STAGES * PAIR * kv4_tile_bytes(NG); }
+template <int NG, int NT> __host__ __device__ constexpr int smem_bytes() { return ring_bytes<NG>() + WARPS * 8 * NT * (32 * NG + 4) * 4; }
+
+// One piece of work of a block: tiles [t_begin, t_end) of the list that the columns from m0 on of (request r, head kvh) see.
+struct Segment {
+    int r, kvh, m0, columns, tok0, start, hi, lo, kept, t_begin, t_end;
+    int slot;               // where the partial result goes; -1: it is the whole
+    bool first;             // begins with the list's first tile
+};
+
+// Columns m0 .. of a request: what they see, as a list of tiles.
+__device__ __forceinline__ int fill(Segment& w, const Problem& a, int cols) {
+    const int G = a.nq / a.nkv, n_q = (int)min((long long)a.cu_q[w.r + 1], a.tokens) - a.cu_q[w.r];
+    w.tok0 = a.cu_q[w.r];
+    w.start = a.q_start[w.r];
+    w.columns = n_q * G;
+    w.hi = w.start + min(n_q - 1, (w.m0 + cols - 1) / G);
+    w.lo = first_visible(w.start + w.m0 / G, a.window);
+    w.kept = kept_tiles<KV4_TILE>(w.lo, a.keep);
+    return w.kept + w.hi / KV4_TILE - w.lo / KV4_TILE + 1;
 }
 
-// grid (splits x column tiles, key/value heads, requests).  TQ: queries and output; 32-bit ones in two parts.  NG: groups of a row.
-// NT: tiles of eight columns that a block takes.
-template <typename TQ, int NG, int NT>
-__global__ void __launch_bounds__(WARPS * 32)
+// Tiles that one column of request ``r`` sees, where requests bring one token each (0 for one that brings none).
+__device__ __forceinline__ int tiles_of(const Problem& a, int r) {
+    if (r >= a.requests || min((long long)a.cu_q[r + 1], a.tokens) <= a.cu_q[r]) return 0;
+    const int pos = a.q_start[r], lo = first_visible(pos, a.window);
+    return min(kept_tiles<KV4_TILE>(lo, a.keep) + pos / KV4_TILE - lo / KV4_TILE + 1, a.bt_stride * (a.ps / KV4_TILE));
+}
+
+// Blocks that are resident on an SM: the registers are cut to that.  16-bit queries at head size 128: three blocks of 168 registers a thread.
+template <typename TQ, int NG, int NT> __host__ __device__ constexpr int blocks_an_sm() { return sizeof(TQ) == 2 && NG * NT <= 4 ? 3 : 2; }
+
+// TQ: queries and output; 32-bit ones in two parts.  NG: groups of a row.  NT: tiles of eight columns that a block takes.
+//
+// SHARED = false: grid (column tiles x splits, heads, requests), the splits of a column tile a thread-block cluster, each with an equal share of its
+// tiles; their results are merged through distributed shared memory: no second kernel.
+// SHARED = true, where every request brings one token: the tiles of all (request, head, column tile) items, one after the other, are cut into as many
+// equal shares as there are blocks, whole rounds of the block's warps each; a block then takes the pieces of items that its share holds.  So
+// lengths that differ leave no block without work (a split of every item into equal parts left a seventh of the time to the last
+// blocks), and nothing on the host depends on them.  A block's share ends at most one item that others began and begins at
+// most one that others end: its partial results are 2 b (an item begun before) and 2 b + 1 (an item begun here).  ``part``: [blocks][2][8 NT]
+// [32 NG + 4] floats (numbers, maximum, sum), then for each item which blocks hold it.
+struct Held { int from, to; };      // blocks from .. to - 1; one block: it wrote the result itself
+template <int NG, int NT> __host__ __device__ constexpr int part_floats() { return 8 * NT * (32 * NG + 4); }
+
+template <typename TQ, int NG, int NT, bool SHARED>
+__global__ void __launch_bounds__(WARPS * 32, blocks_an_sm<TQ, NG, NT>())
 kv4_attention_kernel(const Problem a) {
     griddep_wait();
     griddep_launch_dependents();
@@ -154,445 +209,710 @@ kv4_attention_kernel(const Problem a) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) unsigned long long bars[WARPS][STAGES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % a.splits, r = blockIdx.z, kvh = blockIdx.y, G = a.nq / a.nkv;
-    const int tok0 = a.cu_q[r], n_q = (int)min((long long)a.cu_q[r + 1], a.tokens) - tok0, columns = n_q * G;
-    // the last columns walk the most keys: first
-    const int tiles_of_columns = (columns + COLS - 1) / COLS, m0 = (tiles_of_columns - 1 - (int)(blockIdx.x / a.splits)) * COLS;
-    if (m0 < 0 || columns <= 0) return;
-    const int start = a.q_start[r];
-    const int first_q = m0 / G, last_q = min(n_q - 1, (m0 + COLS - 1) / G);
-    const int hi = start + last_q, lo = first_visible(start + first_q, a.window);
-    const int kept = kept_tiles<KV4_TILE>(lo, a.keep), all_tiles = kept + hi / KV4_TILE - lo / KV4_TILE + 1;
-    const int per = (all_tiles + a.splits - 1) / a.splits, t_begin = split * per, t_end = min(all_tiles, t_begin + per);
-    const int mine = max(0, (t_end - t_begin - warp + WARPS - 1) / WARPS);       // tiles t_begin + warp, + WARPS, ...
-
+    const int G = a.nq / a.nkv;
     if (lane < STAGES) mbar_init(&bars[warp][lane], 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     __syncwarp();
 
-    // ---- where the tiles lie: a lane each for 32 of the warp's tiles at a time
-    const int* table = a.block_table + (long long)r * a.bt_stride;
-    const int per_page = a.ps / KV4_TILE;
-    const unsigned char* at = nullptr;                   // of this lane's tile of the batch whose copies are being started
-    unsigned here_now = 0, here_before = 0;              // which of that batch's and of the one before are in the cache
-    auto look_up = [&](int batch) {
-        const int k = 32 * batch + lane;
-        at = nullptr;
-        if (k < mine) {
-            const int tile = listed_tile<KV4_TILE>(t_begin + warp + WARPS * k, kept, lo);
-            const int page = tile / per_page < a.bt_stride ? table[tile / per_page] : -1;
-            if (page < 0 || page >= a.num_pages) {
-                if (a.status) atomicOr(a.status, FE_STATUS_BAD_PAGE);
+    // ---- what this block does; each warp keeps the piece in hand in shared memory, for the registers' sake
+    __shared__ Segment pieces_of[WARPS];
+    Segment& w = pieces_of[warp];
+    Segment found{};
+    constexpr int ROUND = PAIR * WARPS;
+    int share_end = 0, share = 1, item_tiles = 0, item_at = 0;          // SHARED: in tiles of all items, one after the other
+    const int columns_each = (G + COLS - 1) / COLS, items_each = a.nkv * columns_each;      // of a request
+    if (SHARED) {
+        const int mine = tiles_of(a, lane);                             // of the first 32 requests: asked for once
+        int total = __reduce_add_sync(FULL, mine);
+        for (int base = 32; base < a.requests; base += 32) total += __reduce_add_sync(FULL, tiles_of(a, base + lane));
+        total *= items_each;                                            // fewer than 2^31: asked of the sizes before the launch
+        share = ((total + (int)gridDim.x - 1) / (int)gridDim.x + ROUND - 1) / ROUND * ROUND;
+        const int begin = min(total, (int)blockIdx.x * share);
+        share_end = min(total, begin + share);
+        if (begin >= share_end) return;
+        // the request that holds tile ``begin``, from running sums
+        int before = 0;
+        found.r = -1;
+        for (int base = 0; base < a.requests && found.r < 0; base += 32) {
+            const int n = (base == 0 ? mine : tiles_of(a, base + lane)) * items_each;
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(FULL, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned here = __ballot_sync(FULL, begin >= before + upto - n && begin < before + upto);
+            if (here) {
+                const int at = __ffs(here) - 1;
+                found.r = base + at;
+                item_tiles = __shfl_sync(FULL, n, at) / items_each;
+                before += __shfl_sync(FULL, upto - n, at);
             } else
-                at = a.cache + (((long long)page * a.nkv + kvh) * per_page + tile % per_page) * TILE;
+                before += __shfl_sync(FULL, upto, 31);
         }
-        here_before = here_now;
-        here_now = __ballot_sync(FULL, at != nullptr);
-    };
-    unsigned char* ring = smem + warp * STAGES * TILE;
-    auto begin_copy = [&](int k) {
-        if ((k & 31) == 0) look_up(k >> 5);
-        const unsigned long long from = __shfl_sync(FULL, (unsigned long long)at, k & 31);
-        if (lane == 0) {
-            if (from) copy_tile(ring + (k % STAGES) * TILE, reinterpret_cast<const unsigned char*>(from), TILE, &bars[warp][k % STAGES]);
-            else mbar_arrive(&bars[warp][k % STAGES]);       // nothing to bring: the stage's turn passes all the same
-        }
-    };
-    for (int k = 0; k < STAGES - 1 && k < mine; ++k) begin_copy(k);
-
-    // ---- the queries: column n of tile j as B operands; thread (g, t) holds numbers 32 i + 8 t .. + 7 of column g
-    unsigned qf[NT][NG][4][PARTS], qsum[NT][2];          // qsum: (high, low) of the sums over group t, and over group t + 4
-    float factor[NT][2];                                 // takes a score of columns 2t, 2t + 1 to log2 units
-    int last_key[NT][2], first_key[NT][2];
-    float m[NT][2], l[NT][2];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int c = m0 + 8 * j + g;
-        const bool real = c < columns;
-        const TQ* row = static_cast<const TQ*>(a.q) + (long long)(tok0 + (real ? c / G : 0)) * a.q_stride + (long long)(kvh * G + (real ? c % G : 0)) * a.d;
-        float v[NG][8], largest = 0.f;
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const int from = 32 * i + 8 * t;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-            if (real && from < a.d) load8<TQ>(row + from, v[i]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(v[i][e]));
-        }
-        largest = fmaxf(largest, __shfl_xor_sync(FULL, largest, 1));
-        largest = fmaxf(largest, __shfl_xor_sync(FULL, largest, 2));
-        // a power of two brings the row's largest number to [1, 2): half precision then holds bfloat16 numbers as they are
-        const int e2 = min(max((int)(__float_as_uint(largest) >> 23) - 127, -126), 126);
-        const float down = __uint_as_float((unsigned)(127 - e2) << 23);
-        float sums[NG];
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            sums[i] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { v[i][e] *= down; sums[i] += v[i][e]; }
-            sums[i] += __shfl_xor_sync(FULL, sums[i], 1);
-            sums[i] += __shfl_xor_sync(FULL, sums[i], 2);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                qf[j][i][e][0] = pack(v[i][e], v[i][e + 4]);
-                if (PARTS == 2) qf[j][i][e][PARTS - 1] = pack_rest(v[i][e], v[i][e + 4], qf[j][i][e][0]);
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < NG; ++i)
-                if (i == t + 4 * h) s = sums[i];
-            const float high = __half2float(__float2half_rn(s));
-            qsum[j][h] = pack(high, s - high);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int mc = m0 + 8 * j + 2 * t + h;
-            factor[j][h] = a.scale_log2 * __uint_as_float((unsigned)(127 + __shfl_sync(FULL, e2, (2 * t + h) * 4)) << 23);
-            // a padding column sees what the last query sees: it is computed and never written, and must not make a tile a masked one
-            const int pos = mc < columns ? start + mc / G : hi;
-            last_key[j][h] = pos;
-            first_key[j][h] = mc < columns ? first_visible(pos, a.window) : lo;
-            m[j][h] = -CUDART_INF_F;
-            l[j][h] = 0.f;
-            if (a.sink && split == 0 && warp == 0) {
-                m[j][h] = 0.f;
-                l[j][h] = g == 0 ? 1.f : 0.f;            // the lanes of a column add their sums up at the end
-            }
-        }
+        const int item = (begin - before) / item_tiles;
+        item_at = before + item * item_tiles;
+        found.kvh = item / columns_each;
+        found.m0 = item % columns_each * COLS;
+        fill(found, a, COLS);
+        found.t_begin = begin - item_at;
+        found.t_end = min(item_tiles, share_end - item_at);
+        found.slot = found.t_end - found.t_begin == item_tiles ? -1 : 2 * (int)blockIdx.x + (found.t_begin == 0);
+    } else {
+        found.r = blockIdx.z;
+        found.kvh = blockIdx.y;
+        const int n_q = (int)min((long long)a.cu_q[found.r + 1], a.tokens) - a.cu_q[found.r];
+        // the last columns walk the most keys: first
+        found.m0 = ((n_q * G + COLS - 1) / COLS - 1 - (int)(blockIdx.x / a.splits)) * COLS;
+        if (found.m0 < 0 || n_q <= 0) return;                           // the whole cluster
+        const int all = fill(found, a, COLS), split = (int)(blockIdx.x % a.splits);
+        const int each = ((all + a.splits - 1) / a.splits + ROUND - 1) / ROUND * ROUND;
+        found.t_begin = min(all, split * each);
+        found.t_end = min(all, found.t_begin + each);
+        found.slot = a.splits > 1 ? 0 : -1;
     }
-    int last_least = last_key[0][0], first_most = first_key[0][0];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) { last_least = min(last_least, last_key[j][h]); first_most = max(first_most, first_key[j][h]); }
-    last_least = __reduce_min_sync(FULL, last_least);
-    first_most = __reduce_max_sync(FULL, first_most);
-
-    float o[NT][NG][2][4], oc[NT][NG][2];                // sums over codes, 16 numbers a tile, and over centres (this thread's tokens)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            oc[j][i][0] = oc[j][i][1] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][i][0][e] = o[j][i][1][e] = 0.f;
+    if (lane == 0) w = found;
+    __syncwarp();
+    // the next item of the share: its tiles may be those of another request
+    auto next = [&](Segment n) {
+        item_at += item_tiles;
+        if (!SHARED || item_at >= share_end) return false;
+        n.m0 += COLS;
+        if (n.m0 >= G) {
+            n.m0 = 0;
+            if (++n.kvh == a.nkv) {
+                n.kvh = 0;
+                do item_tiles = tiles_of(a, ++n.r); while (item_tiles == 0 && n.r < a.requests);      // the share ends inside a request that has some
+            }
         }
+        fill(n, a, COLS);
+        n.t_begin = 0;
+        n.t_end = min(item_tiles, share_end - item_at);
+        n.slot = n.t_end == item_tiles ? -1 : 2 * (int)blockIdx.x + 1;
+        __syncwarp();
+        if (lane == 0) w = n;
+        __syncwarp();
+        return true;
+    };
 
     const int even = 2 * t + (t & 1), odd = 2 * t + 1 - (t & 1);      // tokens of rows 2t and 2t + 1 (and of 2t + 8, 2t + 9: 8 on)
     const int key_row = (g & ~1) + ((g & 1) ^ (g >> 1 & 1));          // token of row g
+    const int key_codes = key_row * 16 * NG + t * 4 * NG, key_pairs = kv4_key_pairs(NG) + key_row * 4 * NG;
+    const int even_codes = kv4_value_codes(NG) + even * 16 * NG + g * 2 * NG, odd_codes = kv4_value_codes(NG) + odd * 16 * NG + g * 2 * NG;
+    const int per_page = a.ps / KV4_TILE;
+    unsigned char* ring = smem + warp * STAGES * PAIR * TILE;
+    float* results = reinterpret_cast<float*>(smem + ring_bytes<NG>());
+    unsigned stage = 0, parity = 0;
     bool gone = false;
-    for (int k = 0; k < mine; ++k) {
-        if (k + STAGES - 1 < mine) begin_copy(k + STAGES - 1);
-        if (__any_sync(FULL, !wait_for(&bars[warp][k % STAGES], (k / STAGES) & 1))) {
-            gone = true;
-            for (int later = k + 1; later < min(mine, k + STAGES); ++later) wait_for(&bars[warp][later % STAGES], (later / STAGES) & 1);
-            break;
-        }
-        // the batch of tile k: that of the newest copy or the one before
-        const int newest = min(mine - 1, k + STAGES - 1) >> 5;
-        if (!(((k >> 5) == newest ? here_now : here_before) >> (k & 31) & 1u)) continue;        // a page that is not there: nothing seen
-        const unsigned char* tile = ring + (k % STAGES) * TILE;
-        const int key0 = listed_tile<KV4_TILE>(t_begin + warp + WARPS * k, kept, lo) * KV4_TILE;
-        const bool masked = key0 + KV4_TILE - 1 > last_least || (key0 < first_most && key0 + KV4_TILE > a.keep);
 
-        // ---- scores of tokens key_row and key_row + 8 by columns 2t, 2t + 1
-        float s[NT][4];
-        {
-            unsigned c0 = 0, c1 = 0, c2 = 0, c3 = 0;                  // (centre, centre) of group t, and of group t + 4
-            const unsigned char* pairs = tile + kv4_key_pairs(NG);
-            if (t < NG) {
-                const unsigned w0 = *reinterpret_cast<const unsigned*>(pairs + (key_row * NG + t) * 4);
-                const unsigned w1 = *reinterpret_cast<const unsigned*>(pairs + ((key_row + 8) * NG + t) * 4);
-                c0 = __byte_perm(w0, w0, 0x3232); c1 = __byte_perm(w1, w1, 0x3232);
-            }
-            if (NG > 4 && t + 4 < NG) {
-                const unsigned w0 = *reinterpret_cast<const unsigned*>(pairs + (key_row * NG + t + 4) * 4);
-                const unsigned w1 = *reinterpret_cast<const unsigned*>(pairs + ((key_row + 8) * NG + t + 4) * 4);
-                c2 = __byte_perm(w0, w0, 0x3232); c3 = __byte_perm(w1, w1, 0x3232);
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) mma_fresh(s[j], c0, c1, c2, c3, qsum[j][0], NG > 4 ? qsum[j][1] : 0u);
-            unsigned k0[NG], k1[NG], p0[NG], p1[NG];
-            words<NG>(tile + key_row * 16 * NG + t * 4 * NG, k0);
-            words<NG>(tile + (key_row + 8) * 16 * NG + t * 4 * NG, k1);
-            words<NG>(pairs + key_row * 4 * NG, p0);
-            words<NG>(pairs + (key_row + 8) * 4 * NG, p1);
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                unsigned n0[4], n1[4];
-                kv4_decode(k0[i], n0);
-                kv4_decode(k1[i], n1);
-                const float s0 = low_half(p0[i]), s1 = low_half(p1[i]);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    float part[4];
-                    mma_fresh(part, n0[0], n1[0], n0[1], n1[1], qf[j][i][0][0], qf[j][i][1][0]);
-                    mma(part, n0[2], n1[2], n0[3], n1[3], qf[j][i][2][0], qf[j][i][3][0]);
-                    if (PARTS == 2) {
-                        mma(part, n0[0], n1[0], n0[1], n1[1], qf[j][i][0][PARTS - 1], qf[j][i][1][PARTS - 1]);
-                        mma(part, n0[2], n1[2], n0[3], n1[3], qf[j][i][2][PARTS - 1], qf[j][i][3][PARTS - 1]);
-                    }
-                    s[j][0] = fmaf(s0, part[0], s[j][0]);
-                    s[j][1] = fmaf(s0, part[1], s[j][1]);
-                    s[j][2] = fmaf(s1, part[2], s[j][2]);
-                    s[j][3] = fmaf(s1, part[3], s[j][3]);
-                }
-            }
+    // ---- where the tiles lie: a lane each for 32 of the warp's tiles at a time.  The warp's pairs of tiles are places t_begin + 2 warp,
+    // t_begin + 2 (warp + WARPS), ... of the list and the one after each
+    auto pairs_of = [&](const Segment& w) { return max(0, (w.t_end - w.t_begin - PAIR * warp + PAIR * WARPS - 1) / (PAIR * WARPS)); };
+    int at = -1;                                         // of this lane's tile of the batch whose copies are being started: its number in the cache
+    unsigned here_now = 0, here_before = 0;              // which of that batch's and of the one before are in the cache
+    auto look_up = [&](const Segment& w, int batch) {
+        const int place = w.t_begin + PAIR * (warp + WARPS * (16 * batch + (lane >> 1))) + (lane & 1);
+        at = -1;
+        if (place < w.t_end) {
+            const int tile = listed_tile<KV4_TILE>(place, w.kept, w.lo);
+            const int page = tile / per_page < a.bt_stride ? a.block_table[(long long)w.r * a.bt_stride + tile / per_page] : -1;
+            if (page < 0 || page >= a.num_pages) {
+                if (a.status) atomicOr(a.status, FE_STATUS_BAD_PAGE);
+            } else
+                at = (page * a.nkv + w.kvh) * per_page + tile % per_page;
         }
-        // ---- weights
-        unsigned v0[NG], v1[NG];                                      // (scale, centre) of the two tokens' value groups
-        words<NG>(tile + kv4_value_pairs(NG) + key_row * 4 * NG, v0);
-        words<NG>(tile + kv4_value_pairs(NG) + (key_row + 8) * 4 * NG, v1);
-        float big0 = low_half(v0[0]), big1 = low_half(v1[0]);
-#pragma unroll
-        for (int i = 1; i < NG; ++i) { big0 = fmaxf(big0, low_half(v0[i])); big1 = fmaxf(big1, low_half(v1[i])); }
-        // their exponents; zeros and subnormal numbers count as 2^-24, the least scale there is
-        const float up0 = fmaxf((float)((int)(__float_as_uint(big0) >> 23) - 127), -24.f), up1 = fmaxf((float)((int)(__float_as_uint(big1) >> 23) - 127), -24.f);
-        bool grows = false;
+        here_before = here_now;
+        here_now = __ballot_sync(FULL, at >= 0);
+    };
+    auto begin_copy = [&](const Segment& w, unsigned k, unsigned stage) {
+        if ((k & 15) == 0) look_up(w, k >> 4);
+        const int first = __shfl_sync(FULL, at, 2 * (k & 15)), second = __shfl_sync(FULL, at, 2 * (k & 15) + 1);
+        if (lane == 0) {
+            const unsigned bar = smem_u32(&bars[warp][stage]), to = smem_u32(ring + stage * PAIR * TILE);
+            // a tile that is not there brings nothing; the stage's turn passes all the same
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((first >= 0 ? TILE : 0) + (second >= 0 ? TILE : 0)) : "memory");
+            if (first >= 0) copy_tile(to, a.cache + (long long)first * TILE, TILE, bar);
+            if (second >= 0) copy_tile(to + TILE, a.cache + (long long)second * TILE, TILE, bar);
+        }
+    };
+    int mine = pairs_of(w);
+    if (mine > 0) begin_copy(w, 0, stage);
+
+    for (bool more = true; more;) {
+        const int m0 = w.m0, columns = w.columns, tok0 = w.tok0, start = w.start, kvh = w.kvh, lo = w.lo, kept = w.kept, t_begin = w.t_begin, t_end = w.t_end, slot = w.slot;
+
+        // ---- the queries: column n of tile j as B operands; thread (g, t) holds numbers 32 i + 8 t .. + 7 of column g
+        // Keys' codes are multiplied raised (by 1024 or 64: kv4_raise) where queries are 16-bit; ``lift`` is what that adds to a group's partial
+        // score, and eight codes' worth more, with the sign turned: the sums begin there.  That costs their last bits: with |q| in [1, 2)
+        // they are off by about 2^-24 8,000, a thousandth of what rounding the query to bfloat16 did.  (Values are summed over all keys,
+        // where the part of 1024 would grow: they are decoded in full, and so are keys under 32-bit queries.)
+        constexpr bool RAISED = PARTS == 1;
+        unsigned qf[NT][NG][4][PARTS], qsum[NT][2];          // qsum: (high, low) of the sums over group t, and over group t + 4
+        float lift[NT][NG][2];
+        float factor[NT][2];                                 // takes a score of columns 2t, 2t + 1 to log2 units
+        int last_key[NT][2], first_key[NT][2];
+        float below[NT][2], l[NT][2];                        // minus the reference point (infinite before the first key), the sum
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
+            const int c = m0 + 8 * j + g;
+            const bool real = c < columns;
+            const TQ* row = static_cast<const TQ*>(a.q) + (long long)(tok0 + (real ? c / G : 0)) * a.q_stride + (long long)(kvh * G + (real ? c % G : 0)) * a.d;
+            float v[NG][8], largest = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[j][e] *= factor[j][e & 1];
-                if (masked) {
-                    const int key = key0 + key_row + (e & 2) * 4;
-                    if (!(key <= last_key[j][e & 1] && (key >= first_key[j][e & 1] || key < a.keep))) s[j][e] = -CUDART_INF_F;
+            for (int i = 0; i < NG; ++i) {
+                const int from = 32 * i + 8 * t;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+                if (real && from < a.d) load8<TQ>(row + from, v[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(v[i][e]));
+            }
+            largest = fmaxf(largest, __shfl_xor_sync(FULL, largest, 1));
+            largest = fmaxf(largest, __shfl_xor_sync(FULL, largest, 2));
+            // a power of two brings the row's largest number to [1, 2): half precision then holds bfloat16 numbers as they are
+            const int e2 = min(max((int)(__float_as_uint(largest) >> 23) - 127, -126), 126);
+            const float down = __uint_as_float((unsigned)(127 - e2) << 23);
+            float sums[NG];
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                sums[i] = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { v[i][e] *= down; sums[i] += v[i][e]; }
+                sums[i] += __shfl_xor_sync(FULL, sums[i], 1);
+                sums[i] += __shfl_xor_sync(FULL, sums[i], 2);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    qf[j][i][e][0] = pack(v[i][e], v[i][e + 4]);
+                    if (PARTS == 2) qf[j][i][e][PARTS - 1] = pack_rest(v[i][e], v[i][e + 4], qf[j][i][e][0]);
                 }
-                grows |= s[j][e] + (e < 2 ? up0 : up1) > m[j][e & 1] + MOVE_STEP;
+                float raised = 0.f;
+                if (RAISED) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        raised -= ((e & 1 ? KV4_RAISED_ODD : KV4_RAISED_EVEN) + 8.f) * (low_half(qf[j][i][e][0]) + high_half(qf[j][i][e][0]));
+                    raised += __shfl_xor_sync(FULL, raised, 1);
+                    raised += __shfl_xor_sync(FULL, raised, 2);
+                }
+                lift[j][i][0] = __shfl_sync(FULL, raised, 8 * t);             // of columns 2t and 2t + 1
+                lift[j][i][1] = __shfl_sync(FULL, raised, 8 * t + 4);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < NG; ++i)
+                    if (i == t + 4 * h) s = sums[i];
+                const float high = __half2float(__float2half_rn(s));
+                qsum[j][h] = pack(high, s - high);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int mc = m0 + 8 * j + 2 * t + h;
+                factor[j][h] = a.scale_log2 * __uint_as_float((unsigned)(127 + __shfl_sync(FULL, e2, (2 * t + h) * 4)) << 23);
+                // a padding column sees what the last query sees: it is computed and never written, and must not make a tile a masked one
+                const int pos = mc < columns ? start + mc / G : w.hi;
+                last_key[j][h] = pos;
+                first_key[j][h] = mc < columns ? first_visible(pos, a.window) : lo;
+                below[j][h] = CUDART_INF_F;
+                l[j][h] = 0.f;
+                if (a.sink && t_begin == 0 && warp == 0) {
+                    below[j][h] = 0.f;
+                    l[j][h] = g == 0 ? 1.f : 0.f;            // the lanes of a column add their sums up at the end
+                }
             }
         }
-        if (__any_sync(FULL, grows)) {
+        int last_least = last_key[0][0], first_most = first_key[0][0];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { last_least = min(last_least, last_key[j][h]); first_most = max(first_most, first_key[j][h]); }
+        last_least = __reduce_min_sync(FULL, last_least);
+        first_most = __reduce_max_sync(FULL, first_most);
+
+        float o[NT][NG][2][4], oc[NT][NG][2];                // sums over codes, 16 numbers a tile, and over centres (this thread's tokens)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                oc[j][i][0] = oc[j][i][1] = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][i][0][e] = o[j][i][1][e] = 0.f;
+            }
+
+        // places [clear_from, clear_to) of the list are seen whole by every column (kept tiles are taken with the masked)
+        const int clear_from = kept + (first_most + KV4_TILE - 1) / KV4_TILE - lo / KV4_TILE;
+        const int clear_to = min(t_end, kept + (last_least + 1) / KV4_TILE - lo / KV4_TILE);
+        unsigned poisoned = 0;                                            // bit (j NG + i) 2 + h: column 2t + h of tile j has seen a NaN in group i of the values
+        // a pair of tiles; ``place``: of the first in the list; ``here``: which of the two were brought
+        auto take = [&](auto masked_tag, const unsigned char* pair, int place, unsigned here) {
+            constexpr bool MASKED = decltype(masked_tag)::value;
+            // ---- scores of tokens key_row and key_row + 8 of each tile by columns 2t, 2t + 1
+            float s[PAIR][NT][4];
+#pragma unroll
+            for (int u = 0; u < PAIR; ++u) {
+                const unsigned char* tile = pair + u * TILE;
+                const unsigned char* pairs = tile + key_pairs;
+                unsigned c0 = 0, c1 = 0, c2 = 0, c3 = 0;                  // (centre, centre) of group t, and of group t + 4
+                if (NG >= 4 || t < NG) {
+                    const unsigned w0 = *reinterpret_cast<const unsigned*>(pairs + t * 4);
+                    const unsigned w1 = *reinterpret_cast<const unsigned*>(pairs + t * 4 + 32 * NG);
+                    c0 = __byte_perm(w0, w0, 0x3232); c1 = __byte_perm(w1, w1, 0x3232);
+                }
+                if (NG > 4 && t + 4 < NG) {
+                    const unsigned w0 = *reinterpret_cast<const unsigned*>(pairs + t * 4 + 16);
+                    const unsigned w1 = *reinterpret_cast<const unsigned*>(pairs + t * 4 + 16 + 32 * NG);
+                    c2 = __byte_perm(w0, w0, 0x3232); c3 = __byte_perm(w1, w1, 0x3232);
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mma_from(s[u][j], c0, c1, c2, c3, qsum[j][0], NG > 4 ? qsum[j][1] : 0u, 0.f, 0.f);
+                unsigned k0[NG], k1[NG], p0[NG], p1[NG];
+                words<NG>(tile + key_codes, k0);
+                words<NG>(tile + key_codes + 128 * NG, k1);
+                words<NG>(pairs, p0);
+                words<NG>(pairs + 32 * NG, p1);
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    unsigned n0[4], n1[4];
+                    if (RAISED) { kv4_raise(k0[i], n0); kv4_raise(k1[i], n1); }
+                    else { kv4_decode(k0[i], n0); kv4_decode(k1[i], n1); }
+                    const float s0 = low_half(p0[i]), s1 = low_half(p1[i]);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        float part[4];
+                        mma_from(part, n0[0], n1[0], n0[1], n1[1], qf[j][i][0][0], qf[j][i][1][0], lift[j][i][0], lift[j][i][1]);
+                        mma(part, n0[2], n1[2], n0[3], n1[3], qf[j][i][2][0], qf[j][i][3][0]);
+                        if (PARTS == 2) {
+                            mma(part, n0[0], n1[0], n0[1], n1[1], qf[j][i][0][PARTS - 1], qf[j][i][1][PARTS - 1]);
+                            mma(part, n0[2], n1[2], n0[3], n1[3], qf[j][i][2][PARTS - 1], qf[j][i][3][PARTS - 1]);
+                        }
+                        s[u][j][0] = fmaf(s0, part[0], s[u][j][0]);
+                        s[u][j][1] = fmaf(s0, part[1], s[u][j][1]);
+                        s[u][j][2] = fmaf(s1, part[2], s[u][j][2]);
+                        s[u][j][3] = fmaf(s1, part[3], s[u][j][3]);
+                    }
+                }
+            }
+            // ---- weights
+            unsigned v0[PAIR][NG], v1[PAIR][NG];                          // (scale, centre) of the two tokens' value groups
+            float up0[PAIR], up1[PAIR], y[PAIR][NT][4];
+            bool grows = false;
+#pragma unroll
+            for (int u = 0; u < PAIR; ++u) {
+                words<NG>(pair + u * TILE + key_pairs + 64 * NG, v0[u]);
+                words<NG>(pair + u * TILE + key_pairs + 96 * NG, v1[u]);
+                if (MASKED) {
+                    const int key0 = (here >> u & 1u) ? listed_tile<KV4_TILE>(place + u, kept, lo) * KV4_TILE : 0x40000000;
+                    unsigned nan0 = 0, nan1 = 0;                          // groups that read as NaN; what was never written may
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        if ((v0[u][i] & 0x7c00u) == 0x7c00u) { nan0 |= 1u << (2 * i); v0[u][i] = 0; }
+                        if ((v1[u][i] & 0x7c00u) == 0x7c00u) { nan1 |= 1u << (2 * i); v1[u][i] = 0; }
+                        if (!(here >> u & 1u)) v0[u][i] = v1[u][i] = 0;   // what lay there before may be anything
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + key_row + (e & 2) * 4;
+                            if (!(key <= last_key[j][e & 1] && (key >= first_key[j][e & 1] || key < a.keep))) s[u][j][e] = -CUDART_INF_F;
+                            else poisoned |= (e < 2 ? nan0 : nan1) << (2 * NG * j + (e & 1));
+                        }
+                }
+                float big0 = low_half(v0[u][0]), big1 = low_half(v1[u][0]);
+#pragma unroll
+                for (int i = 1; i < NG; ++i) { big0 = fmaxf(big0, low_half(v0[u][i])); big1 = fmaxf(big1, low_half(v1[u][i])); }
+                // their exponents; zeros and subnormal numbers count as 2^-24, the least scale there is
+                up0[u] = fmaxf((float)(__float_as_uint(big0) >> 23) - 127.f, -24.f);
+                up1[u] = fmaxf((float)(__float_as_uint(big1) >> 23) - 127.f, -24.f);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        y[u][j][e] = fmaf(s[u][j][e], factor[j][e & 1], below[j][e & 1]);
+                        grows |= y[u][j][e] > MOVE_STEP - (e < 2 ? up0[u] : up1[u]);
+                    }
+            }
+            if (__any_sync(FULL, grows)) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float mx = -CUDART_INF_F;
+#pragma unroll
+                        for (int u = 0; u < PAIR; ++u)
+                            mx = fmaxf(mx, fmaxf(fmaf(s[u][j][h], factor[j][h], up0[u]), fmaf(s[u][j][h + 2], factor[j][h], up1[u])));
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, off));
+                        const float to = fmaxf(-below[j][h], mx);
+                        const float by = to == -CUDART_INF_F ? 1.f : ex2(-below[j][h] - to);      // 2^-inf = 0 at the start
+                        below[j][h] = -to;
+                        l[j][h] *= by;
+#pragma unroll
+                        for (int i = 0; i < NG; ++i) {
+                            oc[j][i][h] *= by;
+                            o[j][i][0][h] *= by; o[j][i][0][h + 2] *= by;
+                            o[j][i][1][h] *= by; o[j][i][1][h + 2] *= by;
+                        }
+#pragma unroll
+                        for (int u = 0; u < PAIR; ++u) {
+                            y[u][j][h] = fmaf(s[u][j][h], factor[j][h], -to);
+                            y[u][j][h + 2] = fmaf(s[u][j][h + 2], factor[j][h], -to);
+                        }
+                    }
+            }
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float mx = fmaxf(s[j][h] + up0, s[j][h + 2] + up1);
+                for (int u = 0; u < PAIR; ++u) {
 #pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, off));
-                    const float to = fmaxf(m[j][h], mx);
-                    const float by = to == -CUDART_INF_F ? 1.f : ex2(m[j][h] - to);      // 2^-inf = 0 at the start
-                    m[j][h] = to;
-                    l[j][h] *= by;
+                    for (int e = 0; e < 4; ++e) {
+                        y[u][j][e] = ex2(y[u][j][e]);
+                        if (MASKED && s[u][j][e] == -CUDART_INF_F) y[u][j][e] = 0.f;      // a column that has seen nothing yet has no reference point
+                    }
+                    l[j][0] += y[u][j][0] + y[u][j][2];
+                    l[j][1] += y[u][j][1] + y[u][j][3];
+                }
+            // ---- values: tokens even, odd (+ 8) in pairs; numbers 32 i + 4 g .. + 3
 #pragma unroll
-                    for (int i = 0; i < NG; ++i) {
-                        oc[j][i][h] *= by;
-                        o[j][i][0][h] *= by; o[j][i][0][h + 2] *= by;
-                        o[j][i][1][h] *= by; o[j][i][1][h + 2] *= by;
+            for (int u = 0; u < PAIR; ++u) {
+                constexpr int VW = (NG + 1) / 2;
+                unsigned ve[VW], vo[VW], ve8[VW], vo8[VW];
+                const unsigned char* tile = pair + u * TILE;
+                pieces<NG>(tile + even_codes, ve);
+                pieces<NG>(tile + odd_codes, vo);
+                pieces<NG>(tile + even_codes + 128 * NG, ve8);
+                pieces<NG>(tile + odd_codes + 128 * NG, vo8);
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    unsigned na[4], nb[4];
+                    kv4_decode(__byte_perm(ve[i / 2], vo[i / 2], (i & 1) ? 0x7632 : 0x5410), na);
+                    kv4_decode(__byte_perm(ve8[i / 2], vo8[i / 2], (i & 1) ? 0x7632 : 0x5410), nb);
+                    const float s0 = low_half(v0[u][i]), s1 = low_half(v1[u][i]), c0 = high_half(v0[u][i]), c1 = high_half(v1[u][i]);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const float* w = y[u][j];
+                        oc[j][i][0] = fmaf(w[0], c0, fmaf(w[2], c1, oc[j][i][0]));
+                        oc[j][i][1] = fmaf(w[1], c0, fmaf(w[3], c1, oc[j][i][1]));
+                        const unsigned w0 = pack(w[0] * s0, w[1] * s0), w1 = pack(w[2] * s1, w[3] * s1);
+                        const unsigned b0 = transposed(w0), b1 = transposed(w1);
+                        mma(o[j][i][0], na[0], na[1], nb[0], nb[1], b0, b1);
+                        mma(o[j][i][1], na[2], na[3], nb[2], nb[3], b0, b1);
+                        if (PARTS == 2) {
+                            const unsigned r0 = transposed(pack_rest(w[0] * s0, w[1] * s0, w0)), r1 = transposed(pack_rest(w[2] * s1, w[3] * s1, w1));
+                            mma(o[j][i][0], na[0], na[1], nb[0], nb[1], r0, r1);
+                            mma(o[j][i][1], na[2], na[3], nb[2], nb[3], r0, r1);
+                        }
                     }
                 }
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float ref = m[j][e & 1];
-                s[j][e] = ex2(s[j][e] - (ref == -CUDART_INF_F ? 0.f : ref));
             }
-            l[j][0] += s[j][0] + s[j][2];
-            l[j][1] += s[j][1] + s[j][3];
-        }
-        // ---- values: tokens even, odd (+ 8) in pairs; numbers 32 i + 4 g .. + 3
-        constexpr int VW = (NG + 1) / 2;
-        unsigned ve[VW], vo[VW], ve8[VW], vo8[VW];
-        const unsigned char* codes = tile + kv4_value_codes(NG) + g * 2 * NG;
-        pieces<NG>(codes + even * 16 * NG, ve);
-        pieces<NG>(codes + odd * 16 * NG, vo);
-        pieces<NG>(codes + (even + 8) * 16 * NG, ve8);
-        pieces<NG>(codes + (odd + 8) * 16 * NG, vo8);
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            unsigned na[4], nb[4];
-            kv4_decode(__byte_perm(ve[i / 2], vo[i / 2], (i & 1) ? 0x7632 : 0x5410), na);
-            kv4_decode(__byte_perm(ve8[i / 2], vo8[i / 2], (i & 1) ? 0x7632 : 0x5410), nb);
-            const float s0 = low_half(v0[i]), s1 = low_half(v1[i]), c0 = high_half(v0[i]), c1 = high_half(v1[i]);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                float w[4] = {s[j][0] * s0, s[j][1] * s0, s[j][2] * s1, s[j][3] * s1};
-                float z[4] = {s[j][0] * c0, s[j][1] * c0, s[j][2] * c1, s[j][3] * c1};
-                if (masked) {                                         // what lies behind a mask may be anything, NaN too
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (s[j][e] == 0.f) w[e] = z[e] = 0.f;
-                }
-                oc[j][i][0] += z[0] + z[2];
-                oc[j][i][1] += z[1] + z[3];
-                const unsigned w0 = pack(w[0], w[1]), w1 = pack(w[2], w[3]);
-                const unsigned b0 = transposed(w0), b1 = transposed(w1);
-                mma(o[j][i][0], na[0], na[1], nb[0], nb[1], b0, b1);
-                mma(o[j][i][1], na[2], na[3], nb[2], nb[3], b0, b1);
-                if (PARTS == 2) {
-                    const unsigned r0 = transposed(pack_rest(w[0], w[1], w0)), r1 = transposed(pack_rest(w[2], w[3], w1));
-                    mma(o[j][i][0], na[0], na[1], nb[0], nb[1], r0, r1);
-                    mma(o[j][i][1], na[2], na[3], nb[2], nb[3], r0, r1);
-                }
+        };
+#pragma unroll 1
+        for (unsigned k = 0; k < (unsigned)mine && !gone; ++k) {
+            if (k + 1 < (unsigned)mine) begin_copy(w, k + 1, stage ^ 1);
+            if (__any_sync(FULL, !wait_for(&bars[warp][stage], parity))) {
+                gone = true;
+                if (k + 1 < (unsigned)mine) wait_for(&bars[warp][stage ^ 1], parity ^ stage);
+                break;
             }
+            // the batch of pair k is that of the newest copy or the one before
+            const unsigned newest = min((unsigned)mine - 1, k + 1) >> 4;
+            const unsigned here = ((k >> 4) == newest ? here_now : here_before) >> (2 * (k & 15)) & 3u;
+            const unsigned char* pair = ring + stage * PAIR * TILE;
+            const int place = t_begin + PAIR * (warp + WARPS * (int)k);
+            if (here == 3u && place >= clear_from && place + 1 < clear_to) take(std::false_type{}, pair, place, here);
+            else take(std::true_type{}, pair, place, here);
+            __syncwarp();                                                 // the stage is free: the next turn's copy goes there
+            parity ^= stage;
+            stage ^= 1;
         }
-        __syncwarp();                                                 // the stage is free: the next turn's copy goes there
-    }
-    if (gone && lane == 0 && a.status) atomicOr(a.status, FE_STATUS_WAIT_EXPIRED);
+        // the next piece's first tiles are on their way while this one's results are put together
+        const int item_last = item_at + item_tiles - 1, item = (w.r * a.nkv + kvh) * columns_each + m0 / COLS;
+        more = next(w);
+        if (more && !gone) {
+            mine = pairs_of(w);
+            if (mine > 0) begin_copy(w, 0, stage);
+        }
 
-    // ---- the warp's sums over its lanes, then the four warps' results side by side: [warp][column][32 NG numbers, maximum, sum]
-    constexpr int ROW = 32 * NG + 4;
+        // ---- the warp's sums over its lanes, then the four warps' results side by side: [warp][column][32 NG numbers, maximum, sum]
+        constexpr int ROW = 32 * NG + 4;
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) {
-                l[j][h] += __shfl_xor_sync(FULL, l[j][h], off);
+                for (int off = 4; off < 32; off <<= 1) {
+                    l[j][h] += __shfl_xor_sync(FULL, l[j][h], off);
 #pragma unroll
-                for (int i = 0; i < NG; ++i) oc[j][i][h] += __shfl_xor_sync(FULL, oc[j][i][h], off);
+                    for (int i = 0; i < NG; ++i) oc[j][i][h] += __shfl_xor_sync(FULL, oc[j][i][h], off);
+                }
             }
-        }
-    __syncthreads();                                                  // every warp has read its last tile
-    float* results = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+        for (int off = 4; off < 32; off <<= 1) poisoned |= __shfl_xor_sync(FULL, poisoned, off);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float* to = results + (warp * COLS + 8 * j + 2 * t + h) * ROW;
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int i = 0; i < NG; ++i)
-                *reinterpret_cast<float4*>(to + 32 * i + 4 * g) =
-                    make_float4(o[j][i][0][h] + oc[j][i][h], o[j][i][0][h + 2] + oc[j][i][h], o[j][i][1][h] + oc[j][i][h], o[j][i][1][h + 2] + oc[j][i][h]);
-            if (g == 0) { to[32 * NG] = m[j][h]; to[32 * NG + 1] = l[j][h]; }
-        }
-    __syncthreads();
-    for (int c = warp; c < COLS && m0 + c < columns; c += WARPS) {
-        const int mc = m0 + c, token = tok0 + mc / G, head = kvh * G + mc % G;
-        float top = -CUDART_INF_F;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, results[(w * COLS + c) * ROW + 32 * NG]);
-        float by[WARPS], sum = 0.f;
+                for (int h = 0; h < 2; ++h)
+                    if (poisoned >> (2 * (j * NG + i) + h) & 1u) oc[j][i][h] = CUDART_NAN_F;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float mw = results[(w * COLS + c) * ROW + 32 * NG];
-            by[w] = mw == -CUDART_INF_F ? 0.f : ex2(mw - top);
-            sum += by[w] * results[(w * COLS + c) * ROW + 32 * NG + 1];
-        }
-        const long long line = (long long)token * a.nq + head;
-        const float inv = a.splits > 1 ? 1.f : sum > 0.f ? 1.f / sum : 0.f;
-        for (int i = lane; i < a.d; i += 32) {
-            float v = 0.f;
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) v += by[w] != 0.f ? by[w] * results[(w * COLS + c) * ROW + i] : 0.f;
-            if (a.splits > 1) a.part[(line * a.splits + split) * a.d + i] = v;
-            else put<TQ>(static_cast<TQ*>(a.out) + (long long)token * a.out_stride + (long long)head * a.d + i, v * inv);
+            for (int h = 0; h < 2; ++h) {
+                float* to = results + (warp * COLS + 8 * j + 2 * t + h) * ROW;
+#pragma unroll
+                for (int i = 0; i < NG; ++i)
+                    *reinterpret_cast<float4*>(to + 32 * i + 4 * g) =
+                        make_float4(o[j][i][0][h] + oc[j][i][h], o[j][i][0][h + 2] + oc[j][i][h], o[j][i][1][h] + oc[j][i][h], o[j][i][1][h + 2] + oc[j][i][h]);
+                if (g == 0) { to[32 * NG] = -below[j][h]; to[32 * NG + 1] = l[j][h]; }
+            }
+        __syncthreads();
+        for (int c = warp; c < COLS && m0 + c < columns; c += WARPS) {
+            const int mc = m0 + c, token = tok0 + mc / G, head = kvh * G + mc % G;
+            float top = -CUDART_INF_F;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, results[(w * COLS + c) * ROW + 32 * NG]);
+            float by[WARPS], sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float mw = results[(w * COLS + c) * ROW + 32 * NG];
+                by[w] = mw == -CUDART_INF_F ? 0.f : ex2(mw - top);
+                sum += by[w] * results[(w * COLS + c) * ROW + 32 * NG + 1];
+            }
+            const bool whole = slot < 0;
+            const float inv = !whole ? 1.f : sum > 0.f ? 1.f / sum : 0.f;
+            float* part = whole ? nullptr : SHARED ? a.part + ((long long)slot * COLS + c) * ROW : results + c * ROW;      // in place: see below
+            __syncwarp();                                             // maxima and sums are read
+            TQ* to = static_cast<TQ*>(a.out) + (long long)token * a.out_stride + (long long)head * a.d;
+            for (int i = lane; i < a.d; i += 32) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) v += by[w] != 0.f ? by[w] * results[(w * COLS + c) * ROW + i] : 0.f;
+                if (whole) put<TQ>(to + i, sum != sum ? sum : v * inv);
+                else part[i] = v;
+            }
+            if (!whole && lane == 0) { part[32 * NG] = top; part[32 * NG + 1] = sum; }
         }
-        if (a.splits > 1 && lane == 0)
-            reinterpret_cast<float2*>(a.part + a.tokens * a.nq * a.splits * a.d)[line * a.splits + split] = make_float2(top, sum);
+        if (!SHARED && a.splits > 1) {
+            // A column's sums lie where those of the first warp's were (a thread overwrote what it had read); the cluster's blocks take
+            // every splits-th column, and add the splits in their order.
+            const unsigned splits = a.splits, rank = blockIdx.x % a.splits;
+            cluster_barrier();
+            for (int c = rank + splits * warp; c < COLS && m0 + c < columns; c += splits * WARPS) {
+                const int mc = m0 + c, token = tok0 + mc / G, head = kvh * G + mc % G;
+                const float* own = results + c * ROW;
+                const float at = lane < (int)splits ? ld_cluster(own + 32 * NG, lane) : -CUDART_INF_F;
+                const float top = warp_max(at), by = at == -CUDART_INF_F ? 0.f : ex2(at - top);
+                const float sum = warp_sum(lane < (int)splits ? by * ld_cluster(own + 32 * NG + 1, lane) : 0.f);
+                for (int i0 = 0; i0 < a.d; i0 += 32) {
+                    const int i = i0 + lane;
+                    float v = 0.f;
+                    for (unsigned p = 0; p < splits; ++p) {
+                        const float weight = __shfl_sync(FULL, by, p);
+                        if (weight != 0.f && i < a.d) v += weight * ld_cluster(own + i, p);
+                    }
+                    if (i < a.d) put<TQ>(static_cast<TQ*>(a.out) + (long long)token * a.out_stride + (long long)head * a.d + i, sum != sum ? sum : sum > 0.f ? v / sum : 0.f);
+                }
+            }
+            cluster_barrier();                                        // nobody leaves while its shared memory may still be read
+        }
+        if (SHARED && t_begin == 0 && threadIdx.x == 0) {
+            // which blocks hold this item
+            Held* held = reinterpret_cast<Held*>(a.part + (long long)gridDim.x * 2 * part_floats<NG, NT>());
+            const int b = (int)blockIdx.x;
+            held[item] = Held{b, slot < 0 ? b + 1 : item_last / share + 1};
+        }
+        __syncthreads();                                                  // the results are read: the next piece's go there
     }
 }
 
-constexpr int MAX_SPLITS = 64;
+constexpr int MAX_SPLITS = 8;            // blocks of a cluster
+constexpr int MERGE_THREADS = 256;
 
-// A block per (token, head): the splits' sums, weighted by their maxima, in the splits' order.
-template <typename TQ>
-__global__ void __launch_bounds__(128)
-kv4_merge_kernel(const float* __restrict__ part, TQ* __restrict__ out, long long out_stride, int nq, int d, int splits, long long rows) {
+// A block per (head, request): what several blocks hold of an item is weighted by their maxima and added.  Sets of threads, four numbers of
+// the head a thread, take every sets-th part, AHEAD parts on their way at once, with a running maximum of their own; the sets are
+// added in their order.
+template <typename TQ, int NG, int NT>
+__global__ void __launch_bounds__(MERGE_THREADS)
+kv4_merge_kernel(const Problem a, int blocks) {
     griddep_wait();
     griddep_launch_dependents();
-    __shared__ float by[MAX_SPLITS];
-    const long long line = blockIdx.x;
-    const float2* heads = reinterpret_cast<const float2*>(part + rows * splits * d) + line * splits;
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        float2 h[MAX_SPLITS / 32];
+    constexpr int COLS = 8 * NT, ROW = 32 * NG + 4, SETS = MERGE_THREADS / (8 * NG), AHEAD = 8;
+    __shared__ __align__(16) float sums[SETS][ROW];
+    const int r = blockIdx.y, head = blockIdx.x, G = a.nq / a.nkv, kvh = head / G, m = head % G;
+    const int token = a.cu_q[r], behind = a.cu_q[r + 1];
+    const Held held = reinterpret_cast<const Held*>(a.part + (long long)blocks * 2 * part_floats<NG, NT>())[(r * a.nkv + kvh) * ((G + COLS - 1) / COLS) + m / COLS];
+    if (min((long long)behind, a.tokens) <= token) return;
+    const int n = held.to - held.from;
+    if (n <= 1) return;
+    const int set = threadIdx.x / (8 * NG), i = threadIdx.x % (8 * NG) * 4;
+    if (set < SETS) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float top = -CUDART_INF_F, sum = 0.f;
+        for (int s0 = set; s0 < n; s0 += AHEAD * SETS) {
+            float4 x[AHEAD];
+            float2 end[AHEAD];
+            float most = top;
 #pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 32; ++i) {
-            h[i] = lane + 32 * i < splits ? heads[lane + 32 * i] : make_float2(-CUDART_INF_F, 0.f);
-            top = fmaxf(top, h[i].x);
+            for (int u = 0; u < AHEAD; ++u) {
+                const int s = s0 + u * SETS;
+                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                end[u] = make_float2(-CUDART_INF_F, 0.f);
+                if (s < n) {
+                    // the first block's part is of the item that it began, the others' of the one they found begun
+                    const float* from = a.part + ((long long)(2 * (held.from + s) + (s == 0)) * COLS + m % COLS) * ROW;
+                    end[u] = *reinterpret_cast<const float2*>(from + 32 * NG);
+                    x[u] = *reinterpret_cast<const float4*>(from + i);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) most = fmaxf(most, end[u].x);
+            if (most == -CUDART_INF_F) continue;
+            const float by = ex2(top - most);
+            top = most;
+            sum *= by;
+            v.x *= by; v.y *= by; v.z *= by; v.w *= by;
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (end[u].x == -CUDART_INF_F) continue;             // saw nothing: what it left is not looked at
+                const float w = ex2(end[u].x - most);
+                sum += w * end[u].y;
+                v.x += w * x[u].x; v.y += w * x[u].y; v.z += w * x[u].z; v.w += w * x[u].w;
+            }
         }
-        top = warp_max(top);
-#pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 32; ++i) {
-            h[i].x = h[i].x == -CUDART_INF_F ? 0.f : ex2(h[i].x - top);
-            sum += h[i].x * h[i].y;
-        }
-        sum = warp_sum(sum);
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 32; ++i) by[lane + 32 * i] = h[i].x * inv;
+        *reinterpret_cast<float4*>(&sums[set][i]) = v;
+        if (i == 0) { sums[set][32 * NG] = top; sums[set][32 * NG + 1] = sum; }
     }
     __syncthreads();
-    const float* from = part + line * splits * d;
-    TQ* to = out + line / nq * out_stride + line % nq * d;
-    for (int i = threadIdx.x; i < d; i += blockDim.x) {
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s)
-            if (by[s] != 0.f) v += by[s] * from[(long long)s * d + i];
-        put<TQ>(to + i, v);
+    if (threadIdx.x < a.d) {
+        float top = -CUDART_INF_F, sum = 0.f, v = 0.f;
+        for (int k = 0; k < SETS; ++k) top = fmaxf(top, sums[k][32 * NG]);
+        for (int k = 0; k < SETS; ++k) {
+            const float at = sums[k][32 * NG], by = at == -CUDART_INF_F ? 0.f : ex2(at - top);
+            sum += by * sums[k][32 * NG + 1];
+            v += by * sums[k][threadIdx.x];
+        }
+        put<TQ>(static_cast<TQ*>(a.out) + (long long)token * a.out_stride + (long long)head * a.d + threadIdx.x, sum != sum ? sum : sum > 0.f ? v / sum : 0.f);
     }
 }
 
-template <typename TQ, int NG, int NT>
-int launch_as(const Problem& a, int requests, int column_tiles, cudaStream_t stream) {
+// Blocks of the kernel that the device holds at once (asked of the driver once per device).
+template <typename TQ, int NG, int NT> int resident() {
+    static int cached[64];
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 0;
+    if (cached[device] == 0) {
+        int each = 0;
+        constexpr int smem = smem_bytes<NG, NT>();
+        cudaFuncSetAttribute(kv4_attention_kernel<TQ, NG, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kv4_attention_kernel<TQ, NG, NT, true>, WARPS * 32, smem) != cudaSuccess || each < 1) {
+            cudaGetLastError();
+            each = 1;
+        }
+        cached[device] = each * fe_sm_count();
+    }
+    return cached[device];
+}
+
+struct Launch {
+    const Problem* a;
+    int requests, column_tiles, blocks;
+    cudaStream_t stream;
+};
+
+template <typename TQ, int NG, int NT> int run(const Launch& w) {
     constexpr int smem = smem_bytes<NG, NT>();
-    if (smem > 48 * 1024) {
-        const cudaError_t err = cudaFuncSetAttribute(kv4_attention_kernel<TQ, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        FE_REQUIRE(err == cudaSuccess, "paged_attention_kv4: %s", cudaGetErrorString(err));
-    }
-    fe::launch(kv4_attention_kernel<TQ, NG, NT>, dim3((unsigned)(a.splits * column_tiles), (unsigned)a.nkv, (unsigned)requests), WARPS * 32, smem, stream, a);
-    return fe_check_launch("paged_attention_kv4");
+    const Problem& a = *w.a;
+    auto kernel = w.blocks ? kv4_attention_kernel<TQ, NG, NT, true> : kv4_attention_kernel<TQ, NG, NT, false>;
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    FE_REQUIRE(err == cudaSuccess, "paged_attention_kv4: %s", cudaGetErrorString(err));
+    const dim3 grid = w.blocks ? dim3((unsigned)w.blocks) : dim3((unsigned)(w.column_tiles * a.splits), (unsigned)a.nkv, (unsigned)w.requests);
+    if (!w.blocks && a.splits > 1) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(WARPS * 32);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = w.stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = a.splits;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t launched = cudaLaunchKernelEx(&cfg, kernel, a);
+        FE_REQUIRE(launched == cudaSuccess, "paged_attention_kv4 (clusters of %d): %s", a.splits, cudaGetErrorString(launched));
+    } else
+        fe::launch(kernel, grid, WARPS * 32, smem, w.stream, a);
+    if (const int rc = fe_check_launch("paged_attention_kv4")) return rc;
+    if (!w.blocks) return 0;
+    fe::launch_as(FE_PDL_ELEMENTWISE, kv4_merge_kernel<TQ, NG, NT>, dim3((unsigned)a.nq, (unsigned)w.requests), MERGE_THREADS, 0, w.stream, a, w.blocks);
+    return fe_check_launch("paged_attention_kv4 merge");
 }
 
-template <typename TQ, int NT>
-int launch_groups(const Problem& a, int requests, int column_tiles, cudaStream_t stream) {
-    switch (kv4_groups(a.d)) {
-        case 1: return launch_as<TQ, 1, NT>(a, requests, column_tiles, stream);
-        case 2: return launch_as<TQ, 2, NT>(a, requests, column_tiles, stream);
-        case 3: return launch_as<TQ, 3, NT>(a, requests, column_tiles, stream);
-        case 4: return launch_as<TQ, 4, NT>(a, requests, column_tiles, stream);
-        case 5: return launch_as<TQ, 5, NT>(a, requests, column_tiles, stream);
-        case 6: return launch_as<TQ, 6, NT>(a, requests, column_tiles, stream);
-        case 7: return launch_as<TQ, 7, NT>(a, requests, column_tiles, stream);
-        default: return launch_as<TQ, 8, NT>(a, requests, column_tiles, stream);
+// f(groups of a row as a constant)
+template <typename F> auto with_groups(int d, F f) {
+    switch (kv4_groups(d)) {
+        case 1: return f(std::integral_constant<int, 1>{});
+        case 2: return f(std::integral_constant<int, 2>{});
+        case 3: return f(std::integral_constant<int, 3>{});
+        case 4: return f(std::integral_constant<int, 4>{});
+        case 5: return f(std::integral_constant<int, 5>{});
+        case 6: return f(std::integral_constant<int, 6>{});
+        case 7: return f(std::integral_constant<int, 7>{});
+        default: return f(std::integral_constant<int, 8>{});
     }
 }
-
-template <typename TQ>
-int attend(const Problem& a, int requests, int max_q_len, cudaStream_t stream) {
-    const int column_tiles = (int)(((long long)max_q_len * (a.nq / a.nkv) + 7) / 8);
-    return launch_groups<TQ, 1>(a, requests, column_tiles, stream);
-}
+bool head_size_ok(int d) { return d >= 16 && d % 16 == 0 && d <= KV4_MAX_DIM; }
 
 }  // namespace
 
-extern "C" int fe_kv4_attention_max_splits() { return MAX_SPLITS; }
-
-// Bytes of ``scratch`` for ``tokens`` rows of queries.
-extern "C" long long fe_kv4_attention_scratch_bytes(long long tokens, int nq, int d, int splits) {
-    return splits > 1 ? tokens * nq * splits * (4LL * d + 8) : 0;
+// How a decode step's tiles are dealt out: a positive number is that of the blocks that share the tiles of all items; a negative one, -S, a cluster of S
+// blocks for each item.  ``tiles``: of the longest request.
+//
+// An item of up to 16 tiles is one block's.  A cluster as large as leaves all of them resident at once is the shortest way while a
+// block walks up to 32 tiles; sharing out costs running sums over the requests and a second kernel, and wins where one item is too much for
+// eight blocks or lengths differ.  28/4 heads of 128, microseconds: 8 requests of 2,049 keys 13.7 in clusters of 4, 20 shared; 16 of 2,048
+// 13.7 and 21; 1 of 8,192 17.8 (8) and 14.4; 64 of 1,024 to 8,191 75 (2) and 67.
+extern "C" int fe_kv4_attention_plan(int requests, int tiles, int nq, int nkv, int d, int dtype) {
+    if (!head_size_ok(d) || requests <= 0 || nq <= 0 || nkv <= 0) return -1;
+    const long long items = (long long)requests * nkv * ((nq / nkv + 7) / 8), all = items * tiles;
+    if (tiles <= 16) return -1;
+    const long long most = dtype == FE_F32 ? with_groups(d, [](auto n) { return resident<float, n.value, 1>(); }) : with_groups(d, [](auto n) { return resident<bf16, n.value, 1>(); });
+    const long long fit = most / items, splits = fit < 1 ? 1 : fit > MAX_SPLITS ? MAX_SPLITS : fit;
+    const long long useful = (tiles + 7) / 8, each = splits < useful ? splits : useful;
+    if ((tiles + each - 1) / each <= 32 || all >= (1LL << 31)) return -(int)each;
+    const long long want = (all + 15) / 16;
+    return (int)(want < most ? want : most);
 }
 
-// q [tokens, >= nq d], rows ``q_stride`` elements apart; out likewise; dtype of both.  ``splits``: blocks that share a row's keys.
+// Bytes of ``scratch`` for so many blocks.
+extern "C" long long fe_kv4_attention_scratch_bytes(int blocks, int requests, int nq, int nkv, int d) {
+    if (blocks <= 0 || nkv <= 0) return 0;
+    return (long long)blocks * 2 * 8 * (32 * kv4_groups(d) + 4) * 4 + (long long)requests * nkv * ((nq / nkv + 7) / 8) * (long long)sizeof(Held);
+}
+
+// q [tokens, >= nq d], rows ``q_stride`` elements apart; out likewise; dtype of both.  ``blocks`` > 0 (from fe_kv4_attention_blocks; every request
+// brings one token at most) needs scratch.
 extern "C" int fe_paged_attention_kv4(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, const int* block_table,
                                       int bt_stride, const int* cu_q, const int* q_start, int requests, long long tokens, int max_q_len, int nq,
-                                      int nkv, int d, int ps, int num_pages, float scale, int window, int keep, int sink, int splits, void* scratch,
+                                      int nkv, int d, int ps, int num_pages, float scale, int window, int keep, int sink, int splits, int blocks, void* scratch,
                                       int dtype, int* status, cudaStream_t stream) {
     FE_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0 && nkv <= 65535, "paged_attention_kv4: bad head counts %d/%d", nq, nkv);
-    FE_REQUIRE(d >= 16 && d % 16 == 0 && d <= KV4_MAX_DIM, "paged_attention_kv4: head size %d; multiples of 16 up to %d", d, KV4_MAX_DIM);
-    FE_REQUIRE(ps > 0 && ps % KV4_TILE == 0 && num_pages > 0, "paged_attention_kv4: page size %d (a multiple of %d) or page count", ps, KV4_TILE);
+    FE_REQUIRE(head_size_ok(d), "paged_attention_kv4: head size %d; multiples of 16 up to %d", d, KV4_MAX_DIM);
+    FE_REQUIRE(ps > 0 && ps % KV4_TILE == 0 && num_pages > 0 && bt_stride > 0, "paged_attention_kv4: page size %d (a multiple of %d) or page count", ps, KV4_TILE);
     FE_REQUIRE(q_stride % 8 == 0 && (((size_t)q | (size_t)out | (size_t)cache) & 15) == 0, "paged_attention_kv4: rows must start on 16-byte boundaries");
     FE_REQUIRE(requests >= 0 && requests <= 65535 && max_q_len >= 0 && tokens >= 0, "paged_attention_kv4: bad request count or length");
     FE_REQUIRE(window >= 0 && keep >= 0 && (keep == 0 || window > 0), "paged_attention_kv4: a window is not negative, kept keys go with one");
-    FE_REQUIRE(splits >= 1 && splits <= MAX_SPLITS && (splits == 1 || (scratch && ((size_t)scratch & 15) == 0)), "paged_attention_kv4: %d splits", splits);
+    FE_REQUIRE(blocks >= 0 && (blocks == 0 || (max_q_len <= 1 && scratch && ((size_t)scratch & 15) == 0)), "paged_attention_kv4: %d blocks", blocks);
+    FE_REQUIRE((long long)num_pages * nkv * (ps / KV4_TILE) < (1LL << 31), "paged_attention_kv4: %d pages are too many", num_pages);
+    FE_REQUIRE(splits >= 1 && splits <= MAX_SPLITS && (splits == 1 || blocks == 0), "paged_attention_kv4: %d splits; 1 to %d", splits, MAX_SPLITS);
     FE_REQUIRE((long long)max_q_len * (nq / nkv) * splits < (1LL << 31) - 64, "paged_attention_kv4: grid too large");
-    if (requests == 0 || max_q_len == 0 || tokens == 0) return 0;
-    const Problem a{q, q_stride, out, out_stride, (const unsigned char*)cache, block_table, bt_stride, cu_q, q_start, nq, nkv, d, ps, num_pages,
-                    scale * LOG2E, window, keep, sink, splits, (float*)scratch, tokens, status};
+    FE_REQUIRE(blocks == 0 || (long long)requests * nkv * ((nq / nkv + 7) / 8) * bt_stride * (ps / KV4_TILE) < (1LL << 31), "paged_attention_kv4: too many tiles to share out");
     FE_REQUIRE(dtype == FE_F32 || dtype == FE_BF16, "paged_attention_kv4: unknown type %d", dtype);
-    const int rc = dtype == FE_F32 ? attend<float>(a, requests, max_q_len, stream) : attend<bf16>(a, requests, max_q_len, stream);
-    if (rc || splits == 1) return rc;
-    FE_REQUIRE(tokens * nq < (1LL << 31), "paged_attention_kv4: merge grid too large");
-    if (dtype == FE_F32)
-        fe::launch(kv4_merge_kernel<float>, dim3((unsigned)(tokens * nq)), 128, 0, stream, (const float*)scratch, (float*)out, out_stride, nq, d, splits, tokens * nq);
-    else
-        fe::launch(kv4_merge_kernel<bf16>, dim3((unsigned)(tokens * nq)), 128, 0, stream, (const float*)scratch, (bf16*)out, out_stride, nq, d, splits, tokens * nq);
-    return fe_check_launch("paged_attention_kv4 merge");
+    if (requests == 0 || max_q_len == 0 || tokens == 0) return 0;
+    const Problem a{q, q_stride, out, out_stride, (const unsigned char*)cache, block_table, bt_stride, cu_q, q_start, requests, nq, nkv, d, ps, num_pages,
+                    scale * LOG2E, window, keep, sink, splits, (float*)scratch, tokens, status};
+    const Launch w{&a, requests, (int)(((long long)max_q_len * (nq / nkv) + 7) / 8), blocks, stream};
+    return dtype == FE_F32 ? with_groups(d, [&](auto n) { return run<float, n.value, 1>(w); }) : with_groups(d, [&](auto n) { return run<bf16, n.value, 1>(w); });
 }

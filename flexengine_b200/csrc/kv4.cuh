@@ -35,20 +35,24 @@ __host__ __device__ constexpr int kv4_value_pairs(int groups) { return 576 * gro
 __device__ __forceinline__ int kv4_key_at(int g, int p, int groups) { return ((p >> 1) * groups + g) * 4 + (p & 1) * 2; }
 __device__ __forceinline__ int kv4_value_at(int g, int p, int groups) { return (p * groups + g) * 2; }
 
-// Eight codes of a word as four pairs of half-precision numbers code - 8: pair i holds the codes at bits 4 i and 16 + 4 i.  Four bits put
-// under the exponent of 1024 (or, four bits higher, of 64) are 1024 + code (64 + code); the subtraction is exact.
-__device__ __forceinline__ void kv4_decode(unsigned w, unsigned* out) {
-    const __half2 low = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));        // 1032
-    const __half2 high = __halves2half2(__ushort_as_half(0x5480), __ushort_as_half(0x5480));       // 72
+// Eight codes of a word as four pairs of half-precision numbers: pair i holds the codes at bits 4 i and 16 + 4 i, as KV4_RAISED_EVEN + code
+// (i even: four bits under the exponent of 1024) or KV4_RAISED_ODD + code (i odd: four bits higher, under that of 64).
+constexpr float KV4_RAISED_EVEN = 1024.f, KV4_RAISED_ODD = 64.f;
+__device__ __forceinline__ void kv4_raise(unsigned w, unsigned* out) {
     const unsigned v = w >> 8;
-    unsigned r[4];
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(r[0]) : "r"(w));
-    asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(r[1]) : "r"(w));
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(r[2]) : "r"(v));
-    asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(r[3]) : "r"(v));
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(out[0]) : "r"(w));
+    asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(out[1]) : "r"(w));
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(out[2]) : "r"(v));
+    asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(out[3]) : "r"(v));
+}
+// The same as code - 8; the subtraction is exact.
+__device__ __forceinline__ void kv4_decode(unsigned w, unsigned* out) {
+    const __half2 even = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));       // 1024 + 8
+    const __half2 odd = __halves2half2(__ushort_as_half(0x5480), __ushort_as_half(0x5480));        // 64 + 8
+    kv4_raise(w, out);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&r[i]), (i & 1) ? high : low);
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&out[i]), (i & 1) ? odd : even);
         out[i] = *reinterpret_cast<const unsigned*>(&h);
     }
 }

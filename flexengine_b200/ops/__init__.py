@@ -1755,7 +1755,7 @@ def sample_listed(logits, temperature, top_k, seed, draw):
 # ---- keys and values held in 4 bits (csrc/kv4.cuh has their form) -------------------------------------------------------
 KV4_TILE = 16            # tokens of a tile: page sizes of a 4-bit cache are multiples of it
 KV4_MAX_DIM = 256
-KV4_MAX_SPLITS = 64      # what the merge kernel takes (fe_kv4_attention_max_splits)
+KV4_FORCE = None
 
 
 def kv4_row_bytes(d: int) -> int:
@@ -1852,13 +1852,6 @@ def kv4_rows(cache, slots, nkv, d, page_size, dtype=torch.bfloat16):
     return keys, values
 
 
-def kv4_splits(blocks: int, keys: int, sms: int | None = None) -> int:
-    """Into how many blocks the keys of a row are shared out over a 4-bit cache; ``blocks``: column tiles x key/value heads."""
-    sms = sms or sm_count()
-    tiles = -(-keys // KV4_TILE)
-    return int(max(1, min(4 * sms // max(1, blocks), tiles // 8, KV4_MAX_SPLITS)))
-
-
 def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale, window=0, keep_first=0, sink=False):
     """``paged_attention`` over a 4-bit cache: causal grouped-query attention of the step's tokens over their requests' pages.  q [T, >= nq d],
     bfloat16 or float32, holds the turned queries in its first nq d columns; returns [T, nq d] of its type.  ``ctx``: the step
@@ -1878,18 +1871,19 @@ def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale
             raise ValueError(f"{what}: a window is not negative, and kept first keys go with one")
         if ctx.max_ctx_len > block_table.shape[1] * page_size:
             raise ValueError(f"{what}: {ctx.max_ctx_len} tokens in {block_table.shape[1]} pages of {page_size}")
-        columns = -(-ctx.max_q_len * (nq // nkv) // 8)
-        span = ctx.max_ctx_len if window == 0 else min(ctx.max_ctx_len, window + ctx.max_q_len + KV4_TILE + keep_first)
         out = torch.empty((T, nq * d), dtype=q.dtype, device=q.device)
-        lengths = getattr(ctx, "host_lengths", None)
-        tiles = sum(-(-n * (nq // nkv) // 8) for n in lengths) if lengths else columns * requests
-        splits = kv4_splits(tiles * nkv, span)
-        # of its own for every call: two streams, or two captured graphs, may be at it at once
-        nbytes = _kv4().fe_kv4_attention_scratch_bytes(T, nq, d, splits)
-        part = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _run(_kv4(), "fe_paged_attention_kv4", _ptr(q), q.stride(0) if T > 1 else nq * d, _ptr(out), nq * d, _ptr(cache), _ptr(block_table), block_table.shape[1],
+        lib, splits, blocks, part = _kv4(), 1, 0, None
+        if KV4_FORCE: splits, blocks = KV4_FORCE
+        elif ctx.max_q_len == 1:
+            span = ctx.max_ctx_len if window == 0 else min(ctx.max_ctx_len, window + keep_first + 2 * KV4_TILE)
+            plan = lib.fe_kv4_attention_plan(requests, -(-span // KV4_TILE), nq, nkv, d, _code(q.dtype))
+            splits, blocks = (1, plan) if plan > 0 else (-plan, 0)
+        if blocks:
+                # of its own for every call: two streams, or two captured graphs, may be at it at once
+                part = torch.empty(lib.fe_kv4_attention_scratch_bytes(blocks, requests, nq, nkv, d), dtype=torch.uint8, device=q.device)
+        _run(lib, "fe_paged_attention_kv4", _ptr(q), q.stride(0) if T > 1 else nq * d, _ptr(out), nq * d, _ptr(cache), _ptr(block_table), block_table.shape[1],
              _ptr(ctx.cu_q), _ptr(ctx.q_start), requests, T, ctx.max_q_len, nq, nkv, d, page_size, cache.shape[0], float(scale), window, keep_first,
-             1 if sink else 0, splits, _ptr(part), _code(q.dtype), _ptr(status_word(q.device)), _stream())
+             1 if sink else 0, splits, blocks, _ptr(part), _code(q.dtype), _ptr(status_word(q.device)), _stream())
     return out
 
 
