@@ -1,0 +1,787 @@
+// Drawing from logits with temperature, top-k, top-p and min-p, from given uniform numbers.
+//
+// x = logits / T.  Of a row's tokens, largest logit first and the lower index first among equals, the first k stay (k > 0); of their masses
+// e^(x - max) those stay before which less than top_p of the sum lies (top_p < 1; the first always stays); and of these the ones whose mass is at
+// least min_p of the largest.  The token is the first, in index order, at which the running sum of the masses that stayed passes u times their
+// sum.  T = 0: the lowest index of the maximum.  NaN counts as -inf.  Beside the token: its probability among those that stayed, and their number.
+//
+// Masses are whole numbers of 2^-44 of the largest (fewer bits over 2^18 tokens), so their sums are exact in any order: the result depends neither
+// on the number of blocks a row has nor on what else is in the batch.  Where tens of thousands of tokens stay, one is 1e-5 of the sum or
+// less, and a logit's distance to the maximum is therefore divided by T with what 32 bits lose kept beside it.
+//
+// A row belongs to a thread-block cluster, each block with a contiguous part of it.  Sorting is avoided.  A walk finds the maximum; a second one
+// counts the tokens (for top-k) and adds up their masses to 13 bits (for top-p) by their distance to the maximum, in 4,096 steps of 1/128.  In
+// the step at which the count or the mass passes its limit a few hundred tokens are left to be looked at one by one.  If that step and all
+// before it hold no more than LIST tokens (small k, peaked rows), they are listed and the rest of the work is done on the list, each token
+// against each other.  Else one more walk adds up exactly what lies before the step and lists the step itself; a step with more tokens than the list
+// takes (equal logits, as 16-bit ones often are) is taken apart by the bits of the logits.  A last walk adds up the masses that stay by
+// segments of the row, and the segment in which the target falls is gone through once more.
+#include <math_constants.h>
+
+#define FE_PDL_CLASS 8      // FE_PDL_SAMPLING
+#include "common.cuh"
+
+using namespace fe;
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int THREADS = 1024, WARPS = THREADS / 32;
+constexpr int SEGMENTS = 256;
+constexpr int MAX_CLUSTER = 8;
+constexpr int STEPS = 4096;
+constexpr float STEPS_A_UNIT = 128.f;
+constexpr float FARTHEST = 32.f;              // STEPS / STEPS_A_UNIT: a mass beyond is below 2^-46 of the largest
+constexpr int COARSE_BITS = 13;               // of a token's mass in the second walk, against that of its step
+constexpr int LIST = 2048;
+constexpr int BATCH = 5;                      // 16-byte loads of a lane on their way at once
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ unsigned peer_address(const void* own, unsigned rank) {
+    unsigned remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"((unsigned)__cvta_generic_to_shared(own)), "r"(rank));
+    return remote;
+}
+// the same variable in the shared memory of block ``rank`` of this cluster
+__device__ __forceinline__ unsigned ld_peer(const void* own, unsigned rank) {
+    unsigned v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(peer_address(own, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ u64 ld_peer64(const void* own, unsigned rank) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];\n" : "=l"(v) : "r"(peer_address(own, rank)) : "memory");
+    return v;
+}
+// order-preserving map from float to unsigned
+__device__ __forceinline__ unsigned ordered_key(float v) {
+    const unsigned b = __float_as_uint(v);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float sanitize(float v) { return v != v ? -CUDART_INF_F : v; }
+__device__ __forceinline__ u64 warp_sum64(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+struct Rows {
+    const float* logits;
+    long long ld;
+    int V;
+    const float* temperature;
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* uniform;
+    int* tokens;
+    float* probability;
+    int* kept;
+    int mass_bits;              // masses are whole numbers of 2^-mass_bits of the largest
+};
+
+struct Shared {
+    unsigned counts[STEPS], coarse[STEPS];             // tokens of a step, and their masses
+    unsigned list_key[LIST];                           // this block's
+    int list_index[LIST];
+    unsigned all_key[LIST];                            // the row's
+    int all_index[LIST];
+    u64 all_mass[LIST];
+    u64 all_before[LIST];                              // mass of the tokens before it, largest first
+    unsigned all_rank[LIST];
+    u64 fine[STEPS];                                   // exact masses where a step is taken apart
+    u64 segment_mass[SEGMENTS];                        // this block's segments first, later those of the row
+    int segment_ties[SEGMENTS], segment_kept[SEGMENTS];
+    u64 row_mass[SEGMENTS + 1];
+    int row_ties[SEGMENTS];
+    u64 warp_mass[WARPS];
+    unsigned warp_count[WARPS];
+    u64 own_mass, own_total;
+    unsigned own_count, own_low, own_high;
+    float own_max;
+    int own_index, listed;
+    u64 found_mass;
+    unsigned found_count;
+    int found_at;
+};
+
+// What a row's masses are made of.
+struct Mass {
+    float top, over, over_rest, scale;      // the maximum; 1 / T and what it lacks; 2^mass_bits
+    // distance to the maximum in units of T, and what is lost of it
+    __device__ __forceinline__ float distance(float v, float& rest) const {
+        if (v == top) { rest = 0.f; return 0.f; }              // infinite maxima too
+        const float gap = top - v;
+        const float lost = (top - gap) - v;                    // top - v = gap + lost, nearly always exactly
+        const float far = gap * over;
+        rest = fmaf(gap, over, -far) + fmaf(gap, over_rest, lost * over);
+        return far;
+    }
+    __device__ __forceinline__ u64 of(float far, float rest) const {
+        if (!(far < 100.f)) return 0;
+        const float e = expf(-far);
+        return __float2ull_rn(fmaf(-e, rest, e) * scale);
+    }
+    __device__ __forceinline__ u64 of(float v) const {
+        float rest;
+        const float far = distance(v, rest);
+        return of(far, rest);
+    }
+};
+__device__ __forceinline__ int step_of(float far) { return far < FARTHEST ? (int)(far * STEPS_A_UNIT) : STEPS; }
+
+template <typename F> __device__ __forceinline__ void over_segment(const float* x, int from, int to, bool vector, F f) {
+    const int lane = threadIdx.x & 31;
+    if (vector) {
+        for (int base = from; base < to; base += 128 * BATCH) {
+            float4 v[BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int i = base + 128 * u + 4 * lane;
+                if (i < to) v[u] = *reinterpret_cast<const float4*>(x + i);
+            }
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int i = base + 128 * u + 4 * lane;
+                if (i < to) { f(sanitize(v[u].x), i); f(sanitize(v[u].y), i + 1); f(sanitize(v[u].z), i + 2); f(sanitize(v[u].w), i + 3); }
+            }
+        }
+    } else {
+        for (int base = from; base < to; base += 32 * BATCH) {
+            float v[BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int i = base + 32 * u + lane;
+                if (i < to) v[u] = x[i];
+            }
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int i = base + 32 * u + lane;
+                if (i < to) f(sanitize(v[u]), i);
+            }
+        }
+    }
+}
+
+// Sums over the block; every thread gets the result.
+__device__ __forceinline__ u64 block_sum64(u64 v, Shared& s) {
+    v = warp_sum64(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s.warp_mass[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp_sum64(s.warp_mass[threadIdx.x & 31]);
+}
+__device__ __forceinline__ unsigned block_sum32(unsigned v, Shared& s) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s.warp_count[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, s.warp_count[threadIdx.x & 31]);
+}
+// What threads before this one hold; ``total`` what all do.
+__device__ __forceinline__ u64 block_before64(u64 v, u64& total, Shared& s) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u64 upto = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+    }
+    __syncthreads();
+    if (lane == 31) s.warp_mass[warp] = upto;
+    __syncthreads();
+    const u64 w = s.warp_mass[lane];
+    u64 all = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 up = __shfl_up_sync(0xffffffffu, all, o);
+        if (lane >= o) all += up;
+    }
+    total = __shfl_sync(0xffffffffu, all, 31);
+    return __shfl_sync(0xffffffffu, all - w, warp) + upto - v;
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+sample_filtered_kernel(const Rows of, const int C) {
+    griddep_wait();
+    griddep_launch_dependents();
+    extern __shared__ __align__(16) unsigned char raw[];
+    Shared& s = *reinterpret_cast<Shared*>(raw);
+    const int row = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const unsigned rank = blockIdx.x % C;
+    const float* x = of.logits + (long long)row * of.ld;
+    const int V = of.V, S = ((V + SEGMENTS - 1) / SEGMENTS + 31) / 32 * 32;
+    const int per_block = SEGMENTS / C, per_warp = per_block / WARPS, first_segment = (int)rank * per_block + warp * per_warp;
+    const bool vector = (V & 3) == 0 && ((size_t)x & 15) == 0;
+    // f(logit, index) over this block's part; a warp takes its segments one after the other
+    auto walk = [&](auto f) {
+        for (int j = 0; j < per_warp; ++j)
+            over_segment(x, min((long long)V, (long long)(first_segment + j) * S), min((long long)V, (long long)(first_segment + j + 1) * S), vector, f);
+    };
+
+    // ---- the maximum and its lowest index
+    float best = -CUDART_INF_F;
+    int best_at = 0x7fffffff;
+    walk([&](float v, int i) { if (v > best) { best = v; best_at = i; } });        // a lane meets its indices in rising order
+    auto take = [&](float v, int i) { if (v > best || (v == best && i < best_at)) { best = v; best_at = i; } };
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) take(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_at, o));
+    if (lane == 0) { s.warp_mass[warp] = (u64)__float_as_uint(best) << 32 | (unsigned)best_at; }
+    __syncthreads();
+    if (warp == 0) {
+        const u64 w = s.warp_mass[lane];
+        best = __uint_as_float((unsigned)(w >> 32));
+        best_at = (int)(unsigned)w;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) take(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_at, o));
+        if (lane == 0) { s.own_max = best; s.own_index = best_at; s.listed = 0; }
+    }
+    cluster_sync();
+    float top = -CUDART_INF_F;
+    int top_at = 0x7fffffff;
+    for (int c = 0; c < C; ++c) {
+        const float v = __uint_as_float(ld_peer(&s.own_max, c));
+        const int i = (int)ld_peer(&s.own_index, c);
+        if (v > top || (v == top && i < top_at)) { top = v; top_at = i; }
+    }
+    const float heat = of.temperature[row];
+    if (!(heat > 0.f) || top == -CUDART_INF_F) {
+        // greedy, or a row that leaves nothing: then the lowest index, with no probability
+        const bool none = top == -CUDART_INF_F;
+        if (rank == 0 && tid == 0) {
+            of.tokens[row] = none ? 0 : top_at;
+            of.probability[row] = none ? 0.f : 1.f;
+            of.kept[row] = none ? 0 : 1;
+        }
+        cluster_sync();                                    // no block leaves while another may still read its maximum
+        return;
+    }
+    Mass mass;
+    mass.top = top;
+    mass.over = 1.f / heat;
+    mass.over_rest = (float)(1.0 / (double)heat - (double)mass.over);
+    mass.scale = __uint_as_float((unsigned)(127 + of.mass_bits) << 23);
+    const int k = of.top_k[row];
+    const bool use_k = k > 0 && k < V;
+    const float p = fmaxf(of.top_p[row], 1e-30f), least = of.min_p[row];      // the first token always stays
+    const bool use_p = p < 1.f;
+    // min_p as a logit: mass >= min_p of the largest, so v >= top + T ln min_p, taken in 64 bits and rounded up
+    float low_logit = -CUDART_INF_F;
+    if (least > 0.f) low_logit = least >= 1.f ? top : isinf(top) ? top : __double2float_ru((double)top + (double)heat * log((double)least));
+
+    unsigned thr = 0, need = 0;                            // what stays: keys above thr, and the first ``need`` of those equal to it
+    bool all_ties = true;                                  // all that are equal to it
+    bool from_list = false;
+    // adds up a 64-bit and a 32-bit number over the cluster (s.own_mass and s.own_count are free)
+    auto cluster_sum = [&](u64 m, unsigned n, u64& all_m, unsigned& all_n) {
+        m = block_sum64(m, s);
+        n = block_sum32(n, s);
+        if (tid == 0) { s.own_mass = m; s.own_count = n; }
+        cluster_sync();
+        all_m = 0; all_n = 0;
+        for (int c = 0; c < C; ++c) { all_m += ld_peer64(&s.own_mass, c); all_n += ld_peer(&s.own_count, c); }
+        cluster_sync();
+    };
+
+    if (use_k || use_p) {
+        // ---- counts and masses by steps
+        for (int i = tid; i < STEPS; i += THREADS) { s.counts[i] = 0; s.coarse[i] = 0; }
+        __syncthreads();
+        u64 total = 0;
+        walk([&](float v, int) {
+            float rest;
+            const float far = mass.distance(v, rest);
+            const int step = step_of(far);
+            if (step >= STEPS) return;
+            if (use_k) atomicAdd(&s.counts[step], 1u);
+            if (use_p) {
+                // e^-(distance inside the step), the step 1/128 long: two terms of the series are good to 1e-7
+                const float in = far - (float)step * (1.f / STEPS_A_UNIT);
+                atomicAdd(&s.coarse[step], (unsigned)__float2int_rn((1.f - in * (1.f - 0.5f * in)) * (float)(1 << COARSE_BITS)));
+                total += mass.of(far, rest);
+            }
+        });
+        unsigned nothing;
+        cluster_sum(total, 0u, total, nothing);            // the barrier inside: every block's steps are there
+        // the row's steps, four a thread; the same in every block
+        unsigned count[4];
+        u64 coarse[4], own_coarse = 0;
+        u64 own_count = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int step = 4 * tid + e;
+            count[e] = 0;
+            u64 sum = 0;
+            for (int c = 0; c < C; ++c) {
+                if (use_k) count[e] += ld_peer(&s.counts[step], c);
+                if (use_p) sum += ld_peer(&s.coarse[step], c);
+            }
+            coarse[e] = use_p ? __float2ull_rn((float)sum * expf(-(float)step * (1.f / STEPS_A_UNIT)) * 65536.f) : 0;
+            own_count += count[e];
+            own_coarse += coarse[e];
+        }
+        u64 all_count, all_coarse;
+        const u64 count_before = block_before64(own_count, all_count, s);
+        const u64 coarse_before = block_before64(own_coarse, all_coarse, s);
+        // the first step at which a running sum reaches ``limit``, the last one that holds anything if none does
+        auto step_at = [&](const auto* each, u64 before, u64 all, double limit) {
+            if (tid == 0) s.found_at = -1;
+            __syncthreads();
+            u64 run = before;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const u64 upto = run + each[e];
+                if (each[e] > 0 && (double)run < limit && ((double)upto >= limit || upto == all)) s.found_at = 4 * tid + e;
+                run = upto;
+            }
+            __syncthreads();
+            const int at = s.found_at;
+            __syncthreads();
+            return at;
+        };
+        auto listed_up_to = [&](int step) {                // tokens up to the step, from the counts
+            if (tid == step / 4) {
+                u64 run = count_before;
+                for (int e = 0; e <= step % 4; ++e) run += count[e];
+                s.found_mass = run;
+            }
+            __syncthreads();
+            const u64 n = s.found_mass;
+            __syncthreads();
+            return n;
+        };
+        // Puts the tokens of steps [from, to] into the row's list, in every block; false when they do not fit.  ``above`` and ``above_count``:
+        // exact sums of the steps before, ``low`` and ``high`` the least and the greatest key in them.
+        u64 above = 0;
+        unsigned above_count = 0, low = 0, high = 0;
+        int n = 0;
+        auto list = [&](int from, int to) {
+            if (tid == 0) s.listed = 0;
+            __syncthreads();
+            u64 m = 0;
+            unsigned cnt = 0, least_key = 0xffffffffu, most_key = 0;
+            walk([&](float v, int i) {
+                float rest;
+                const float far = mass.distance(v, rest);
+                const int step = step_of(far);
+                if (step > to) return;
+                if (step < from) { m += mass.of(far, rest); ++cnt; return; }
+                const unsigned key = ordered_key(v);
+                least_key = min(least_key, key);
+                most_key = max(most_key, key);
+                const int at = atomicAdd(&s.listed, 1);
+                if (at < LIST) { s.list_key[at] = key; s.list_index[at] = i; }
+            });
+            least_key = __reduce_min_sync(0xffffffffu, least_key);
+            most_key = __reduce_max_sync(0xffffffffu, most_key);
+            if (tid == 0) { s.own_low = 0xffffffffu; s.own_high = 0; }
+            __syncthreads();
+            if (lane == 0) { atomicMin(&s.own_low, least_key); atomicMax(&s.own_high, most_key); }
+            cluster_sum(m, cnt, above, above_count);       // barriers inside: lists and keys are there
+            int total_listed = 0;
+            low = 0xffffffffu; high = 0;
+            for (int c = 0; c < C; ++c) {
+                const int here = (int)ld_peer(&s.listed, c);
+                low = min(low, ld_peer(&s.own_low, c));
+                high = max(high, ld_peer(&s.own_high, c));
+                for (int i = tid; i < here && total_listed + i < LIST && i < LIST; i += THREADS) {
+                    s.all_key[total_listed + i] = ld_peer(&s.list_key[i], c);
+                    s.all_index[total_listed + i] = (int)ld_peer(&s.list_index[i], c);
+                }
+                total_listed += here;
+            }
+            n = total_listed;
+            cluster_sync();                                // the peers' lists are read
+            return n <= LIST;
+        };
+        auto logit_of = [](unsigned key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key); };
+        // Every listed token's mass, its place and the mass before it, largest first and the lower index first among equals.
+        auto rank_list = [&]() {
+            for (int i = tid; i < n; i += THREADS) s.all_mass[i] = mass.of(logit_of(s.all_key[i]));
+            __syncthreads();
+            for (int i = tid; i < n; i += THREADS) {
+                const unsigned key = s.all_key[i];
+                const int index = s.all_index[i];
+                u64 before = 0;
+                unsigned place = 0;
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) {
+                    const bool ahead = s.all_key[j] > key || (s.all_key[j] == key && s.all_index[j] < index);
+                    before += ahead ? s.all_mass[j] : 0;
+                    place += ahead;
+                }
+                s.all_before[i] = before;
+                s.all_rank[i] = place;
+            }
+            __syncthreads();
+        };
+
+        const int step_k = use_k ? step_at(count, count_before, all_count, (double)k) : -1;
+        const int step_p = use_p && !use_k ? step_at(coarse, coarse_before, all_coarse, (double)p * (double)all_coarse) : -1;
+        // where k reaches beyond the last step, the long way takes what lies there as one step more
+        const bool k_bites = use_k && all_count >= (u64)k;
+        // whether everything up to the limit's step may fit the list: known from the counts, or (top-p alone) likely from the masses
+        bool fits = false;
+        int last = -1;
+        if (k_bites) { last = step_k; fits = listed_up_to(step_k) <= LIST; }
+        else if (use_p && !use_k) {
+            // a step's tokens have nearly the same mass: its number of them is its coarse mass over the full one
+            u64 own = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (4 * tid + e <= step_p) {
+                    u64 sum = 0;
+                    for (int c = 0; c < C; ++c) sum += ld_peer(&s.coarse[4 * tid + e], c);
+                    own += sum;
+                }
+            last = step_p;
+            fits = (block_sum64(own, s) >> COARSE_BITS) < LIST - LIST / 16;
+        }
+        cluster_sync();                                    // the peers' steps are read: they may be overwritten
+        if (fits && list(0, last)) {
+            rank_list();
+            // what stays of the list: rank below k, less than p of the sum before it
+            u64 mine = 0;
+            for (int i = tid; i < n; i += THREADS)
+                if (!k_bites || s.all_rank[i] < (unsigned)k) mine += s.all_mass[i];
+            const u64 sum = k_bites ? block_sum64(mine, s) : total;
+            const double limit = (double)p * (double)sum;
+            // the coarse sums may have chosen a step too early: the list then does not reach the limit, and the long way is taken
+            const u64 in_list = block_sum64(mine, s);
+            from_list = k_bites || (double)in_list >= limit;
+            if (from_list) {
+                u64 kept_mass = 0;
+                unsigned kept_count = 0;
+                for (int i = tid; i < n; i += THREADS) {
+                    const bool stays = (!k_bites || s.all_rank[i] < (unsigned)k) && (!use_p || s.all_rank[i] == 0 || (double)s.all_before[i] < limit) &&
+                                       logit_of(s.all_key[i]) >= low_logit;
+                    if (!stays) s.all_mass[i] = 0;
+                    else { kept_mass += s.all_mass[i]; ++kept_count; }
+                }
+                kept_mass = block_sum64(kept_mass, s);
+                kept_count = block_sum32(kept_count, s);
+                if (rank == 0) {
+                    const float u = of.uniform[row];
+                    double target = (u > 0.f ? (double)fminf(u, 1.f) : 0.0) * (double)kept_mass;
+                    if (target >= (double)kept_mass) target = nextafter((double)kept_mass, 0.0);
+                    if (tid == 0) s.found_at = 0;
+                    __syncthreads();
+                    for (int i = tid; i < n; i += THREADS) {
+                        const u64 own = s.all_mass[i];
+                        if (own == 0) continue;
+                        const int index = s.all_index[i];
+                        u64 before = 0;
+#pragma unroll 4
+                        for (int j = 0; j < n; ++j) before += s.all_index[j] < index ? s.all_mass[j] : 0;
+                        if ((double)before <= target && target < (double)(before + own)) s.found_at = i;
+                    }
+                    __syncthreads();
+                    if (tid == 0) {
+                        of.tokens[row] = s.all_index[s.found_at];
+                        of.probability[row] = (float)((double)s.all_mass[s.found_at] / (double)kept_mass);
+                        of.kept[row] = (int)kept_count;
+                    }
+                }
+                return;                                    // no block reads another's memory any more
+            }
+        }
+        // ---- the long way: one limit after the other, each an exact cut (thr, need)
+        // ``limit`` in tokens or in mass; ``at``: the step that is likely to hold it
+        auto cut = [&](bool by_mass, double limit, int at) {
+            while (true) {
+                const bool whole = list(at, at);
+                // what the step holds in all
+                u64 here_mass = 0;
+                if (whole) {
+                    u64 mine = 0;
+                    for (int i = tid; i < n; i += THREADS) mine += mass.of(logit_of(s.all_key[i]));
+                    here_mass = block_sum64(mine, s);
+                } else {
+                    u64 mine = 0;
+                    unsigned nothing_more;
+                    walk([&](float v, int) {
+                        float rest;
+                        const float far = mass.distance(v, rest);
+                        if (step_of(far) == at) mine += mass.of(far, rest);
+                    });
+                    cluster_sum(mine, 0u, here_mass, nothing_more);
+                }
+                const double before = by_mass ? (double)above : (double)above_count, here = by_mass ? (double)here_mass : (double)n;
+                // the coarse sums may be a step off
+                if (before >= limit && at > 0 && above_count > 0) { --at; continue; }
+                if (before + here < limit && at + 1 < STEPS) { ++at; continue; }
+                if (whole) {
+                    rank_list();
+                    // the last that stays: the one of highest place among those before which less than the limit lies
+                    if (tid == 0) s.found_count = 0;
+                    __syncthreads();
+                    for (int i = tid; i < n; i += THREADS) {
+                        const double ahead = by_mass ? (double)(above + s.all_before[i]) : (double)(above_count + s.all_rank[i]);
+                        if (ahead < limit || (above_count == 0 && s.all_rank[i] == 0)) atomicMax(&s.found_count, s.all_rank[i]);
+                    }
+                    __syncthreads();
+                    const unsigned place = s.found_count;
+                    for (int i = tid; i < n; i += THREADS)
+                        if (s.all_rank[i] == place) s.found_at = (int)s.all_key[i];
+                    __syncthreads();
+                    thr = (unsigned)s.found_at;
+                    unsigned stay = 0, ties = 0;
+                    u64 sum = 0;
+                    for (int i = tid; i < n; i += THREADS) {
+                        ties += s.all_key[i] == thr;
+                        stay += s.all_key[i] == thr && s.all_rank[i] <= place;
+                        if (s.all_rank[i] <= place) sum += s.all_mass[i];
+                    }
+                    need = block_sum32(stay, s);
+                    all_ties = need == block_sum32(ties, s);
+                    return above + block_sum64(sum, s);
+                }
+                // too many for the list: by the bits of the keys, until one key is left
+                unsigned from = low, upto = high;
+                u64 run = above;
+                u64 run_count = above_count;
+                while (from < upto) {
+                    int shift = 0;
+                    while (((upto - from) >> shift) >= (unsigned)STEPS) ++shift;
+                    for (int i = tid; i < STEPS; i += THREADS) { s.counts[i] = 0; s.fine[i] = 0; }
+                    __syncthreads();
+                    walk([&](float v, int) {
+                        float rest;
+                        const float far = mass.distance(v, rest);
+                        if (step_of(far) != at) return;
+                        const unsigned key = ordered_key(v);
+                        if (key < from || key > upto) return;
+                        const int bin = (int)((upto - key) >> shift);          // largest first
+                        atomicAdd(&s.counts[bin], 1u);
+                        atomicAdd(&s.fine[bin], mass.of(far, rest));
+                    });
+                    cluster_sync();
+                    u64 m[4], cnt[4], own_m = 0, own_n = 0, total_m, total_n;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        m[e] = cnt[e] = 0;
+                        for (int c = 0; c < C; ++c) { m[e] += ld_peer64(&s.fine[4 * tid + e], c); cnt[e] += ld_peer(&s.counts[4 * tid + e], c); }
+                        own_m += m[e];
+                        own_n += cnt[e];
+                    }
+                    u64 bm = run + block_before64(own_m, total_m, s), bn = run_count + block_before64(own_n, total_n, s);
+                    if (tid == 0) s.found_at = -1;
+                    __syncthreads();
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const double b = by_mass ? (double)bm : (double)bn, a = by_mass ? (double)(bm + m[e]) : (double)(bn + cnt[e]);
+                        // the bin at which the limit is reached; the first that holds anything where nothing may come before it; the last of all
+                        if (cnt[e] > 0 && (b < limit || bn == 0) && (a >= limit || bn + cnt[e] == run_count + total_n)) {
+                            s.found_at = 4 * tid + e;
+                            s.found_mass = bm;
+                            s.found_count = (unsigned)bn;
+                        }
+                        bm += m[e];
+                        bn += cnt[e];
+                    }
+                    __syncthreads();
+                    const int bin = s.found_at;
+                    run = s.found_mass;
+                    run_count = s.found_count;
+                    cluster_sync();                        // the peers' bins are read
+                    const unsigned above_key = (unsigned)bin << shift;
+                    const unsigned new_upto = upto - above_key, width = (1u << shift) - 1u;
+                    from = new_upto - from < width ? from : new_upto - width;
+                    upto = new_upto;
+                }
+                thr = from;
+                unsigned ties = 0;
+                walk([&](float v, int) { ties += ordered_key(v) == thr; });
+                u64 nothing64;
+                cluster_sum(0, ties, nothing64, ties);
+                const u64 each = mass.of(logit_of(thr));
+                if (by_mass) {
+                    // the fewest with which the limit is reached, and one at least where nothing comes before
+                    const double more = each > 0 ? ceil((limit - (double)run) / (double)each) : 1.0;
+                    unsigned want = more < 1.0 ? 1u : more > (double)ties ? ties : (unsigned)more;
+                    while (want > 1 && (double)(run + (u64)(want - 1) * each) >= limit) --want;
+                    while (want < ties && (double)(run + (u64)want * each) < limit) ++want;
+                    need = want;
+                } else
+                    need = min(ties, (unsigned)(u64)(limit - (double)run_count));
+                all_ties = need == ties;
+                return run + (u64)need * each;
+            }
+        };
+        u64 within = total;                                // top-p alone: of all
+        if (use_k) within = cut(false, (double)k, k_bites ? step_k : STEPS);
+        if (use_p) {
+            const double limit = (double)p * (double)within;
+            // the step by the coarse sums, against the exact sum where top-k has cut them
+            const double unit = all_coarse > 0 && total > 0 ? (double)all_coarse / (double)total : 0.0;
+            const int at = step_at(coarse, coarse_before, all_coarse, limit * unit);
+            cut(true, limit, at < 0 ? 0 : at);
+        }
+    }
+
+    // ---- what stays, by segments of the row
+    if (!all_ties) {
+        for (int j = 0; j < per_warp; ++j) {
+            unsigned ties = 0;
+            over_segment(x, min((long long)V, (long long)(first_segment + j) * S), min((long long)V, (long long)(first_segment + j + 1) * S), vector,
+                         [&](float v, int) { ties += ordered_key(v) == thr; });
+            ties = __reduce_add_sync(0xffffffffu, ties);
+            if (lane == 0) s.segment_ties[warp * per_warp + j] = (int)ties;
+        }
+        cluster_sync();
+        u64 before = 0, nothing;
+        if (tid < SEGMENTS) before = ld_peer(&s.segment_ties[tid % per_block], tid / per_block);
+        before = block_before64(before, nothing, s);
+        if (tid < SEGMENTS) s.row_ties[tid] = (int)min(before, (u64)0x7fffffff);
+        cluster_sync();
+    }
+    // Whether a token stays; ``seen``: ties before it.  Only where ties are cut does their order count, and then 32 tokens at a time are taken in order.
+    auto segment_sums = [&](int segment, u64& sum, unsigned& number, auto each) {
+        const int from = (int)min((long long)V, (long long)segment * S), to = (int)min((long long)V, (long long)(segment + 1) * S);
+        sum = 0;
+        number = 0;
+        if (all_ties) {
+            over_segment(x, from, to, vector, [&](float v, int i) {
+                if (ordered_key(v) < thr || v < low_logit) return;
+                const u64 m = mass.of(v);
+                sum += m;
+                // as many as have a probability at all, however small: e^-x in 64 bits is above zero up to 745
+                float rest;
+                number += mass.distance(v, rest) < 745.f;
+                each(m, i);
+            });
+        } else {
+            unsigned seen = (unsigned)s.row_ties[segment];
+            for (int base = from; base < to; base += 32) {
+                const int i = base + lane;
+                const float v = i < to ? sanitize(x[i]) : -CUDART_INF_F;
+                const unsigned key = ordered_key(v), tied = __ballot_sync(0xffffffffu, i < to && key == thr);
+                const unsigned place = seen + __popc(tied & ((1u << lane) - 1u));
+                seen += __popc(tied);
+                if (i < to && (key > thr || (key == thr && place < need)) && v >= low_logit) {
+                    const u64 m = mass.of(v);
+                    sum += m;
+                    ++number;
+                    each(m, i);
+                }
+            }
+        }
+    };
+    unsigned number_all = 0;
+    for (int j = 0; j < per_warp; ++j) {
+        u64 sum;
+        unsigned number;
+        segment_sums(first_segment + j, sum, number, [](u64, int) {});
+        sum = warp_sum64(sum);
+        number_all += number;
+        if (lane == 0) s.segment_mass[warp * per_warp + j] = sum;
+    }
+    number_all = block_sum32(number_all, s);
+    if (tid == 0) s.own_count = number_all;
+    cluster_sync();
+    u64 mine = 0, total;
+    if (tid < SEGMENTS) mine = ld_peer64(&s.segment_mass[tid % per_block], tid / per_block);
+    const u64 before = block_before64(mine, total, s);
+    if (tid < SEGMENTS) s.row_mass[tid] = before;
+    if (tid == 0) s.row_mass[SEGMENTS] = total;
+    number_all = 0;
+    for (int c = 0; c < C; ++c) number_all += ld_peer(&s.own_count, c);
+    __syncthreads();
+    cluster_sync();                                        // the others' sums are read: they may leave
+    const float u = of.uniform[row];
+    double target = (u > 0.f ? (double)fminf(u, 1.f) : 0.0) * (double)total;
+    if (target >= (double)total) target = nextafter((double)total, 0.0);
+    for (int j = 0; j < per_warp; ++j) {
+        const int segment = first_segment + j;
+        if (!((double)s.row_mass[segment] <= target && target < (double)s.row_mass[segment + 1])) continue;
+        // one warp of the row: its segment in index order, 32 tokens at a time
+        const int from = (int)min((long long)V, (long long)segment * S), to = (int)min((long long)V, (long long)(segment + 1) * S);
+        u64 run = s.row_mass[segment];
+        unsigned seen = all_ties ? 0u : (unsigned)s.row_ties[segment];
+        for (int base = from; base < to; base += 32) {
+            const int i = base + lane;
+            const float v = i < to ? sanitize(x[i]) : -CUDART_INF_F;
+            const unsigned key = ordered_key(v), tied = __ballot_sync(0xffffffffu, i < to && key == thr);
+            const unsigned place = seen + __popc(tied & ((1u << lane) - 1u));
+            seen += __popc(tied);
+            const bool stays = i < to && (key > thr || (key == thr && (all_ties || place < need))) && v >= low_logit;
+            const u64 m = stays ? mass.of(v) : 0;
+            u64 upto = m;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 up = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += up;
+            }
+            if (m > 0 && (double)(run + upto - m) <= target && target < (double)(run + upto)) {
+                of.tokens[row] = i;
+                of.probability[row] = (float)((double)m / (double)total);
+                of.kept[row] = (int)number_all;
+            }
+            run += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+}
+
+// How many clusters of ``blocks`` blocks of the kernel the device holds at once; asked of the driver once per size and device.
+int clusters_resident(int blocks) {
+    static int cached[64][4];
+    int device = 0, slot = blocks == 8 ? 3 : blocks == 4 ? 2 : blocks == 2 ? 1 : 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 0;
+    if (cached[device][slot] == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)blocks);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = sizeof(Shared);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = blocks;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, sample_filtered_kernel, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            clusters = 0;
+        }
+        cached[device][slot] = clusters > 0 ? clusters : -1;
+    }
+    return cached[device][slot] > 0 ? cached[device][slot] : 0;
+}
+
+}  // namespace
+
+// ``blocks``: how many share a row (1, 2, 4 or 8); 0: the most that still lets every row's cluster be resident at once.  The results do not depend on it.
+extern "C" int fe_sample_filtered(const float* logits, long long ld, int R, int V, const float* temperature, const int* top_k, const float* top_p,
+                                  const float* min_p, const float* uniform, int* tokens, float* probability, int* kept, int blocks, cudaStream_t stream) {
+    FE_REQUIRE(R >= 0 && V > 0 && ld >= V, "sample_filtered: bad sizes R=%d V=%d ld=%lld", R, V, ld);
+    FE_REQUIRE(V < (1 << 19) && (long long)R * MAX_CLUSTER < (1LL << 31), "sample_filtered: %d rows of %d logits; fewer than 2^19 logits and 2^28 rows", R, V);      // a step's coarse mass is 32 bits
+    FE_REQUIRE(blocks == 0 || blocks == 1 || blocks == 2 || blocks == 4 || blocks == 8, "sample_filtered: %d blocks a row; 1, 2, 4 or 8", blocks);
+    if (R == 0) return 0;
+    const cudaError_t set = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
+    FE_REQUIRE(set == cudaSuccess, "sample_filtered: %s", cudaGetErrorString(set));
+    if (blocks == 0)
+        for (blocks = MAX_CLUSTER; blocks > 1 && R > clusters_resident(blocks);) blocks >>= 1;
+    int bits = 0;
+    while ((1LL << bits) < V) ++bits;
+    const Rows of{logits, ld, V, temperature, top_k, top_p, min_p, uniform, tokens, probability, kept, bits <= 18 ? 44 : 62 - bits};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(R * blocks));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = sizeof(Shared);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = blocks;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, sample_filtered_kernel, of, blocks);
+    FE_REQUIRE(err == cudaSuccess, "sample_filtered (clusters of %d): %s", blocks, cudaGetErrorString(err));
+    return fe_check_launch("sample_filtered");
+}

@@ -1752,6 +1752,29 @@ def sample_listed(logits, temperature, top_k, seed, draw):
     return out
 
 
+def sample_filtered(logits, temperature, top_k, top_p, min_p, uniform, blocks: int = 0):
+    """One token per row of float32 logits [R, V] with temperature, top-k, top-p and min-p, drawn with given numbers: (tokens int32, their
+    probabilities among the tokens that stayed float32, the number of those int32), all [R].  ``temperature``, ``top_p``, ``min_p`` and ``uniform``
+    float32, ``top_k`` int32, all [R]: temperature 0 takes the lowest index of the maximum; of the others top_k > 0 keeps the first so many (largest
+    logit first, the lower index first among equals), top_p < 1 of these as few as hold that share of their mass, min_p > 0 of these what
+    has that share of the largest one's mass; ``uniform`` in [0, 1) picks by the running sum in index order.  See csrc/sampling_filtered.cu.
+    ``blocks``: how many thread blocks (1, 2, 4 or 8) share a row, 0 for the library's choice; the results do not depend on it."""
+    what = "sample_filtered"
+    with _on(what, logits, temperature, top_k, top_p, min_p, uniform):
+        R, V = logits.shape
+        if logits.dtype != torch.float32 or logits.stride(1) != 1:
+            raise TypeError(f"{what}: logits must be float32 with unit column stride")
+        for name, t, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                               ("min_p", min_p, torch.float32), ("uniform", uniform, torch.float32)):
+            if t.dtype != dtype or t.numel() != R or not t.is_contiguous():
+                raise TypeError(f"{what}: {name} is contiguous {dtype} [{R}]")
+        tokens, kept = (torch.empty(R, dtype=torch.int32, device=logits.device) for _ in range(2))
+        probability = torch.empty(R, dtype=torch.float32, device=logits.device)
+        _run(_core(), "fe_sample_filtered", _ptr(logits), logits.stride(0) if R > 1 else V, R, V, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+             _ptr(uniform), _ptr(tokens), _ptr(probability), _ptr(kept), blocks, _stream())
+    return tokens, probability, kept
+
+
 # ---- keys and values held in 4 bits (csrc/kv4.cuh has their form) -------------------------------------------------------
 KV4_TILE = 16            # tokens of a tile: page sizes of a 4-bit cache are multiples of it
 KV4_MAX_DIM = 256
