@@ -57,6 +57,11 @@ __device__ __forceinline__ u64 ld_peer64(const void* own, unsigned rank) {
     asm volatile("ld.shared::cluster.u64 %0, [%1];\n" : "=l"(v) : "r"(peer_address(own, rank)) : "memory");
     return v;
 }
+__device__ __forceinline__ uint4 ld_peer4(const void* own, unsigned rank) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(peer_address(own, rank)) : "memory");
+    return v;
+}
 // order-preserving map from float to unsigned
 __device__ __forceinline__ unsigned ordered_key(float v) {
     const unsigned b = __float_as_uint(v);
@@ -86,21 +91,18 @@ struct Rows {
 
 struct Shared {
     unsigned counts[STEPS], coarse[STEPS];             // tokens of a step, and their masses
-    unsigned list_key[LIST];                           // this block's
-    int list_index[LIST];
-    unsigned all_key[LIST];                            // the row's
-    int all_index[LIST];
-    u64 all_mass[LIST];
-    u64 all_before[LIST];                              // mass of the tokens before it, largest first
-    unsigned all_rank[LIST];
     u64 fine[STEPS];                                   // exact masses where a step is taken apart
-    u64 segment_mass[SEGMENTS];                        // this block's segments first, later those of the row
-    int segment_ties[SEGMENTS], segment_kept[SEGMENTS];
+    u64 list[LIST];                                    // this block's: ordered key turned over, then the index
+    u64 all[LIST];                                     // the row's; sorted: the largest logit first, the lower index first among equals
+    u64 all_mass[LIST];
+    u64 all_before[LIST];                              // mass of the tokens before it
+    u64 segment_mass[SEGMENTS];                        // this block's segments
+    int segment_ties[SEGMENTS];
     u64 row_mass[SEGMENTS + 1];
     int row_ties[SEGMENTS];
     u64 warp_mass[WARPS];
     unsigned warp_count[WARPS];
-    u64 own_mass, own_total;
+    u64 own_mass;
     unsigned own_count, own_low, own_high;
     float own_max;
     int own_index, listed;
@@ -205,6 +207,24 @@ __device__ __forceinline__ u64 block_before64(u64 v, u64& total, Shared& s) {
     return __shfl_sync(0xffffffffu, all - w, warp) + upto - v;
 }
 
+// Sorts a[0 .. n) upwards, n <= LIST (a bitonic network over the next power of two; places from n on are taken as the largest).
+__device__ __forceinline__ void sort_list(u64* a, int n) {
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += THREADS) a[i] = ~0ull;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const int i = (threadIdx.x & ~(j - 1)) * 2 + (threadIdx.x & (j - 1));      // LIST / 2 threads' worth of pairs
+            if (i + j < size) {
+                const u64 x = a[i], y = a[i + j];
+                if ((x > y) == ((i & k) == 0)) { a[i] = y; a[i + j] = x; }
+            }
+            __syncthreads();
+        }
+}
+static_assert(LIST == 2 * THREADS, "a pair a thread");
+
 __global__ void __launch_bounds__(THREADS, 1)
 sample_filtered_kernel(const Rows of, const int C) {
     griddep_wait();
@@ -217,10 +237,26 @@ sample_filtered_kernel(const Rows of, const int C) {
     const int V = of.V, S = ((V + SEGMENTS - 1) / SEGMENTS + 31) / 32 * 32;
     const int per_block = SEGMENTS / C, per_warp = per_block / WARPS, first_segment = (int)rank * per_block + warp * per_warp;
     const bool vector = (V & 3) == 0 && ((size_t)x & 15) == 0;
+    bool by_segments = false;                              // the segments' sums are there already
+    unsigned number_all = 0;                               // this thread's tokens that stay
     // f(logit, index) over this block's part; a warp takes its segments one after the other
     auto walk = [&](auto f) {
         for (int j = 0; j < per_warp; ++j)
             over_segment(x, min((long long)V, (long long)(first_segment + j) * S), min((long long)V, (long long)(first_segment + j + 1) * S), vector, f);
+    };
+
+    struct Sums { u64 mass; unsigned number; };
+    // the same; f(logit, index, sums) adds up what stays, a segment at a time
+    auto walk_segments = [&](auto f) {
+        number_all = 0;
+        for (int j = 0; j < per_warp; ++j) {
+            Sums here{0, 0};
+            over_segment(x, min((long long)V, (long long)(first_segment + j) * S), min((long long)V, (long long)(first_segment + j + 1) * S), vector,
+                         [&](float v, int i) { f(v, i, here); });
+            here.mass = warp_sum64(here.mass);
+            if (lane == 0) s.segment_mass[warp * per_warp + j] = here.mass;
+            number_all += here.number;
+        }
     };
 
     // ---- the maximum and its lowest index
@@ -241,13 +277,12 @@ sample_filtered_kernel(const Rows of, const int C) {
         if (lane == 0) { s.own_max = best; s.own_index = best_at; s.listed = 0; }
     }
     cluster_sync();
-    float top = -CUDART_INF_F;
-    int top_at = 0x7fffffff;
-    for (int c = 0; c < C; ++c) {
-        const float v = __uint_as_float(ld_peer(&s.own_max, c));
-        const int i = (int)ld_peer(&s.own_index, c);
-        if (v > top || (v == top && i < top_at)) { top = v; top_at = i; }
-    }
+    best = lane < C ? __uint_as_float(ld_peer(&s.own_max, lane)) : -CUDART_INF_F;      // a lane a block: one trip, not one after the other
+    best_at = lane < C ? (int)ld_peer(&s.own_index, lane) : 0x7fffffff;
+#pragma unroll
+    for (int o = MAX_CLUSTER / 2; o > 0; o >>= 1) take(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_at, o));
+    const float top = __shfl_sync(0xffffffffu, best, 0);
+    const int top_at = __shfl_sync(0xffffffffu, best_at, 0);
     const float heat = of.temperature[row];
     if (!(heat > 0.f) || top == -CUDART_INF_F) {
         // greedy, or a row that leaves nothing: then the lowest index, with no probability
@@ -275,15 +310,14 @@ sample_filtered_kernel(const Rows of, const int C) {
 
     unsigned thr = 0, need = 0;                            // what stays: keys above thr, and the first ``need`` of those equal to it
     bool all_ties = true;                                  // all that are equal to it
-    bool from_list = false;
     // adds up a 64-bit and a 32-bit number over the cluster (s.own_mass and s.own_count are free)
     auto cluster_sum = [&](u64 m, unsigned n, u64& all_m, unsigned& all_n) {
         m = block_sum64(m, s);
         n = block_sum32(n, s);
         if (tid == 0) { s.own_mass = m; s.own_count = n; }
         cluster_sync();
-        all_m = 0; all_n = 0;
-        for (int c = 0; c < C; ++c) { all_m += ld_peer64(&s.own_mass, c); all_n += ld_peer(&s.own_count, c); }
+        all_m = warp_sum64(lane < C ? ld_peer64(&s.own_mass, lane) : 0);
+        all_n = __reduce_add_sync(0xffffffffu, lane < C ? ld_peer(&s.own_count, lane) : 0);
         cluster_sync();
     };
 
@@ -309,19 +343,26 @@ sample_filtered_kernel(const Rows of, const int C) {
         cluster_sum(total, 0u, total, nothing);            // the barrier inside: every block's steps are there
         // the row's steps, four a thread; the same in every block
         unsigned count[4];
-        u64 coarse[4], own_coarse = 0;
+        u64 coarse[4], flat[4], own_coarse = 0;           // flat: as if every token of a step weighed the same
         u64 own_count = 0;
+        auto all_blocks = [&](const unsigned* own, u64* sum) {         // of four steps; all blocks' are asked for at once
+            uint4 v[MAX_CLUSTER];
+#pragma unroll
+            for (int c = 0; c < MAX_CLUSTER; ++c) v[c] = c < C ? ld_peer4(own, c) : make_uint4(0, 0, 0, 0);
+            sum[0] = sum[1] = sum[2] = sum[3] = 0;
+#pragma unroll
+            for (int c = 0; c < MAX_CLUSTER; ++c) { sum[0] += v[c].x; sum[1] += v[c].y; sum[2] += v[c].z; sum[3] += v[c].w; }
+        };
+        {
+            u64 sum[4] = {0, 0, 0, 0};
+            if (use_k) all_blocks(&s.counts[4 * tid], sum);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { count[e] = (unsigned)sum[e]; own_count += sum[e]; flat[e] = 0; }
+        }
+        if (use_p) all_blocks(&s.coarse[4 * tid], flat);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int step = 4 * tid + e;
-            count[e] = 0;
-            u64 sum = 0;
-            for (int c = 0; c < C; ++c) {
-                if (use_k) count[e] += ld_peer(&s.counts[step], c);
-                if (use_p) sum += ld_peer(&s.coarse[step], c);
-            }
-            coarse[e] = use_p ? __float2ull_rn((float)sum * expf(-(float)step * (1.f / STEPS_A_UNIT)) * 65536.f) : 0;
-            own_count += count[e];
+            coarse[e] = use_p ? __float2ull_rn((float)flat[e] * expf(-(float)(4 * tid + e) * (1.f / STEPS_A_UNIT)) * 65536.f) : 0;
             own_coarse += coarse[e];
         }
         u64 all_count, all_coarse;
@@ -364,17 +405,23 @@ sample_filtered_kernel(const Rows of, const int C) {
             __syncthreads();
             u64 m = 0;
             unsigned cnt = 0, least_key = 0xffffffffu, most_key = 0;
-            walk([&](float v, int i) {
+            walk_segments([&](float v, int i, Sums& here) {
                 float rest;
                 const float far = mass.distance(v, rest);
                 const int step = step_of(far);
                 if (step > to) return;
-                if (step < from) { m += mass.of(far, rest); ++cnt; return; }
+                if (step < from) {
+                    const u64 own = mass.of(far, rest);
+                    m += own;
+                    ++cnt;
+                    if (v >= low_logit) { here.mass += own; ++here.number; }
+                    return;
+                }
                 const unsigned key = ordered_key(v);
                 least_key = min(least_key, key);
                 most_key = max(most_key, key);
                 const int at = atomicAdd(&s.listed, 1);
-                if (at < LIST) { s.list_key[at] = key; s.list_index[at] = i; }
+                if (at < LIST) s.list[at] = (u64)~key << 32 | (unsigned)i;
             });
             least_key = __reduce_min_sync(0xffffffffu, least_key);
             most_key = __reduce_max_sync(0xffffffffu, most_key);
@@ -382,41 +429,43 @@ sample_filtered_kernel(const Rows of, const int C) {
             __syncthreads();
             if (lane == 0) { atomicMin(&s.own_low, least_key); atomicMax(&s.own_high, most_key); }
             cluster_sum(m, cnt, above, above_count);       // barriers inside: lists and keys are there
-            int total_listed = 0;
-            low = 0xffffffffu; high = 0;
-            for (int c = 0; c < C; ++c) {
-                const int here = (int)ld_peer(&s.listed, c);
-                low = min(low, ld_peer(&s.own_low, c));
-                high = max(high, ld_peer(&s.own_high, c));
-                for (int i = tid; i < here && total_listed + i < LIST && i < LIST; i += THREADS) {
-                    s.all_key[total_listed + i] = ld_peer(&s.list_key[i], c);
-                    s.all_index[total_listed + i] = (int)ld_peer(&s.list_index[i], c);
+            int here = lane < C ? (int)ld_peer(&s.listed, lane) : 0, upto = here;
+            low = __reduce_min_sync(0xffffffffu, lane < C ? ld_peer(&s.own_low, lane) : 0xffffffffu);
+            high = __reduce_max_sync(0xffffffffu, lane < C ? ld_peer(&s.own_high, lane) : 0u);
+#pragma unroll
+            for (int o = 1; o < MAX_CLUSTER; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += up;
+            }
+            const int total_listed = __shfl_sync(0xffffffffu, upto, C - 1);
+            if (total_listed <= LIST) {
+                // entry i of the row is of the block in whose share of the running sums it lies
+                const int most = (total_listed + 31) & ~31;
+                for (int i = tid; i < most; i += THREADS) {
+                    int block = 0, first = 0;
+#pragma unroll
+                    for (int c = 0; c < MAX_CLUSTER - 1; ++c) {
+                        const int end = __shfl_sync(0xffffffffu, upto, c);
+                        if (c < C - 1 && i >= end) { block = c + 1; first = end; }
+                    }
+                    if (i < total_listed) s.all[i] = ld_peer64(&s.list[i - first], block);
                 }
-                total_listed += here;
             }
             n = total_listed;
             cluster_sync();                                // the peers' lists are read
             return n <= LIST;
         };
+        auto key_of = [](u64 entry) { return ~(unsigned)(entry >> 32); };
         auto logit_of = [](unsigned key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key); };
-        // Every listed token's mass, its place and the mass before it, largest first and the lower index first among equals.
+        // The list in order, every token's mass and the mass before it.
         auto rank_list = [&]() {
-            for (int i = tid; i < n; i += THREADS) s.all_mass[i] = mass.of(logit_of(s.all_key[i]));
-            __syncthreads();
-            for (int i = tid; i < n; i += THREADS) {
-                const unsigned key = s.all_key[i];
-                const int index = s.all_index[i];
-                u64 before = 0;
-                unsigned place = 0;
-#pragma unroll 4
-                for (int j = 0; j < n; ++j) {
-                    const bool ahead = s.all_key[j] > key || (s.all_key[j] == key && s.all_index[j] < index);
-                    before += ahead ? s.all_mass[j] : 0;
-                    place += ahead;
-                }
-                s.all_before[i] = before;
-                s.all_rank[i] = place;
-            }
+            sort_list(s.all, n);
+            u64 m[2], nothing64;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) m[e] = 2 * tid + e < n ? mass.of(logit_of(key_of(s.all[2 * tid + e]))) : 0;
+            const u64 before = block_before64(m[0] + m[1], nothing64, s);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) { s.all_mass[2 * tid + e] = m[e]; s.all_before[2 * tid + e] = before + (e ? m[0] : 0); }
             __syncthreads();
         };
 
@@ -433,57 +482,47 @@ sample_filtered_kernel(const Rows of, const int C) {
             u64 own = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (4 * tid + e <= step_p) {
-                    u64 sum = 0;
-                    for (int c = 0; c < C; ++c) sum += ld_peer(&s.coarse[4 * tid + e], c);
-                    own += sum;
-                }
+                if (4 * tid + e <= step_p) own += flat[e];
             last = step_p;
             fits = (block_sum64(own, s) >> COARSE_BITS) < LIST - LIST / 16;
         }
         cluster_sync();                                    // the peers' steps are read: they may be overwritten
         if (fits && list(0, last)) {
             rank_list();
-            // what stays of the list: rank below k, less than p of the sum before it
-            u64 mine = 0;
-            for (int i = tid; i < n; i += THREADS)
-                if (!k_bites || s.all_rank[i] < (unsigned)k) mine += s.all_mass[i];
-            const u64 sum = k_bites ? block_sum64(mine, s) : total;
+            // what stays of the list: a place below k, less than p of the sum before it
+            const int reach = k_bites ? k : n;             // the list holds k tokens at least
+            const u64 in_list = s.all_before[reach - 1] + s.all_mass[reach - 1], sum = k_bites ? in_list : total;
             const double limit = (double)p * (double)sum;
             // the coarse sums may have chosen a step too early: the list then does not reach the limit, and the long way is taken
-            const u64 in_list = block_sum64(mine, s);
-            from_list = k_bites || (double)in_list >= limit;
-            if (from_list) {
+            if (k_bites || (double)in_list >= limit) {
                 u64 kept_mass = 0;
                 unsigned kept_count = 0;
                 for (int i = tid; i < n; i += THREADS) {
-                    const bool stays = (!k_bites || s.all_rank[i] < (unsigned)k) && (!use_p || s.all_rank[i] == 0 || (double)s.all_before[i] < limit) &&
-                                       logit_of(s.all_key[i]) >= low_logit;
-                    if (!stays) s.all_mass[i] = 0;
-                    else { kept_mass += s.all_mass[i]; ++kept_count; }
+                    const bool stays = i < reach && (!use_p || i == 0 || (double)s.all_before[i] < limit) && logit_of(key_of(s.all[i])) >= low_logit;
+                    if (stays) { kept_mass += s.all_mass[i]; ++kept_count; }
                 }
                 kept_mass = block_sum64(kept_mass, s);
-                kept_count = block_sum32(kept_count, s);
+                kept_count = block_sum32(kept_count, s);   // a token stays with all that are ahead of it: the first so many
                 if (rank == 0) {
+                    // the tokens that stay by index, each with its place
+                    for (int i = tid; i < (int)kept_count; i += THREADS) s.list[i] = s.all[i] << 32 | (unsigned)i;
+                    __syncthreads();
+                    sort_list(s.list, (int)kept_count);
+                    u64 m[2], nothing64;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) m[e] = 2 * tid + e < (int)kept_count ? s.all_mass[(unsigned)s.list[2 * tid + e]] : 0;
+                    u64 before = block_before64(m[0] + m[1], nothing64, s);
                     const float u = of.uniform[row];
                     double target = (u > 0.f ? (double)fminf(u, 1.f) : 0.0) * (double)kept_mass;
                     if (target >= (double)kept_mass) target = nextafter((double)kept_mass, 0.0);
-                    if (tid == 0) s.found_at = 0;
-                    __syncthreads();
-                    for (int i = tid; i < n; i += THREADS) {
-                        const u64 own = s.all_mass[i];
-                        if (own == 0) continue;
-                        const int index = s.all_index[i];
-                        u64 before = 0;
-#pragma unroll 4
-                        for (int j = 0; j < n; ++j) before += s.all_index[j] < index ? s.all_mass[j] : 0;
-                        if ((double)before <= target && target < (double)(before + own)) s.found_at = i;
-                    }
-                    __syncthreads();
-                    if (tid == 0) {
-                        of.tokens[row] = s.all_index[s.found_at];
-                        of.probability[row] = (float)((double)s.all_mass[s.found_at] / (double)kept_mass);
-                        of.kept[row] = (int)kept_count;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (m[e] > 0 && (double)before <= target && target < (double)(before + m[e])) {
+                            of.tokens[row] = (int)(s.list[2 * tid + e] >> 32);
+                            of.probability[row] = (float)((double)m[e] / (double)kept_mass);
+                            of.kept[row] = (int)kept_count;
+                        }
+                        before += m[e];
                     }
                 }
                 return;                                    // no block reads another's memory any more
@@ -491,15 +530,15 @@ sample_filtered_kernel(const Rows of, const int C) {
         }
         // ---- the long way: one limit after the other, each an exact cut (thr, need)
         // ``limit`` in tokens or in mass; ``at``: the step that is likely to hold it
+        u64 last_entry = 0;                                // of the last cut: the last listed token that stays
         auto cut = [&](bool by_mass, double limit, int at) {
             while (true) {
-                const bool whole = list(at, at);
+                const bool whole = by_segments = list(at, at);
                 // what the step holds in all
                 u64 here_mass = 0;
                 if (whole) {
-                    u64 mine = 0;
-                    for (int i = tid; i < n; i += THREADS) mine += mass.of(logit_of(s.all_key[i]));
-                    here_mass = block_sum64(mine, s);
+                    rank_list();
+                    here_mass = n > 0 ? s.all_before[n - 1] + s.all_mass[n - 1] : 0;
                 } else {
                     u64 mine = 0;
                     unsigned nothing_more;
@@ -515,30 +554,23 @@ sample_filtered_kernel(const Rows of, const int C) {
                 if (before >= limit && at > 0 && above_count > 0) { --at; continue; }
                 if (before + here < limit && at + 1 < STEPS) { ++at; continue; }
                 if (whole) {
-                    rank_list();
-                    // the last that stays: the one of highest place among those before which less than the limit lies
+                    // the last that stays: the one of highest place before which less than the limit lies
                     if (tid == 0) s.found_count = 0;
                     __syncthreads();
                     for (int i = tid; i < n; i += THREADS) {
-                        const double ahead = by_mass ? (double)(above + s.all_before[i]) : (double)(above_count + s.all_rank[i]);
-                        if (ahead < limit || (above_count == 0 && s.all_rank[i] == 0)) atomicMax(&s.found_count, s.all_rank[i]);
+                        const double ahead = by_mass ? (double)(above + s.all_before[i]) : (double)((u64)above_count + i);
+                        if (ahead < limit) atomicMax(&s.found_count, (unsigned)i);
                     }
                     __syncthreads();
-                    const unsigned place = s.found_count;
-                    for (int i = tid; i < n; i += THREADS)
-                        if (s.all_rank[i] == place) s.found_at = (int)s.all_key[i];
-                    __syncthreads();
-                    thr = (unsigned)s.found_at;
+                    const int place = (int)s.found_count;
+                    thr = key_of(s.all[place]);
                     unsigned stay = 0, ties = 0;
-                    u64 sum = 0;
-                    for (int i = tid; i < n; i += THREADS) {
-                        ties += s.all_key[i] == thr;
-                        stay += s.all_key[i] == thr && s.all_rank[i] <= place;
-                        if (s.all_rank[i] <= place) sum += s.all_mass[i];
-                    }
+                    for (int i = tid; i < n; i += THREADS)
+                        if (key_of(s.all[i]) == thr) { ++ties; stay += i <= place; }
                     need = block_sum32(stay, s);
                     all_ties = need == block_sum32(ties, s);
-                    return above + block_sum64(sum, s);
+                    last_entry = s.all[place];
+                    return above + s.all_before[place] + s.all_mass[place];
                 }
                 // too many for the list: by the bits of the keys, until one key is left
                 unsigned from = low, upto = high;
@@ -561,10 +593,11 @@ sample_filtered_kernel(const Rows of, const int C) {
                     });
                     cluster_sync();
                     u64 m[4], cnt[4], own_m = 0, own_n = 0, total_m, total_n;
+                    all_blocks(&s.counts[4 * tid], cnt);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        m[e] = cnt[e] = 0;
-                        for (int c = 0; c < C; ++c) { m[e] += ld_peer64(&s.fine[4 * tid + e], c); cnt[e] += ld_peer(&s.counts[4 * tid + e], c); }
+                        m[e] = 0;
+                        for (int c = 0; c < C; ++c) m[e] += ld_peer64(&s.fine[4 * tid + e], c);
                         own_m += m[e];
                         own_n += cnt[e];
                     }
@@ -594,6 +627,7 @@ sample_filtered_kernel(const Rows of, const int C) {
                     upto = new_upto;
                 }
                 thr = from;
+                by_segments = false;
                 unsigned ties = 0;
                 walk([&](float v, int) { ties += ordered_key(v) == thr; });
                 u64 nothing64;
@@ -621,9 +655,21 @@ sample_filtered_kernel(const Rows of, const int C) {
             const int at = step_at(coarse, coarse_before, all_coarse, limit * unit);
             cut(true, limit, at < 0 ? 0 : at);
         }
+        if (by_segments) {
+            // the segments hold what lies before the last cut's step: the tokens of the step that stay come to it, each block's own
+            __syncthreads();
+            for (int i = tid; i < s.listed; i += THREADS) {
+                const u64 entry = s.list[i];
+                const float v = logit_of(key_of(entry));
+                if (entry > last_entry || v < low_logit) continue;
+                atomicAdd(&s.segment_mass[(int)(unsigned)entry / S - (int)rank * per_block], mass.of(v));
+                float rest;
+                number_all += mass.distance(v, rest) < 745.f;
+            }
+        }
     }
 
-    // ---- what stays, by segments of the row
+    // ---- what stays, by segments of the row.  Only where ties are cut does their order count.
     if (!all_ties) {
         for (int j = 0; j < per_warp; ++j) {
             unsigned ties = 0;
@@ -636,49 +682,43 @@ sample_filtered_kernel(const Rows of, const int C) {
         u64 before = 0, nothing;
         if (tid < SEGMENTS) before = ld_peer(&s.segment_ties[tid % per_block], tid / per_block);
         before = block_before64(before, nothing, s);
-        if (tid < SEGMENTS) s.row_ties[tid] = (int)min(before, (u64)0x7fffffff);
+        if (tid < SEGMENTS) s.row_ties[tid] = (int)before;
         cluster_sync();
     }
-    // Whether a token stays; ``seen``: ties before it.  Only where ties are cut does their order count, and then 32 tokens at a time are taken in order.
-    auto segment_sums = [&](int segment, u64& sum, unsigned& number, auto each) {
-        const int from = (int)min((long long)V, (long long)segment * S), to = (int)min((long long)V, (long long)(segment + 1) * S);
-        sum = 0;
-        number = 0;
-        if (all_ties) {
-            over_segment(x, from, to, vector, [&](float v, int i) {
+    if (!by_segments) {
+        if (all_ties)
+            walk_segments([&](float v, int, Sums& here) {
                 if (ordered_key(v) < thr || v < low_logit) return;
-                const u64 m = mass.of(v);
-                sum += m;
                 // as many as have a probability at all, however small: e^-x in 64 bits is above zero up to 745
                 float rest;
-                number += mass.distance(v, rest) < 745.f;
-                each(m, i);
+                const float far = mass.distance(v, rest);
+                here.mass += mass.of(far, rest);
+                here.number += far < 745.f;
             });
-        } else {
-            unsigned seen = (unsigned)s.row_ties[segment];
-            for (int base = from; base < to; base += 32) {
-                const int i = base + lane;
-                const float v = i < to ? sanitize(x[i]) : -CUDART_INF_F;
-                const unsigned key = ordered_key(v), tied = __ballot_sync(0xffffffffu, i < to && key == thr);
-                const unsigned place = seen + __popc(tied & ((1u << lane) - 1u));
-                seen += __popc(tied);
-                if (i < to && (key > thr || (key == thr && place < need)) && v >= low_logit) {
-                    const u64 m = mass.of(v);
-                    sum += m;
-                    ++number;
-                    each(m, i);
+        else {
+            number_all = 0;
+            for (int j = 0; j < per_warp; ++j) {           // 32 tokens at a time, in order
+                const int segment = first_segment + j;
+                const int from = (int)min((long long)V, (long long)segment * S), to = (int)min((long long)V, (long long)(segment + 1) * S);
+                unsigned seen = (unsigned)s.row_ties[segment];
+                u64 sum = 0;
+                for (int base = from; base < to; base += 32) {
+                    const int i = base + lane;
+                    const float v = i < to ? sanitize(x[i]) : -CUDART_INF_F;
+                    const unsigned key = ordered_key(v), tied = __ballot_sync(0xffffffffu, i < to && key == thr);
+                    const unsigned place = seen + __popc(tied & ((1u << lane) - 1u));
+                    seen += __popc(tied);
+                    if (i < to && (key > thr || (key == thr && place < need)) && v >= low_logit) {
+                        float rest;
+                        const float far = mass.distance(v, rest);
+                        sum += mass.of(far, rest);
+                        number_all += far < 745.f;
+                    }
                 }
+                sum = warp_sum64(sum);
+                if (lane == 0) s.segment_mass[warp * per_warp + j] = sum;
             }
         }
-    };
-    unsigned number_all = 0;
-    for (int j = 0; j < per_warp; ++j) {
-        u64 sum;
-        unsigned number;
-        segment_sums(first_segment + j, sum, number, [](u64, int) {});
-        sum = warp_sum64(sum);
-        number_all += number;
-        if (lane == 0) s.segment_mass[warp * per_warp + j] = sum;
     }
     number_all = block_sum32(number_all, s);
     if (tid == 0) s.own_count = number_all;
@@ -688,8 +728,7 @@ sample_filtered_kernel(const Rows of, const int C) {
     const u64 before = block_before64(mine, total, s);
     if (tid < SEGMENTS) s.row_mass[tid] = before;
     if (tid == 0) s.row_mass[SEGMENTS] = total;
-    number_all = 0;
-    for (int c = 0; c < C; ++c) number_all += ld_peer(&s.own_count, c);
+    number_all = __reduce_add_sync(0xffffffffu, lane < C ? ld_peer(&s.own_count, lane) : 0);
     __syncthreads();
     cluster_sync();                                        // the others' sums are read: they may leave
     const float u = of.uniform[row];
