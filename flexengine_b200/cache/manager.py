@@ -11,7 +11,8 @@ chunk group, once the window or the chunk of the next token has passed them.  ``
 
 Storage of a paged group: ``[slots, planes, pages, kv_heads, page_size, head_dim]`` (keys at
 index 0, values at 1; a group of one plane keeps a single vector per token that serves as both), so one
-(page, head) tile is contiguous.
+(page, head) tile is contiguous.  A group held in 4 bits (``kv_cache_dtype`` "int4"): uint8 ``[slots, pages, kv_heads,
+page_size / 16, bytes of a tile of 16 tokens]``, keys and values of a tile in one piece (csrc/kv4.cuh).
 """
 from __future__ import annotations
 
@@ -25,6 +26,21 @@ import torch
 from .page_pool import CacheExhausted, PagePool
 
 RELEASED = -1      # block-table entry of a page that a window has passed
+KV4_TILE = 16      # tokens of a tile of a 4-bit cache: its pages hold a multiple of it
+
+
+def kv4_row_bytes(head_dim: int) -> int:
+    """Bytes of one token's key and value of one head in 4 bits: groups of 32 numbers, 16 bytes of codes and 4 of (scale, centre) each."""
+    if head_dim % 16 or not 16 <= head_dim <= 256:
+        raise ValueError(f"head size {head_dim}: a 4-bit cache takes multiples of 16 from 16 to 256")
+    return 40 * -(-head_dim // 32)
+
+
+def kv4_shape(pages: int, kv_heads: int, page_size: int, head_dim: int) -> tuple:
+    """The shape of a 4-bit cache of ``pages`` pages, a uint8 tensor."""
+    if page_size < KV4_TILE or page_size % KV4_TILE:
+        raise ValueError(f"page size {page_size}: pages of a 4-bit cache hold a multiple of {KV4_TILE} tokens")
+    return (pages, kv_heads, page_size // KV4_TILE, KV4_TILE * kv4_row_bytes(head_dim))
 
 
 @dataclass
@@ -37,13 +53,18 @@ class RequestCache:
 
 
 class PagedGroup:
-    def __init__(self, spec, num_pages: int, page_size: int, dtype, device, max_requests: int = 1):
+    def __init__(self, spec, num_pages: int, page_size: int, dtype, device, max_requests: int = 1, four_bit: bool = False):
         self.spec = spec
+        self.four_bit = bool(four_bit)
         self.page_size = int(page_size)
         self.pool = PagePool(num_pages)
         self.planes = int(getattr(spec, "planes", 2))
-        self.storage = torch.zeros((spec.slots, self.planes, num_pages, spec.kv_heads, self.page_size, spec.head_dim),
-                                   dtype=dtype, device=device)
+        if self.four_bit:
+            self.storage = torch.zeros((spec.slots,) + kv4_shape(num_pages, spec.kv_heads, self.page_size, spec.head_dim),
+                                       dtype=torch.uint8, device=device)
+        else:
+            self.storage = torch.zeros((spec.slots, self.planes, num_pages, spec.kv_heads, self.page_size, spec.head_dim),
+                                       dtype=dtype, device=device)
         # the block tables once more, as one matrix with a row per seat (a request's state slot): what a step's
         # metadata is gathered from with a few array operations instead of a loop over requests and pages
         self.table_rows = np.full((max_requests, 64), RELEASED, dtype=np.int32)
@@ -61,9 +82,13 @@ class PagedGroup:
         self.table_rows[seat, first:] = RELEASED
 
     def kv_slot(self, slot: int):
+        if self.four_bit:
+            raise TypeError(f"group {self.spec.name!r} is held in 4 bits: its slots have no key and value planes")
         return self.storage[slot, 0], self.storage[slot, self.planes - 1]
 
     def bytes_per_token(self) -> int:
+        if self.four_bit:
+            return self.spec.slots * self.spec.kv_heads * kv4_row_bytes(self.spec.head_dim)
         return self.planes * self.spec.slots * self.spec.kv_heads * self.spec.head_dim * self.storage.element_size()
 
 
@@ -76,10 +101,14 @@ class StateGroup:
 
 class CacheManager:
     def __init__(self, group_specs, num_pages, page_size: int, max_requests: int, dtype=torch.float32,
-                 device="cpu"):
+                 device="cpu", kv_cache_dtype: str = "auto"):
         """``num_pages``: pages per paged group (an int for all, or a list per group).  ``page_size``: tokens a
         page for groups whose spec names none.  An int ``num_pages`` is meant for pages of that default size: a
-        group with another page size gets as many pages as hold the same number of tokens."""
+        group with another page size gets as many pages as hold the same number of tokens.  ``kv_cache_dtype`` "int4":
+        every paged group keeps its keys and values in 4 bits (the engine asks the model's mixers first)."""
+        if kv_cache_dtype not in ("auto", "int4"):
+            raise ValueError(f"unknown kv_cache_dtype {kv_cache_dtype!r}")
+        self.kv_cache_dtype = kv_cache_dtype
         self.page_size = int(page_size)
         self.max_requests = int(max_requests)
         self.device = torch.device(device)
@@ -95,7 +124,7 @@ class CacheManager:
                     n = num_pages[gi]
                 else:
                     n = -(-num_pages * self.page_size // own)
-                self.groups.append(PagedGroup(spec, n, own, dtype, self.device, self.max_requests))
+                self.groups.append(PagedGroup(spec, n, own, dtype, self.device, self.max_requests, kv_cache_dtype == "int4"))
         self.requests: dict[str, RequestCache] = {}
         self.free_state_slots = list(range(self.max_requests - 1, -1, -1))
         self._paged = [(gi, g) for gi, g in enumerate(self.groups) if isinstance(g, PagedGroup)]

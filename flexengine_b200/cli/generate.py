@@ -5,7 +5,7 @@ Engine options carry the reference's names and meanings (src/flexengine/serving/
 --max-model-len, --max-num-seqs, --trace-dir, --[no-]cuda-graph; like there, each one
 overrides the matching ``FLEX_*`` variable (src/flexengine/engine/config.py:64-86).
 Sampling options are those of a request (src/flexengine/engine/runtime.py:89): --max-tokens,
---temperature, --top-k, --seed.
+--temperature, --top-k, --seed; --top-p, --min-p and --kv-cache-dtype have no counterpart there.
 """
 from __future__ import annotations
 
@@ -25,6 +25,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--max-tokens", type=int, default=128)
     p.add_argument("--temperature", type=float, default=0.0)
     p.add_argument("--top-k", type=int, default=0)
+    p.add_argument("--top-p", type=float, default=1.0)
+    p.add_argument("--min-p", type=float, default=0.0)
     p.add_argument("--seed", type=int, default=None)
     p.add_argument("--dtype", choices=["bfloat16", "bf16", "float32", "fp32"], default=None)
     p.add_argument("--device", default=None)
@@ -34,6 +36,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--prefill-chunk-size", type=int, default=None)
     p.add_argument("--block-size", type=int, default=None)
     p.add_argument("--num-blocks", type=int, default=None)
+    p.add_argument("--kv-cache-dtype", choices=["auto", "int4"], default=None, help="int4: keys and values in 4 bits")
     p.add_argument("--max-model-len", type=int, default=None)
     p.add_argument("--max-num-seqs", type=int, default=None)
     p.add_argument("--cuda-graph", action=argparse.BooleanOptionalAction, default=None)
@@ -46,7 +49,7 @@ def engine_config_from_args(args):
         model=args.model, dtype=args.dtype, device=args.device, scheduler_policy=args.policy,
         trace_dir=args.trace_dir, max_num_batched_tokens=args.token_budget,
         prefill_chunk_size=args.prefill_chunk_size, kv_block_size=args.block_size, kv_num_blocks=args.num_blocks,
-        max_model_len=args.max_model_len, max_num_seqs=args.max_num_seqs, cuda_graph=args.cuda_graph)
+        max_model_len=args.max_model_len, max_num_seqs=args.max_num_seqs, cuda_graph=args.cuda_graph, kv_cache_dtype=args.kv_cache_dtype)
 
 
 def load_tokenizer(model_dir: str):
@@ -92,7 +95,7 @@ def main(argv=None) -> int:
         _typed, _plan, model = load_model(args.model, config.dtype, config.device)
     engine = Engine.from_model(model, config, tokenizer=tokenizer)
     outputs = engine.generate(prompts, max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k,
-                              seed=args.seed)
+                              seed=args.seed, top_p=args.top_p, min_p=args.min_p)
     for out in outputs:
         print(json.dumps({"request_id": out.request_id, "prompt_tokens": len(out.prompt_ids),
                           "token_ids": out.token_ids, "text": out.text, "finish_reason": out.finish_reason}))

@@ -5,7 +5,9 @@ Names, defaults and checks follow the reference's EngineConfig
 (config.py:64-86).  ``attention_backend`` and ``rmsnorm_backend`` are gone (there is
 one kernel path); ``dtype`` is "bfloat16" or "float32"; ``kv_num_blocks=0`` sizes the
 pool from free device memory; ``overlap_steps`` (no counterpart in the reference) lets the
-host plan and launch a step while the device still runs the one before.
+host plan and launch a step while the device still runs the one before; ``kv_cache_dtype`` (none either):
+"auto" keeps keys and values in the compute dtype, "int4" in 4 bits with a scale and a centre per 32
+numbers (5 bits a number: 3.2 times as many tokens as bfloat16 in the same memory).
 """
 from __future__ import annotations
 
@@ -13,6 +15,8 @@ import os
 from dataclasses import dataclass, fields, replace
 
 POLICIES = ("fcfs", "decode_first", "slo_aware", "adaptive")
+KV_CACHE_DTYPES = ("auto", "int4")
+KV4_PAGE_STEP = 16                 # pages of a 4-bit cache hold a multiple of this many tokens
 DTYPES = {"bfloat16": "bfloat16", "bf16": "bfloat16", "float32": "float32", "fp32": "float32"}
 
 
@@ -39,6 +43,7 @@ class EngineConfig:
     trace_steps: bool = True
     max_output_tokens: int = 512
     random_seed: int = 42
+    kv_cache_dtype: str = "auto"       # "int4": keys and values in 4 bits
 
     def __post_init__(self) -> None:
         for name in ("max_model_len", "max_num_seqs", "max_num_batched_tokens", "prefill_chunk_size",
@@ -51,6 +56,10 @@ class EngineConfig:
             raise ValueError("max_waiting must be nonnegative")
         if self.scheduler_policy not in POLICIES:
             raise ValueError("Unknown scheduler_policy")
+        if self.kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ValueError(f"Unknown kv_cache_dtype {self.kv_cache_dtype!r}; expected one of {list(KV_CACHE_DTYPES)}")
+        if self.kv_cache_dtype == "int4" and self.kv_block_size % KV4_PAGE_STEP:
+            raise ValueError(f"kv_block_size={self.kv_block_size}: pages of a 4-bit cache hold a multiple of {KV4_PAGE_STEP} tokens")
         if self.dtype not in DTYPES:
             raise ValueError(f"Unknown dtype {self.dtype!r}; expected one of {sorted(DTYPES)}")
         object.__setattr__(self, "dtype", DTYPES[self.dtype])

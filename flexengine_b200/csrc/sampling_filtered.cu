@@ -7,7 +7,7 @@
 //
 // Masses are whole numbers of 2^-44 of the largest (fewer bits over 2^18 tokens), so their sums are exact in any order: the result depends neither
 // on the number of blocks a row has nor on what else is in the batch.  Where tens of thousands of tokens stay, one is 1e-5 of the sum or
-// less, and a logit's distance to the maximum is therefore divided by T with what 32 bits lose kept beside it.
+// less, and equal ones share their error, so masses are taken in 64 bits.
 //
 // A row belongs to a thread-block cluster, each block with a contiguous part of it.  Sorting is avoided.  A walk finds the maximum; a second one
 // counts the tokens (for top-k) and adds up their masses to 13 bits (for top-p) by their distance to the maximum, in 4,096 steps of 1/128.  In
@@ -67,7 +67,7 @@ __device__ __forceinline__ unsigned ordered_key(float v) {
     const unsigned b = __float_as_uint(v);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float sanitize(float v) { return v != v ? -CUDART_INF_F : v; }
+__device__ __forceinline__ float sanitize(float v) { return v != v ? -CUDART_INF_F : v + 0.f; }      // -0 and 0 are equal: one key
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -89,6 +89,8 @@ struct Rows {
     int mass_bits;              // masses are whole numbers of 2^-mass_bits of the largest
 };
 
+constexpr int ROOTS = 16;                     // 2^(-i / 16) in a table
+
 struct Shared {
     unsigned counts[STEPS], coarse[STEPS];             // tokens of a step, and their masses
     u64 fine[STEPS];                                   // exact masses where a step is taken apart
@@ -109,29 +111,37 @@ struct Shared {
     u64 found_mass;
     unsigned found_count;
     int found_at;
+    double roots[ROOTS];
 };
 
-// What a row's masses are made of.
+// What a row's masses are made of.  A mass is a whole number that is right to 2^-42 of itself: where logits are equal, as 16-bit ones often are,
+// thousands of tokens have the same one, and an error of a 32-bit exponential would come thousands of times.  e^-x = 2^-y is
+// taken with a table of the 16th roots and a polynomial between them (Tang's table-driven exponential): y 16 = n + r, |r| <= 1/2, and with
+// h = r ln 2 / 16 <= 0.022 the Taylor polynomial of e^-h to the fifth power leaves out less than h^6 / 720 = 2^-42.  Fourteen operations in 64
+// bits, of which an SM does 64 a clock.
 struct Mass {
-    float top, over, over_rest, scale;      // the maximum; 1 / T and what it lacks; 2^mass_bits
-    // distance to the maximum in units of T, and what is lost of it
-    __device__ __forceinline__ float distance(float v, float& rest) const {
-        if (v == top) { rest = 0.f; return 0.f; }              // infinite maxima too
-        const float gap = top - v;
-        const float lost = (top - gap) - v;                    // top - v = gap + lost, nearly always exactly
-        const float far = gap * over;
-        rest = fmaf(gap, over, -far) + fmaf(gap, over_rest, lost * over);
-        return far;
-    }
-    __device__ __forceinline__ u64 of(float far, float rest) const {
-        if (!(far < 100.f)) return 0;
-        const float e = expf(-far);
-        return __float2ull_rn(fmaf(-e, rest, e) * scale);
-    }
+    float top, over;                         // the maximum, 1 / T
+    double steps;                            // 16 log2(e) / T
+    int bits;
+    const double* roots;                     // shared memory
+    __device__ __forceinline__ float distance(float v) const { return v == top ? 0.f : (top - v) * over; }      // infinite maxima too
     __device__ __forceinline__ u64 of(float v) const {
-        float rest;
-        const float far = distance(v, rest);
-        return of(far, rest);
+        if (v == top) return 1ull << bits;
+        const double y = ((double)top - (double)v) * steps;
+        if (!(y < 16.0 * 62.0)) return 0;
+        const double magic = 6755399441055744.0;             // 1.5 2^52: adding it rounds to a whole number
+        const double t = y + magic;
+        const int n = __double2loint(t);
+        const double r = y - (t - magic);
+        constexpr double L = 0.69314718055994530942 / ROOTS;
+        double p = -L * L * L * L * L / 120.0;
+        p = fma(p, r, L * L * L * L / 24.0);
+        p = fma(p, r, -L * L * L / 6.0);
+        p = fma(p, r, L * L / 2.0);
+        p = fma(p, r, -L);
+        p = fma(p, r, 1.0);
+        const double unit = __hiloint2double((1023 + bits - n / ROOTS) << 20, 0);
+        return __double2ull_rn(p * roots[n % ROOTS] * unit);
     }
 };
 __device__ __forceinline__ int step_of(float far) { return far < FARTHEST ? (int)(far * STEPS_A_UNIT) : STEPS; }
@@ -266,6 +276,7 @@ sample_filtered_kernel(const Rows of, const int C) {
     auto take = [&](float v, int i) { if (v > best || (v == best && i < best_at)) { best = v; best_at = i; } };
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) take(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_at, o));
+    if (tid < ROOTS) s.roots[tid] = exp2(-(double)tid / ROOTS);
     if (lane == 0) { s.warp_mass[warp] = (u64)__float_as_uint(best) << 32 | (unsigned)best_at; }
     __syncthreads();
     if (warp == 0) {
@@ -298,8 +309,9 @@ sample_filtered_kernel(const Rows of, const int C) {
     Mass mass;
     mass.top = top;
     mass.over = 1.f / heat;
-    mass.over_rest = (float)(1.0 / (double)heat - (double)mass.over);
-    mass.scale = __uint_as_float((unsigned)(127 + of.mass_bits) << 23);
+    mass.steps = ROOTS * 1.44269504088896340736 / (double)heat;
+    mass.bits = of.mass_bits;
+    mass.roots = s.roots;
     const int k = of.top_k[row];
     const bool use_k = k > 0 && k < V;
     const float p = fmaxf(of.top_p[row], 1e-30f), least = of.min_p[row];      // the first token always stays
@@ -327,8 +339,7 @@ sample_filtered_kernel(const Rows of, const int C) {
         __syncthreads();
         u64 total = 0;
         walk([&](float v, int) {
-            float rest;
-            const float far = mass.distance(v, rest);
+            const float far = mass.distance(v);
             const int step = step_of(far);
             if (step >= STEPS) return;
             if (use_k) atomicAdd(&s.counts[step], 1u);
@@ -336,7 +347,7 @@ sample_filtered_kernel(const Rows of, const int C) {
                 // e^-(distance inside the step), the step 1/128 long: two terms of the series are good to 1e-7
                 const float in = far - (float)step * (1.f / STEPS_A_UNIT);
                 atomicAdd(&s.coarse[step], (unsigned)__float2int_rn((1.f - in * (1.f - 0.5f * in)) * (float)(1 << COARSE_BITS)));
-                total += mass.of(far, rest);
+                total += mass.of(v);
             }
         });
         unsigned nothing;
@@ -406,12 +417,10 @@ sample_filtered_kernel(const Rows of, const int C) {
             u64 m = 0;
             unsigned cnt = 0, least_key = 0xffffffffu, most_key = 0;
             walk_segments([&](float v, int i, Sums& here) {
-                float rest;
-                const float far = mass.distance(v, rest);
-                const int step = step_of(far);
+                const int step = step_of(mass.distance(v));
                 if (step > to) return;
                 if (step < from) {
-                    const u64 own = mass.of(far, rest);
+                    const u64 own = mass.of(v);
                     m += own;
                     ++cnt;
                     if (v >= low_logit) { here.mass += own; ++here.number; }
@@ -543,9 +552,7 @@ sample_filtered_kernel(const Rows of, const int C) {
                     u64 mine = 0;
                     unsigned nothing_more;
                     walk([&](float v, int) {
-                        float rest;
-                        const float far = mass.distance(v, rest);
-                        if (step_of(far) == at) mine += mass.of(far, rest);
+                        if (step_of(mass.distance(v)) == at) mine += mass.of(v);
                     });
                     cluster_sum(mine, 0u, here_mass, nothing_more);
                 }
@@ -582,14 +589,12 @@ sample_filtered_kernel(const Rows of, const int C) {
                     for (int i = tid; i < STEPS; i += THREADS) { s.counts[i] = 0; s.fine[i] = 0; }
                     __syncthreads();
                     walk([&](float v, int) {
-                        float rest;
-                        const float far = mass.distance(v, rest);
-                        if (step_of(far) != at) return;
+                        if (step_of(mass.distance(v)) != at) return;
                         const unsigned key = ordered_key(v);
                         if (key < from || key > upto) return;
                         const int bin = (int)((upto - key) >> shift);          // largest first
                         atomicAdd(&s.counts[bin], 1u);
-                        atomicAdd(&s.fine[bin], mass.of(far, rest));
+                        atomicAdd(&s.fine[bin], mass.of(v));
                     });
                     cluster_sync();
                     u64 m[4], cnt[4], own_m = 0, own_n = 0, total_m, total_n;
@@ -663,8 +668,7 @@ sample_filtered_kernel(const Rows of, const int C) {
                 const float v = logit_of(key_of(entry));
                 if (entry > last_entry || v < low_logit) continue;
                 atomicAdd(&s.segment_mass[(int)(unsigned)entry / S - (int)rank * per_block], mass.of(v));
-                float rest;
-                number_all += mass.distance(v, rest) < 745.f;
+                number_all += mass.distance(v) < 745.f;
             }
         }
     }
@@ -690,10 +694,8 @@ sample_filtered_kernel(const Rows of, const int C) {
             walk_segments([&](float v, int, Sums& here) {
                 if (ordered_key(v) < thr || v < low_logit) return;
                 // as many as have a probability at all, however small: e^-x in 64 bits is above zero up to 745
-                float rest;
-                const float far = mass.distance(v, rest);
-                here.mass += mass.of(far, rest);
-                here.number += far < 745.f;
+                here.mass += mass.of(v);
+                here.number += mass.distance(v) < 745.f;
             });
         else {
             number_all = 0;
@@ -709,10 +711,8 @@ sample_filtered_kernel(const Rows of, const int C) {
                     const unsigned place = seen + __popc(tied & ((1u << lane) - 1u));
                     seen += __popc(tied);
                     if (i < to && (key > thr || (key == thr && place < need)) && v >= low_logit) {
-                        float rest;
-                        const float far = mass.distance(v, rest);
-                        sum += mass.of(far, rest);
-                        number_all += far < 745.f;
+                        sum += mass.of(v);
+                        number_all += mass.distance(v) < 745.f;
                     }
                 }
                 sum = warp_sum64(sum);

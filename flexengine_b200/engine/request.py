@@ -60,6 +60,8 @@ class Request:
     top_k: int = 0
     priority: int = 0
     seed: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
     created: int = field(default_factory=lambda: int(time.time()))
     arrived: float = field(default_factory=time.monotonic)
     state: State = State.WAITING

@@ -31,11 +31,11 @@ from dataclasses import dataclass
 
 import torch
 
-from ..cache.manager import CacheManager
+from ..cache.manager import CacheManager, kv4_row_bytes
 from ..cache.page_pool import CacheExhausted
 from ..config.engine_config import EngineConfig
 from ..observability.traces import RunTrace, marked
-from ..sampling.sampler import Sampler
+from ..sampling.sampler import Sampler, validate_filters
 from .request import PENDING, TERMINAL, Event, Request, State
 from .scheduler import Scheduler
 from .step import ModelRunner, StepEntry
@@ -116,7 +116,10 @@ class Engine:
         plan = model.plan
         dtype = {"bfloat16": torch.bfloat16, "float32": torch.float32}[config.dtype]
         pages = config.kv_num_blocks or pages_that_fit(plan, config, dtype)
-        cache = CacheManager(plan.cache_groups, pages, config.kv_block_size, config.max_num_seqs, dtype, config.device)
+        if config.kv_cache_dtype == "int4":
+            check_kv4(plan)
+        cache = CacheManager(plan.cache_groups, pages, config.kv_block_size, config.max_num_seqs, dtype, config.device,
+                             kv_cache_dtype=config.kv_cache_dtype)
         runner = ModelRunner(model, cache, ops=ops)
         if config.cuda_graph:
             runner.enable_decode_graphs(config.max_num_seqs, config.max_model_len)
@@ -165,9 +168,10 @@ class Engine:
         return ids
 
     def submit(self, prompt, max_tokens: int = 128, temperature: float = 0.0, top_k: int = 0, priority: int = 0,
-               seed: int | None = None) -> Request:
-        """Queue a request.  ``prompt`` is text (needs a tokenizer) or a list of token ids.  Raises ValueError
-        for what can never run and BusyError when the engine takes nothing now."""
+               seed: int | None = None, top_p: float = 1.0, min_p: float = 0.0) -> Request:
+        """Queue a request.  ``prompt`` is text (needs a tokenizer) or a list of token ids.  ``top_p``: of the tokens that
+        ``top_k`` leaves, as few of the likeliest as hold that share of their probability; ``min_p``: of these, what has that
+        share of the likeliest one's.  Raises ValueError for what can never run and BusyError when the engine takes nothing now."""
         ids = self._token_ids(prompt)
         cfg = self.config
         if not 1 <= max_tokens <= cfg.max_output_tokens:
@@ -177,6 +181,7 @@ class Engine:
             raise ValueError(f"temperature={temperature} is outside {low}..{high}")
         if top_k < 0:
             raise ValueError(f"top_k={top_k} is negative")
+        validate_filters(top_p, min_p)
         if len(ids) + max_tokens > cfg.max_model_len:
             raise ValueError(f"{len(ids)} prompt tokens + max_tokens={max_tokens} exceed max_model_len={cfg.max_model_len}")
         with self.lock:
@@ -184,7 +189,8 @@ class Engine:
                 raise BusyError("the engine has stopped" if not self.fault else f"the engine faulted: {self.fault}")
             if len(self.waiting) >= cfg.max_waiting:
                 raise BusyError(f"{len(self.waiting)} requests are waiting already (max_waiting)")
-            request = Request(f"cmpl-{uuid.uuid4().hex}", ids, int(max_tokens), float(temperature), int(top_k), int(priority))
+            request = Request(f"cmpl-{uuid.uuid4().hex}", ids, int(max_tokens), float(temperature), int(top_k), int(priority),
+                              top_p=float(top_p), min_p=float(min_p))
             # a default seed that depends only on the order of submission: the same requests in the same order
             # draw the same tokens under every policy and batching (runtime.py:112-116)
             request.seed = cfg.random_seed + self.counters.submitted if seed is None else int(seed)
@@ -368,8 +374,11 @@ class Engine:
         logits = self._run_step(entries, earlier.tokens if earlier is not None else None)
         tokens = None
         if sampled:
+            filters = {}
+            if any(r.top_p < 1.0 or r.min_p > 0.0 for r in sampled):
+                filters = {"top_ps": [r.top_p for r in sampled], "min_ps": [r.min_p for r in sampled]}
             tokens = self.sampler.sample_on_device(logits, [r.temperature for r in sampled], [r.top_k for r in sampled],
-                                                   [r.seed for r in sampled], [len(r.generated_ids) for r in sampled])
+                                                   [r.seed for r in sampled], [len(r.generated_ids) for r in sampled], **filters)
         now = time.monotonic()
         places = []
         for chunk in chunks:
@@ -483,7 +492,7 @@ class Engine:
 
     # ---- entry points -----------------------------------------------------------------------------------------------
     def generate(self, prompts, max_tokens: int = 128, temperature: float = 0.0, top_k: int = 0,
-                 seed: int | None = None, max_steps: int | None = None) -> list:
+                 seed: int | None = None, max_steps: int | None = None, top_p: float = 1.0, min_p: float = 0.0) -> list:
         """Generate for every prompt (text, or lists of token ids) and return the outputs in the order given.
         Steps inline until all have ended; prompts beyond the waiting bound are submitted as room appears.
         ``seed``: prompt i draws with ``seed + i``."""
@@ -495,7 +504,7 @@ class Engine:
             while len(requests) < len(prompts) and len(self.waiting) < self.config.max_waiting:
                 i = len(requests)
                 requests.append(self.submit(prompts[i], max_tokens=max_tokens, temperature=temperature, top_k=top_k,
-                                            seed=None if seed is None else seed + i))
+                                            seed=None if seed is None else seed + i, top_p=top_p, min_p=min_p))
             alive = [r for r in requests if r.state not in TERMINAL]
             if not alive and len(requests) == len(prompts):
                 break
@@ -537,14 +546,27 @@ class Engine:
         self.trace.close()
 
 
+def check_kv4(plan) -> None:
+    """Whether every mixer with a paged cache of its own works on one held in 4 bits; ValueError otherwise."""
+    from ..parts.base import mixer_kind
+    paged = [g.kind != "state" for g in plan.cache_groups]
+    for entry in plan.run:
+        kind = plan.layers[entry.layer].mixer.kind
+        for group in (entry.cache_group,) + tuple(g for g, _ in entry.more):
+            spec = plan.cache_groups[group]
+            if paged[group] and (not getattr(mixer_kind(kind), "reads_kv4", False) or spec.planes != 2 or spec.kind not in ("full", "window")):
+                raise ValueError(f"kv_cache_dtype 'int4': the mixer {kind!r} of layer {entry.layer} does not read a 4-bit cache")
+
+
 def pages_that_fit(plan, config: EngineConfig, dtype) -> int:
     """Pages per paged cache group that fill ``kv_memory_fraction`` of the device memory that is free now."""
     if not str(config.device).startswith("cuda"):
         raise ValueError("kv_num_blocks=0 (size the pool from free memory) needs a CUDA device")
     free, _total = torch.cuda.mem_get_info(torch.device(config.device))
     width = torch.empty((), dtype=dtype).element_size()
-    page_bytes = sum(getattr(g, "planes", 2) * g.slots * g.kv_heads * g.head_dim * (g.page_size or config.kv_block_size) * width
-                     for g in plan.cache_groups if g.kind != "state")
+    row = (lambda g: kv4_row_bytes(g.head_dim)) if config.kv_cache_dtype == "int4" else \
+        (lambda g: getattr(g, "planes", 2) * g.head_dim * width)
+    page_bytes = sum(g.slots * g.kv_heads * row(g) * (g.page_size or config.kv_block_size) for g in plan.cache_groups if g.kind != "state")
     pages = int(free * config.kv_memory_fraction) // max(page_bytes, 1)
     smallest = min((g.page_size or config.kv_block_size for g in plan.cache_groups if g.kind != "state"),
                    default=config.kv_block_size)

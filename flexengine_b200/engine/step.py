@@ -36,13 +36,20 @@ class GroupView:
         self.kind = group.spec.kind
         self.storage = group.storage
         self.page_size = page_size
+        self.four_bit = getattr(group, "four_bit", False)     # keys and values in 4 bits: kv4_slot instead of kv_slot
         self.slot_mapping = None      # int32 [T]: flat slot of every token (paged groups)
         self.block_table = None       # int32 [R, max_pages] (paged groups)
         self.max_pages = 0
 
     def kv_slot(self, slot: int):
         """(keys, values) of one cache slot; a group of one plane hands out that plane twice."""
+        if self.four_bit:
+            raise TypeError(f"group {self.spec.name!r} is held in 4 bits: its slots have no key and value planes")
         return self.storage[slot, 0], self.storage[slot, self.storage.shape[1] - 1]
+
+    def kv4_slot(self, slot: int):
+        """The 4-bit cache of one slot: uint8 [pages, kv heads, page size / 16, bytes of a tile]."""
+        return self.storage[slot]
 
     def state(self, slot: int):
         """[max_requests, *state_shape] storage of one state slot layer; index with ctx.state_slots."""

@@ -16,6 +16,7 @@ from array import array
 import torch
 
 from . import library
+from ..cache.manager import KV4_TILE, kv4_row_bytes, kv4_shape  # noqa: F401 - the form of a 4-bit cache
 
 # Arguments go to the entry points as plain Python values: the loader has given every entry point the parameter
 # types of its C declaration (ops/library.py), so ctypes converts them itself, and refuses a call whose number of
@@ -1776,27 +1777,14 @@ def sample_filtered(logits, temperature, top_k, top_p, min_p, uniform, blocks: i
 
 
 # ---- keys and values held in 4 bits (csrc/kv4.cuh has their form) -------------------------------------------------------
-KV4_TILE = 16            # tokens of a tile: page sizes of a 4-bit cache are multiples of it
-KV4_MAX_DIM = 256
-KV4_FORCE = None
-
-
-def kv4_row_bytes(d: int) -> int:
-    """Bytes of one token's key and value of one head: 5 bits a number, groups of 32 with a scale and a centre each."""
-    if d % 16 or not 16 <= d <= KV4_MAX_DIM:
-        raise ValueError(f"head size {d}: a 4-bit cache takes multiples of 16 from 16 to {KV4_MAX_DIM}")
-    return 40 * -(-d // 32)
-
-
-def kv4_shape(pages: int, nkv: int, page_size: int, d: int) -> tuple:
-    """The shape of a 4-bit cache of ``pages`` pages, a uint8 tensor: [pages, nkv, page_size / 16, bytes of a tile of 16 tokens]."""
-    if page_size < KV4_TILE or page_size % KV4_TILE:
-        raise ValueError(f"page size {page_size}: a 4-bit cache takes multiples of {KV4_TILE}")
-    return (pages, nkv, page_size // KV4_TILE, KV4_TILE * kv4_row_bytes(d))
+_kv4_library = None
 
 
 def _kv4():
-    return library.load("kv4")
+    global _kv4_library
+    if _kv4_library is None:
+        _kv4_library = library.load("kv4")
+    return _kv4_library
 
 
 class _NoGuard:
@@ -1810,26 +1798,34 @@ class _NoGuard:
 _NO_GUARD = _NoGuard()
 
 
-def _on(what, *tensors):
+def _on(what, first, *others):
     """A context in which the device of the tensors (which all lie on one) is the current one; refuses others."""
-    _need_cuda(*tensors)
-    device = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: tensors on {device} and {t.device}")
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+    if index < 0:
+        _need_cuda(first)
+    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _index_ok(what, name, t, shape) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{what}: {name} is a contiguous int32 {list(shape)}, not {t.dtype} {list(t.shape)}")
+def _index_ok(what, name, t, n, columns=None) -> None:
+    if t.dtype is not torch.int32 or t.shape != ((n,) if columns is None else (n, columns)) or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} is a contiguous int32 {[n] if columns is None else [n, columns]}, not {t.dtype} {list(t.shape)}")
+
+
+_kv4_geometries: set = set()      # (shape, heads, head size, page size) that were found to belong together
 
 
 def _kv4_cache_ok(what, cache, nkv, d, page_size) -> None:
-    if cache.dtype != torch.uint8 or cache.dim() != 4 or tuple(cache.shape) != kv4_shape(cache.shape[0], nkv, page_size, d) \
-            or not cache.is_contiguous() or cache.data_ptr() % 16:
-        raise ValueError(f"{what}: the cache is a contiguous uint8 {list(kv4_shape(cache.shape[0], nkv, page_size, d))} on a 16-byte boundary, "
-                         f"not {cache.dtype} {list(cache.shape)}")
+    geometry = (cache.shape, nkv, d, page_size)
+    if geometry not in _kv4_geometries:
+        want = kv4_shape(cache.shape[0], nkv, page_size, d)
+        if tuple(cache.shape) != want:
+            raise ValueError(f"{what}: the cache is uint8 {list(want)}, not {list(cache.shape)}")
+        _kv4_geometries.add(geometry)
+    if cache.dtype is not torch.uint8 or not cache.is_contiguous() or cache.data_ptr() % 16:
+        raise ValueError(f"{what}: the cache is contiguous uint8 on a 16-byte boundary, not {cache.dtype}")
 
 
 def qkv_rope_kv4(projected, bias, positions, inv_freq, rot, slot_mapping, cache, nq, nkv, d, page_size, pairs="halves", rot_gain=1.0,
@@ -1848,9 +1844,9 @@ def qkv_rope_kv4(projected, bias, positions, inv_freq, rot, slot_mapping, cache,
             raise ValueError(f"{what}: pairs {pairs!r}; 'halves' or 'interleaved'")
         T, out_dtype = projected.shape[0], out_dtype or projected.dtype
         _kv4_cache_ok(what, cache, nkv, d, page_size)
-        _index_ok(what, "positions", positions, (T,))
+        _index_ok(what, "positions", positions, T)
         if slot_mapping is not None:
-            _index_ok(what, "slot_mapping", slot_mapping, (T,))
+            _index_ok(what, "slot_mapping", slot_mapping, T)
         if bias is not None and (bias.dtype != torch.float32 or bias.numel() != (nq + 2 * nkv) * d or not bias.is_contiguous()):
             raise ValueError(f"{what}: the bias is contiguous float32 [(nq + 2 nkv) d]")
         if rot and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2 or not inv_freq.is_contiguous()):
@@ -1868,11 +1864,27 @@ def kv4_rows(cache, slots, nkv, d, page_size, dtype=torch.bfloat16):
     with _on(what, cache, slots):
         _kv4_cache_ok(what, cache, nkv, d, page_size)
         n = slots.numel()
-        _index_ok(what, "slots", slots, (n,))
+        _index_ok(what, "slots", slots, n)
         keys, values = (torch.empty((n, nkv, d), dtype=dtype, device=cache.device) for _ in range(2))
         _run(_kv4(), "fe_kv4_rows", _ptr(cache), _ptr(slots), _ptr(keys), _ptr(values), _code(dtype), n, nkv, d, page_size, cache.shape[0] * page_size,
              _ptr(status_word(cache.device)), _stream())
     return keys, values
+
+
+_KV4_PLANS: dict = {}
+
+
+def kv4_plan(requests: int, tiles: int, nq: int, nkv: int, d: int, code: int) -> tuple:
+    """(plan, bytes of scratch) of a decode step over a 4-bit cache: how its tiles are dealt out (fe_kv4_attention_plan), asked once a shape and
+    device: the answer rests on how many blocks the device holds."""
+    key = (requests, tiles, nq, nkv, d, code, torch.cuda.current_device())
+    known = _KV4_PLANS.get(key)
+    if known is None:
+        plan = int(_kv4().fe_kv4_attention_plan(requests, tiles, nq, nkv, d, code))
+        known = _KV4_PLANS[key] = (plan, int(_kv4().fe_kv4_attention_scratch_bytes(max(plan, 0), requests, nq, nkv, d)))
+        if len(_KV4_PLANS) > 4096:
+            _KV4_PLANS.clear()
+    return known
 
 
 def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale, window=0, keep_first=0, sink=False):
@@ -1883,30 +1895,29 @@ def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale
     bits (csrc/attention_kv4.cu); float32 queries keep 22 bits through the products."""
     what = "paged_attention_kv4"
     with _on(what, q, cache, block_table, ctx.cu_q, ctx.q_start):
-        T, requests = q.shape[0], ctx.cu_q.numel() - 1
+        T, requests, pages, code = q.shape[0], ctx.cu_q.numel() - 1, block_table.shape[-1], _code(q.dtype)
         if q.dim() != 2 or q.shape[1] < nq * d or q.stride(1) != 1 or (T > 1 and q.stride(0) % 8) or q.data_ptr() % 16:
             raise ValueError(f"{what}: q is [T, >= nq d] with unit column stride, rows on 16-byte boundaries")
         _kv4_cache_ok(what, cache, nkv, d, page_size)
-        _index_ok(what, "cu_q", ctx.cu_q, (requests + 1,))
-        _index_ok(what, "q_start", ctx.q_start, (requests,))
-        _index_ok(what, "block_table", block_table, (requests, block_table.shape[-1]))
+        _index_ok(what, "cu_q", ctx.cu_q, requests + 1)
+        _index_ok(what, "q_start", ctx.q_start, requests)
+        _index_ok(what, "block_table", block_table, requests, pages)
         if window < 0 or keep_first < 0 or (keep_first and not window):
             raise ValueError(f"{what}: a window is not negative, and kept first keys go with one")
-        if ctx.max_ctx_len > block_table.shape[1] * page_size:
-            raise ValueError(f"{what}: {ctx.max_ctx_len} tokens in {block_table.shape[1]} pages of {page_size}")
+        if ctx.max_ctx_len > pages * page_size:
+            raise ValueError(f"{what}: {ctx.max_ctx_len} tokens in {pages} pages of {page_size}")
         out = torch.empty((T, nq * d), dtype=q.dtype, device=q.device)
         lib, splits, blocks, part = _kv4(), 1, 0, None
-        if KV4_FORCE: splits, blocks = KV4_FORCE
-        elif ctx.max_q_len == 1:
+        if ctx.max_q_len == 1:
             span = ctx.max_ctx_len if window == 0 else min(ctx.max_ctx_len, window + keep_first + 2 * KV4_TILE)
-            plan = lib.fe_kv4_attention_plan(requests, -(-span // KV4_TILE), nq, nkv, d, _code(q.dtype))
+            plan, nbytes = kv4_plan(requests, -(-span // KV4_TILE), nq, nkv, d, code)
             splits, blocks = (1, plan) if plan > 0 else (-plan, 0)
-        if blocks:
+            if blocks:
                 # of its own for every call: two streams, or two captured graphs, may be at it at once
-                part = torch.empty(lib.fe_kv4_attention_scratch_bytes(blocks, requests, nq, nkv, d), dtype=torch.uint8, device=q.device)
-        _run(lib, "fe_paged_attention_kv4", _ptr(q), q.stride(0) if T > 1 else nq * d, _ptr(out), nq * d, _ptr(cache), _ptr(block_table), block_table.shape[1],
-             _ptr(ctx.cu_q), _ptr(ctx.q_start), requests, T, ctx.max_q_len, nq, nkv, d, page_size, cache.shape[0], float(scale), window, keep_first,
-             1 if sink else 0, splits, blocks, _ptr(part), _code(q.dtype), _ptr(status_word(q.device)), _stream())
+                part = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _run(lib, "fe_paged_attention_kv4", q.data_ptr(), q.stride(0) if T > 1 else nq * d, out.data_ptr(), nq * d, cache.data_ptr(), block_table.data_ptr(), pages,
+             ctx.cu_q.data_ptr(), ctx.q_start.data_ptr(), requests, T, ctx.max_q_len, nq, nkv, d, page_size, cache.shape[0], float(scale), window, keep_first,
+             1 if sink else 0, splits, blocks, _ptr(part), code, status_word(q.device).data_ptr(), _stream())
     return out
 
 

@@ -19,6 +19,7 @@ from .spec import PartSpec
 
 class AttentionMixer(Mixer):
     takes_prenormed = True
+    reads_kv4 = True
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
                  position: PartSpec | dict | None = None, qkv_bias: bool = True, out_bias: bool = False,
@@ -61,9 +62,12 @@ class AttentionMixer(Mixer):
     def forward(self, ctx, h, entry, follow=None, upcoming=None):
         ops = ctx.ops
         group = ctx.groups[entry.cache_group]
-        k_cache, v_cache = group.kv_slot(entry.cache_slot)
         slot_mapping = group.slot_mapping if entry.write_cache else None
         nq, nkv, d = self.num_heads, self.num_kv_heads, self.head_dim
+        if group.four_bit:
+            out = self._attend_kv4(ctx, h, group, group.kv4_slot(entry.cache_slot), slot_mapping)
+            return ops.linear(out, self.out_weight, self.out_bias, **({} if follow is None else {"follow": follow, "upcoming": upcoming}))
+        k_cache, v_cache = group.kv_slot(entry.cache_slot)
         if self.position.applies_itself:
             # an encoding of its own: projection and bias, the encoding on the query and key heads in place,
             # then the keys and values to their cache slots
@@ -83,6 +87,21 @@ class AttentionMixer(Mixer):
         if follow is not None:
             return ops.linear(out, self.out_weight, self.out_bias, follow=follow, upcoming=upcoming)
         return ops.linear(out, self.out_weight, self.out_bias)
+
+
+    def _attend_kv4(self, ctx, h, group, cache, slot_mapping):
+        """Projection, cache and attention where keys and values are held in 4 bits: they are rounded to them once, from 32 bits."""
+        ops = ctx.ops
+        nq, nkv, d = self.num_heads, self.num_kv_heads, self.head_dim
+        if self.position.applies_itself:
+            qkv = ops.linear(h, self.qkv_weight, self.qkv_bias)
+            self.position.apply(ctx, qkv[:, :nq * d].view(-1, nq, d), qkv[:, nq * d:(nq + nkv) * d].view(-1, nkv, d))
+            bias, inv_freq, rot = None, None, 0
+        else:
+            qkv, bias = ops.linear(h, self.qkv_weight, out_float32=True), self.qkv_bias
+            inv_freq, rot = self.position.rotary_table(qkv.device) or (None, 0)
+        queries = ops.qkv_rope_kv4(qkv, bias, ctx.positions, inv_freq, rot, slot_mapping, cache, nq, nkv, d, group.page_size, out_dtype=ctx.dtype)
+        return ops.paged_attention_kv4(queries, cache, group.block_table, ctx, nq, nkv, d, group.page_size, self.scale, self.window)
 
 
 class GatedAttentionMixer(Mixer):

@@ -17,6 +17,8 @@ Mixer:           ``cache_need() -> dict | None`` (what cache group it needs) and
                  never read.  The same holds for cache slot -1 in ``slot_mapping``: nothing is written.
                  Under CUDA graphs the slots must be taken from the device tensors (``ctx.state_slots``),
                  not from their host copies, whose values a captured graph would keep for good.
+                 ``reads_kv4`` says that the mixer also works on a paged group held in 4 bits
+                 (``ctx.groups[g].four_bit``); others are refused such a cache when the engine is built.
 FeedForward:     ``forward(ctx, h) -> delta [T, hidden]``.
 Norm:            ``forward(ctx, residual, delta, rows=None) -> h``: adds ``delta`` (may be None)
                  to the float32 residual stream in place and returns the normalised rows
@@ -99,6 +101,11 @@ def build_part(family: str, spec):
     if spec.kind not in table:
         raise KeyError(f"unknown {family} kind {spec.kind!r}; known: {sorted(table)}")
     return table[spec.kind](**dict(spec.params))
+
+
+def mixer_kind(kind: str):
+    """What a mixer kind was registered with (its class, as a rule), without making one."""
+    return _REGISTRIES["mixer"].get(kind)
 
 
 def block_factory(kind: str) -> Callable:

@@ -58,7 +58,7 @@ class PreNormBlock:
             layer = self._native = self._native_layer(ctx) or False
         group = ctx.groups[entry.cache_group]
         if (layer is False or (pending is not None and not torch.is_tensor(pending)) or group.kind not in ("full", "window")
-                or group.storage.dtype != torch.bfloat16):
+                or group.storage.dtype != torch.bfloat16 or group.four_bit):
             return None
         steps = ctx.__dict__.setdefault("_native_steps", {})
         step_key = (entry.cache_group, entry.write_cache, layer.hidden, layer.nq, layer.nkv, layer.d, layer.intermediate, layer.window)
