@@ -26,10 +26,19 @@
 // Warps 8..11 gather keys and values from the pages with 16-byte asynchronous copies into a
 // four-stage ring; lane 0 of warp 12 + i issues the products of row tile i.
 //
+// FOUR = true: the cache is held in 4 bits (kv4.cuh has its form).  Bulk copies bring a key tile's codes, scales and centres as they lie into a ring
+// of their own, three tiles deep; the loader warps make half-precision rows of them, code * scale + centre (rounded once, 2^-11 of the number at
+// most), where the others copy rows, once for the block's 256 rows.  The eight numbers of a 16-byte chunk lie as 0, 4, 1, 5, 2, 6, 3, 7, the order in which
+// a word of codes comes apart: queries are laid out alike, and the result's columns are put back in order as it is
+// written.  Queries are half-precision too, a power of two bringing a row's largest number to [1, 2), and so are the weights P.  A stored
+// group that reads as NaN enters as zeros; where one was met, every row looks at the scales of the keys that it sees and
+// writes NaN itself (0 times NaN would reach rows that do not see it).
+//
 // Every wait on an mbarrier is bounded, and ends early once any thread of the block has given up;
 // the block then records it in the status word, leaves its loops and frees its tensor memory.
 #include <math_constants.h>
 
+#include "kv4.cuh"
 #include "tcgen05.cuh"
 
 using namespace fe;
@@ -67,6 +76,12 @@ __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait_but() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+// the loaders' barrier, and whether any of them says so
+__device__ __forceinline__ bool loader_any(bool mine) {
+    unsigned any;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"(mine ? 1u : 0u) : "memory");
+    return any != 0;
+}
 __device__ __forceinline__ void loader_barrier() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); }
 
 // Shared-memory descriptor of an MN-major operand, 128-byte swizzle (V as it lies in the cache: one row per key, 64 head elements = 128 bytes
@@ -118,18 +133,51 @@ __device__ __forceinline__ int swizzled(int r, int c, int block_bytes) {
     return (c >> 3) * block_bytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
+// Half precision instead of bfloat16: the two bits of the instruction descriptor that name the operands' types.
+__host__ __device__ constexpr unsigned half_operands(unsigned idesc) { return idesc & ~((1u << 7) | (1u << 10)); }
+constexpr int RAW_STAGES = 3;            // key tiles of a 4-bit cache as they lie in memory
+constexpr int SUBTILES = KEYS / KV4_TILE;
+
+__device__ __forceinline__ void bulk_copy(unsigned to, const unsigned char* from, int bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ unsigned half_pair(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+// Eight codes times their scale plus their centre, four pairs as they lie in a chunk.
+__device__ __forceinline__ uint4 four_bit_chunk(unsigned codes, __half2 pair) {
+    unsigned n[4];
+    kv4_decode(codes, n);
+    const __half2 scale = __low2half2(pair), centre = __high2half2(pair);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&n[i]), scale, centre);
+        n[i] = *reinterpret_cast<const unsigned*>(&x);
+    }
+    return make_uint4(n[0], n[1], n[2], n[3]);
+}
+// Eight columns of a result over a 4-bit cache, back in order.
+__device__ __forceinline__ void in_order(float* v) {
+    const float x1 = v[1], x2 = v[2], x3 = v[3], x4 = v[4], x5 = v[5], x6 = v[6];
+    v[1] = x2; v[2] = x4; v[3] = x6; v[4] = x1; v[5] = x3; v[6] = x5;
+}
+
 // The softmax of one row over a key tile, the 64 scores in registers.  MASKED: the tile crosses
 // the causal edge or the window's edge for some row of the warp; what this row sees of the tile is then two words of bits, made once a
 // tile (a comparison per key with its short-circuit branches took a tile that crosses an edge from 1.1 to 3.9 us).
 struct Seen { unsigned word[2]; };
 __device__ __forceinline__ unsigned low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 // ``hi`` and ``lo``: the row's last and first visible key relative to the tile; keys below ``keep`` are visible however far back they are.
-__device__ __forceinline__ Seen seen_keys(int hi, int lo, int keep) {
+// Bit i of ``gone``: keys 16 i .. 16 i + 15 of the tile are not in the cache.
+__device__ __forceinline__ Seen seen_keys(int hi, int lo, int keep, unsigned gone) {
     Seen seen;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         const int at = 32 * w;
         seen.word[w] = low_bits(hi + 1 - at) & (~low_bits(lo - at) | low_bits(keep - at));
+        if (gone) seen.word[w] &= ~(((gone >> (2 * w)) & 1u) * 0xffffu | ((gone >> (2 * w + 1)) & 1u) * 0xffff0000u);
     }
     return seen;
 }
@@ -139,10 +187,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;\n" : "=f"(m) : "f"(a), "f"(b), "f"(c));
     return m;
 }
-struct Edges { int hi, lo, keep; };           // of a row, relative to the tile
+struct Edges { int hi, lo, keep; unsigned gone; };           // of a row, relative to the tile
 template <bool MASKED>
 __device__ __forceinline__ float row_max(const unsigned* r, const Edges& edges) {
-    const Seen seen = MASKED ? seen_keys(edges.hi, edges.lo, edges.keep) : Seen{};
+    const Seen seen = MASKED ? seen_keys(edges.hi, edges.lo, edges.keep, edges.gone) : Seen{};
     float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, m2 = -CUDART_INF_F, m3 = -CUDART_INF_F;
 #pragma unroll
     for (int i = 0; i < KEYS; i += 8) {
@@ -158,9 +206,9 @@ __device__ __forceinline__ float row_max(const unsigned* r, const Edges& edges) 
 }
 // P = 2^(s scale - ref) as bfloat16 pairs over the scores' own columns (32 of the 64); returns the row's sum.
 // The multiply-adds and the sums run two floats per instruction.
-template <bool MASKED>
+template <bool MASKED, bool HALF = false>
 __device__ __forceinline__ float row_exp(const unsigned* r, unsigned p_addr, const Edges& edges, float scale_log2, float ref) {
-    const Seen seen = MASKED ? seen_keys(edges.hi, edges.lo, edges.keep) : Seen{};
+    const Seen seen = MASKED ? seen_keys(edges.hi, edges.lo, edges.keep, edges.gone) : Seen{};
     float2 sum = make_float2(0.f, 0.f);
     const float2 scale2 = make_float2(scale_log2, scale_log2), ref2 = make_float2(-ref, -ref);
 #pragma unroll
@@ -176,8 +224,11 @@ __device__ __forceinline__ float row_exp(const unsigned* r, unsigned p_addr, con
                 if (hidden(k + 1, seen)) e.y = 0.f;
             }
             sum = __fadd2_rn(sum, e);
-            const __nv_bfloat162 pair = __floats2bfloat162_rn(e.x, e.y);
-            packed[i] = *reinterpret_cast<const unsigned*>(&pair);
+            if (HALF) packed[i] = half_pair(e.x, e.y);
+            else {
+                const __nv_bfloat162 pair = __floats2bfloat162_rn(e.x, e.y);
+                packed[i] = *reinterpret_cast<const unsigned*>(&pair);
+            }
         }
         tmem_store16(p_addr + (c >> 1), packed);
     }
@@ -188,7 +239,7 @@ __device__ __forceinline__ float row_exp(const unsigned* r, unsigned p_addr, con
 // nothing is summed, a masked key weighs 0.
 template <bool MASKED>
 __device__ __forceinline__ void row_sigmoid(const unsigned* r, unsigned p_addr, const Edges& edges, float scale_log2, float bias) {
-    const Seen seen = MASKED ? seen_keys(edges.hi, edges.lo, edges.keep) : Seen{};
+    const Seen seen = MASKED ? seen_keys(edges.hi, edges.lo, edges.keep, edges.gone) : Seen{};
     const float2 scale2 = make_float2(-scale_log2, -scale_log2), bias2 = make_float2(-bias, -bias);
 #pragma unroll
     for (int c = 0; c < KEYS; c += 32) {
@@ -324,7 +375,7 @@ __device__ __forceinline__ void pick_item(int item, const int* __restrict__ cu_q
     }
 }
 
-template <int D>
+template <int D, bool FOUR = false>
 __global__ void __launch_bounds__(THREADS, 1)
 paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __restrict__ out, long long out_stride,
                              const bf16* __restrict__ kc, const bf16* __restrict__ vc,
@@ -341,6 +392,10 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
     __shared__ volatile int give_up;
     __shared__ int item_request, item_pair;
     __shared__ long long row_place[2 * ROWS];        // where each row's result goes, -1 for padding rows
+    __shared__ float row_factor[FOUR ? 2 * ROWS : 1];                     // what brings a row's largest query number to [1, 2), the other way
+    __shared__ __align__(8) unsigned long long raw_full[FOUR ? RAW_STAGES : 1];
+    __shared__ unsigned gone_of[FOUR ? KV_STAGES : 1], missing_of[FOUR ? RAW_STAGES : 1];      // subtiles of a key tile that are not in the cache
+    __shared__ int saw_nan;                          // some value group read as NaN
     constexpr int DB = D / 64;                       // 64-element blocks per row
     constexpr int Q_BYTES = DB * Q_BLOCK;            // one row tile of Q
     constexpr int KV_BYTES = DB * KV_BLOCK;          // one key tile of K or of V
@@ -348,6 +403,8 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* q_s = smem;                       // row tile i at q_s + i * Q_BYTES
     unsigned char* kv_s = q_s + 2 * Q_BYTES;         // stage s: K at kv_s + s * 2 * KV_BYTES, V after it
+    constexpr int GROUPS = D / KV4_GROUP, SUB_BYTES = kv4_tile_bytes(GROUPS), RAW_BYTES = SUBTILES * SUB_BYTES;
+    unsigned char* raw_s = kv_s + KV_STAGES * 2 * KV_BYTES;               // FOUR: key tiles as they lie in memory
 
     griddep_wait();
     griddep_launch_dependents();
@@ -398,6 +455,10 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
             mbar_init(&pv_done[i], 1);
             mbar_init(&o_final[i], 1);
         }
+        if (FOUR) {
+            for (int i = 0; i < RAW_STAGES; ++i) mbar_init(&raw_full[i], 1);
+            saw_nan = 0;
+        }
         give_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -428,6 +489,24 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
         // the warp's 32 query rows into shared memory, swizzled like a TMA tile (zeros for padding rows)
         unsigned char* dst = q_s + ti * Q_BYTES;
         const int c = lane % CPR;
+        if (FOUR) {
+#pragma unroll 4
+            for (int k = 0; k < CPR; ++k) {
+                const int row_in_warp = k * RPI + lane / CPR;
+                const long long from = __shfl_sync(FULL, q_off, row_in_warp);
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, largest = 0.f;
+                if (from >= 0) load8<bf16>(q + from + c * 8, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(v[e]));
+#pragma unroll
+                for (int o = CPR / 2; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(FULL, largest, o));
+                const int e2 = min(max((int)(__float_as_uint(largest) >> 23) - 127, -126), 126);
+                const float down = __uint_as_float((unsigned)(127 - e2) << 23);
+                if (c == 0) row_factor[warp * 32 + row_in_warp] = __uint_as_float((unsigned)(127 + e2) << 23);
+                *reinterpret_cast<uint4*>(dst + swizzled((warp & 3) * 32 + row_in_warp, c, Q_BLOCK)) =
+                    make_uint4(half_pair(v[0] * down, v[4] * down), half_pair(v[1] * down, v[5] * down), half_pair(v[2] * down, v[6] * down), half_pair(v[3] * down, v[7] * down));
+            }
+        } else
 #pragma unroll
         for (int k = 0; k < CPR; ++k) {
             const int row_in_warp = k * RPI + lane / CPR;
@@ -442,7 +521,99 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
     tc_fence_after();
     const unsigned tmem_base = tmem_holder;
 
-    if (warp >= 8 && warp < 12) {
+    if (FOUR && warp >= 8 && warp < 12) {
+        // ---- loaders of a 4-bit cache.  In iteration j warp 8 asks for the pages of tile j + 3 (a lane a subtile) and starts the copies of
+        // tile j + 2, whose place tile j - 1 has left; then all four warps make rows of tile j ----
+        const unsigned char* cache = reinterpret_cast<const unsigned char*>(kc);
+        const int lt = tid - 256, per_page = ps / KV4_TILE;
+        constexpr int ROW_STEP = 128 / CPR;
+        const int chunk = lt % CPR, row0 = lt / CPR, smem_off0 = swizzled(row0, chunk, KV_BLOCK), group = chunk / 4;
+        // warp 8, lanes 0 .. 3: the page of a subtile of tile j, asked for long before it is looked at; -1: not needed
+        auto page_of = [&](int j) {
+            if (lane >= SUBTILES || j >= n_tiles) return -1;
+            const int key = listed_tile<KEYS>(t_begin + j, kept, lo) * KEYS + lane * KV4_TILE;
+            if (key > hi || (key + KV4_TILE <= lo && key >= keep)) return -1;
+            return block_table[(size_t)r * bt_stride + key / ps];
+        };
+        auto start = [&](int j, int page) {
+            if (j >= n_tiles) return;
+            const int stage = j % RAW_STAGES, key = listed_tile<KEYS>(t_begin + j, kept, lo) * KEYS + lane * KV4_TILE;
+            const bool wanted = lane < SUBTILES && !(key > hi || (key + KV4_TILE <= lo && key >= keep));
+            const bool there = wanted && page >= 0 && page < num_pages;
+            if (wanted && !there && status) atomicOr(status, FE_STATUS_BAD_PAGE);
+            const unsigned here = __ballot_sync(FULL, there), missing = __ballot_sync(FULL, wanted && !there);
+            if (lane == 0) {
+                missing_of[stage] = missing;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(&raw_full[stage])), "r"((int)__popc(here) * SUB_BYTES) : "memory");
+            }
+            __syncwarp();
+            if (there)
+                bulk_copy(smem_u32(raw_s + stage * RAW_BYTES + lane * SUB_BYTES), cache + (((long long)page * nkv + kvh) * per_page + key % ps / KV4_TILE) * SUB_BYTES,
+                          SUB_BYTES, smem_u32(&raw_full[stage]));
+        };
+        int coming = -1;
+        if (warp == 8) {
+            const int p0 = page_of(0), p1 = page_of(1);
+            coming = page_of(2);
+            start(0, p0);
+            start(1, p1);
+        }
+        for (int j = 0; j < n_tiles; ++j) {
+            if (warp == 8) {
+                const int page = coming;
+                coming = page_of(j + 3);
+                start(j + 2, page);
+            }
+            const int s = j % KV_STAGES, stage = j % RAW_STAGES;
+            mbar_wait(&raw_full[stage], (j / RAW_STAGES) & 1, &give_up);
+            mbar_wait(&kv_empty[s], ((j / KV_STAGES) & 1) ^ 1, &give_up);
+            const int key0 = listed_tile<KEYS>(t_begin + j, kept, lo) * KEYS;
+            const unsigned missing = missing_of[stage];
+            unsigned char* k_s = kv_s + s * 2 * KV_BYTES;
+            unsigned char* v_s = k_s + KV_BYTES;
+            // Rows are loaded together, whatever they hold, and those out of range, of pages that are not there, or whose scale is NaN take a scale and a
+            // centre of zero: their numbers are zeros.  (A branch a row had one row on its way at a time: 2.4 us a key tile.)
+            const unsigned char* raw_tile = raw_s + stage * RAW_BYTES;
+            const bool whole = key0 >= lo && key0 + KEYS - 1 <= hi && missing == 0;
+            constexpr int TOGETHER = KEYS / ROW_STEP < 8 ? KEYS / ROW_STEP : 8;
+#pragma unroll
+            for (int i0 = 0; i0 < KEYS / ROW_STEP; i0 += TOGETHER) {
+                unsigned kcodes[TOGETHER], vcodes[TOGETHER], kpair[TOGETHER], vpair[TOGETHER];
+#pragma unroll
+                for (int u = 0; u < TOGETHER; ++u) {
+                    const int row = row0 + (i0 + u) * ROW_STEP, at_row = row % KV4_TILE;
+                    const unsigned char* tile = raw_tile + row / KV4_TILE * SUB_BYTES;
+                    kcodes[u] = *reinterpret_cast<const unsigned*>(tile + at_row * 16 * GROUPS + kv4_key_at(group, 2 * (chunk % 4), GROUPS));
+                    const unsigned char* vp = tile + kv4_value_codes(GROUPS) + at_row * 16 * GROUPS + kv4_value_at(group, 2 * (chunk % 4), GROUPS);
+                    vcodes[u] = *reinterpret_cast<const unsigned short*>(vp) | (unsigned)*reinterpret_cast<const unsigned short*>(vp + 2 * GROUPS) << 16;
+                    kpair[u] = *reinterpret_cast<const unsigned*>(tile + kv4_key_pairs(GROUPS) + (at_row * GROUPS + group) * 4);
+                    vpair[u] = *reinterpret_cast<const unsigned*>(tile + kv4_value_pairs(GROUPS) + (at_row * GROUPS + group) * 4);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int u = 0; u < TOGETHER; ++u) {
+                        const int row = row0 + (i0 + u) * ROW_STEP, key = key0 + row;
+                        if (!((key >= lo || key < keep) && key <= hi) || (missing >> (row / KV4_TILE) & 1u)) kpair[u] = vpair[u] = 0;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < TOGETHER; ++u) {
+                    if ((vpair[u] & 0x7c00u) == 0x7c00u) { vpair[u] = 0; saw_nan = 1; }
+                    *reinterpret_cast<uint4*>(k_s + smem_off0 + (i0 + u) * ROW_STEP * 128) = four_bit_chunk(kcodes[u], *reinterpret_cast<const __half2*>(&kpair[u]));
+                    *reinterpret_cast<uint4*>(v_s + smem_off0 + (i0 + u) * ROW_STEP * 128) = four_bit_chunk(vcodes[u], *reinterpret_cast<const __half2*>(&vpair[u]));
+                }
+            }
+            if (lt == 0) gone_of[s] = missing;
+            fence_proxy_async();
+            mbar_arrive(&kv_full[s]);
+            // the raw tile is read: its place may be filled; all loaders leave together
+            if (loader_any(give_up != 0)) {
+                for (int later = j + 1; later <= j + 2 && later < n_tiles; ++later)       // copies on their way to memory that the block is about to leave
+                    fe::mbar_wait(&raw_full[later % RAW_STAGES], (later / RAW_STAGES) & 1, WAIT_LIMIT);
+                break;
+            }
+        }
+    } else if (warp >= 8 && warp < 12) {
         // ---- loaders: the first 64 look up one key of the tile each, then all copy ----
         const int lt = tid - 256;
         const int ps_shift = (ps & (ps - 1)) == 0 ? __ffs(ps) - 1 : -1;
@@ -497,7 +668,8 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
         // ---- lane 0 of warp 12 + i issues the products of row tile i; the tensor cores keep each thread's order ----
         const int i = warp - 12;
         if (lane == 0 && (i == 0 || two)) {
-            constexpr unsigned idesc_s = instr_desc(ROWS, KEYS, false), idesc_pv = instr_desc(ROWS, D, true);
+            constexpr unsigned idesc_s = FOUR ? half_operands(instr_desc(ROWS, KEYS, false)) : instr_desc(ROWS, KEYS, false),
+                               idesc_pv = FOUR ? half_operands(instr_desc(ROWS, D, true)) : instr_desc(ROWS, D, true);
             constexpr unsigned STAGE16 = (2 * KV_BYTES) >> 4;      // a stage's size in descriptor units
             const unsigned long long q_desc = desc_k_major(q_s + i * Q_BYTES), k_desc0 = desc_k_major(kv_s),
                                      v_desc0 = desc_mn_major(kv_s + KV_BYTES, KV_BLOCK);
@@ -551,7 +723,7 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
         const float bias = (sigmoid && per_head && valid) ? per_head[head] * 1.4426950408889634f : 0.f;
         const float unit = (cap_log2 > 0.f ? 2.f * scale_log2 * 1.4426950408889634f / cap_log2 : scale_log2) *
                            (mapped && per_head && valid ? per_head[head] : 1.f);
-        const float to_log2 = mapped ? 1.f : scale_log2;          // what is left to multiply the (mapped) scores by
+        const float to_log2 = mapped ? 1.f : FOUR ? scale_log2 * row_factor[tid] : scale_log2;          // what is left to multiply the (mapped) scores by
         bool ok = true;
         for (int j = 0; j < n_tiles; ++j) {
             ok = __all_sync(FULL, mbar_wait(&s_ready[ti][j & 1], (j >> 1) & 1, &give_up));
@@ -568,8 +740,9 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
             tmem_issue_load32(s_addr + 32, raw + 32);
             tmem_arrived<KEYS>(raw);
             const int key0 = listed_tile<KEYS>(t_begin + j, kept, lo) * KEYS;
-            const bool unmasked = key0 + KEYS - 1 <= pos_min && (key0 >= lo_max || key0 + KEYS <= keep);      // for the whole warp
-            const Edges edges = {pos - key0, row_lo - key0, keep - key0};
+            const unsigned gone = FOUR ? gone_of[j % KV_STAGES] : 0u;
+            const bool unmasked = key0 + KEYS - 1 <= pos_min && (key0 >= lo_max || key0 + KEYS <= keep) && gone == 0;      // for the whole warp
+            const Edges edges = {pos - key0, row_lo - key0, keep - key0, gone};
             if (sigmoid) {
                 if (unmasked) row_sigmoid<false>(raw, s_addr, edges, scale_log2, bias);
                 else row_sigmoid<true>(raw, s_addr, edges, scale_log2, bias);
@@ -601,13 +774,28 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
                 m_ref = m_new;
             }
             const float m_safe = m_ref == -CUDART_INF_F ? 0.f : m_ref;
-            row_sum += unmasked ? row_exp<false>(raw, s_addr, edges, to_log2, m_safe)
-                                : row_exp<true>(raw, s_addr, edges, to_log2, m_safe);
+            row_sum += unmasked ? row_exp<false, FOUR>(raw, s_addr, edges, to_log2, m_safe)
+                                : row_exp<true, FOUR>(raw, s_addr, edges, to_log2, m_safe);
             tmem_store_wait();
             tc_fence_before();
             mbar_arrive(&p_ready[ti][j & 1]);
         }
         if (ok) ok = __all_sync(FULL, mbar_wait(&o_final[ti], 0, &give_up));
+        // bit g: this row sees a value whose group g reads as NaN
+        unsigned poisoned = 0;
+        if (FOUR && ok && saw_nan) {
+            for (int j = 0; j < n_tiles && valid; ++j) {
+                const int key0 = listed_tile<KEYS>(t_begin + j, kept, lo) * KEYS;
+                for (int key = key0; key < key0 + KEYS; ++key) {
+                    if (key > pos || (key < row_lo && key >= keep)) continue;
+                    const int page = block_table[(size_t)r * bt_stride + key / ps];
+                    if (page < 0 || page >= num_pages) continue;
+                    const unsigned char* tile = reinterpret_cast<const unsigned char*>(kc) + (((long long)page * nkv + kvh) * (ps / KV4_TILE) + key % ps / KV4_TILE) * SUB_BYTES;
+                    for (int g = 0; g < GROUPS; ++g)
+                        if (__hisnan(*reinterpret_cast<const __half*>(tile + kv4_value_pairs(GROUPS) + (key % KV4_TILE * GROUPS + g) * 4))) poisoned |= 1u << g;
+                }
+            }
+        }
         // partial results are staged where keys and values lay: the other row tile must have read its last ones
         if (ok && splits > 1 && two) ok = __all_sync(FULL, mbar_wait(&o_final[ti ^ 1], 0, &give_up));
         if (ok && splits == 1) {
@@ -622,6 +810,12 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
                 tmem_load32(o_addr + c, v);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] *= inv;
+                if (FOUR) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) in_order(v + i);
+                    if (poisoned >> (c / 32) & 1u)
+                        for (int i = 0; i < 32; ++i) v[i] = CUDART_NAN_F;
+                }
 #pragma unroll
                 for (int i = 0; i < 32; i += 8)
                     store8<bf16>(reinterpret_cast<bf16*>(stage + lane * (2 * D) + ((((c + i) >> 3) ^ (lane & 7)) << 4)), v + i);
@@ -645,6 +839,12 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
             for (int c = 0; c < D; c += 32) {
                 float v[32];
                 tmem_load32(o_addr + c, v);
+                if (FOUR) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) in_order(v + i);
+                    if (poisoned >> (c / 32) & 1u)
+                        for (int i = 0; i < 32; ++i) v[i] = CUDART_NAN_F;
+                }
 #pragma unroll
                 for (int i = 0; i < 32; i += 4)
                     *reinterpret_cast<float4*>(stage + lane * D + ((((c + i) >> 2) ^ (lane & 7)) << 2)) =
@@ -705,13 +905,13 @@ prefill_merge_kernel(const float* __restrict__ part_o, const float* __restrict__
     }
 }
 
-template <int D>
+template <int D, bool FOUR = false>
 int launch(const void* q, long long q_stride, void* out, long long out_stride, const void* kc, const void* vc,
            const int* block_table, int bt_stride, const int* cu_q, const int* q_start, int requests, int max_q_len, int nq,
            int nkv, int ps, int num_pages, float scale, int window, int keep, int sink, int splits, float* scratch, long long total_tokens,
            int* status, const float* per_head, float softcap, cudaStream_t stream) {
-    const size_t smem = (size_t)(D / 64) * (2 * Q_BLOCK + 2 * KV_STAGES * KV_BLOCK) + 1024;
-    const cudaError_t err = cudaFuncSetAttribute(paged_prefill_tcgen05_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const size_t smem = (size_t)(D / 64) * (2 * Q_BLOCK + 2 * KV_STAGES * KV_BLOCK) + 1024 + (FOUR ? RAW_STAGES * SUBTILES * kv4_tile_bytes(D / KV4_GROUP) : 0);
+    const cudaError_t err = cudaFuncSetAttribute(paged_prefill_tcgen05_kernel<D, FOUR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     FE_REQUIRE(err == cudaSuccess, "paged_prefill_tcgen05: %s", cudaGetErrorString(err));
     // every request's pairs of row tiles: as many as the longest one's each, and at most one more each than the rows fill
     const long long group = nq / nkv, each = (max_q_len * group + 2 * ROWS - 1) / (2 * ROWS) * requests;
@@ -721,7 +921,7 @@ int launch(const void* q, long long q_stride, void* out, long long out_stride, c
     // partial results: [token, head, split, D] float32, then [token, head, split] logarithms of the sums
     float* part_o = splits > 1 ? scratch : nullptr;
     float* part_lse = splits > 1 ? scratch + (size_t)total_tokens * nq * splits * D : nullptr;
-    fe::launch(paged_prefill_tcgen05_kernel<D>, dim3((unsigned)blocks), THREADS, smem, stream, (const bf16*)q, q_stride,
+    fe::launch(paged_prefill_tcgen05_kernel<D, FOUR>, dim3((unsigned)blocks), THREADS, smem, stream, (const bf16*)q, q_stride,
                (bf16*)out, out_stride, (const bf16*)kc, (const bf16*)vc, block_table, bt_stride, cu_q, q_start, requests, nq, nkv, ps,
                num_pages, scale * LOG2E, window, keep, sink, splits, part_o, part_lse, status, per_head, softcap * LOG2E);
     if (fe_check_launch("paged_prefill_tcgen05")) return 1;
@@ -765,4 +965,25 @@ extern "C" int fe_paged_prefill_tcgen05(const void* q, long long q_stride, void*
                           ps, num_pages, scale, window, keep, sink, splits, (float*)scratch, total_tokens, status, per_head, softcap, stream);
     return launch<128>(q, q_stride, out, out_stride, kc, vc, block_table, bt_stride, cu_q, q_start, requests, max_q_len, nq, nkv, ps,
                        num_pages, scale, window, keep, sink, splits, (float*)scratch, total_tokens, status, per_head, softcap, stream);
+}
+
+// The same over a cache held in 4 bits: uint8 [pages, nkv, page size / 16, 640 ceil(d / 32)]; softmax weights, windows and kept keys, a sink.
+extern "C" int fe_paged_prefill_kv4(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, const int* block_table,
+                                    int bt_stride, const int* cu_q, const int* q_start, int requests, int max_q_len, int nq, int nkv, int d, int ps,
+                                    int num_pages, float scale, int window, int keep, int sink, int splits, void* scratch, long long total_tokens,
+                                    int* status, cudaStream_t stream) {
+    FE_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "paged_prefill_kv4: bad head counts %d/%d", nq, nkv);
+    FE_REQUIRE(d == 64 || d == 128, "paged_prefill_kv4: head size %d; this kernel takes 64 and 128", d);
+    FE_REQUIRE(ps > 0 && ps % KV4_TILE == 0 && num_pages > 0, "paged_prefill_kv4: page size %d (a multiple of %d) or page count", ps, KV4_TILE);
+    FE_REQUIRE((long long)num_pages * nkv * (ps / KV4_TILE) < (1LL << 31), "paged_prefill_kv4: %d pages are too many", num_pages);
+    FE_REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0 && (((size_t)q | (size_t)out | (size_t)cache) & 15) == 0, "paged_prefill_kv4: rows must start on 16-byte boundaries");
+    FE_REQUIRE(requests >= 0 && max_q_len >= 0 && window >= 0 && keep >= 0 && (keep == 0 || window > 0), "paged_prefill_kv4: bad request count or length, or kept keys without a window");
+    FE_REQUIRE(splits >= 1 && splits <= MAX_SPLITS && total_tokens > 0 && (splits == 1 || (scratch != nullptr && ((size_t)scratch & 15) == 0)),
+               "paged_prefill_kv4: %d splits (1 to %d) without scratch, or no tokens", splits, MAX_SPLITS);
+    if (requests == 0 || max_q_len == 0) return 0;
+    if (d == 64)
+        return launch<64, true>(q, q_stride, out, out_stride, cache, nullptr, block_table, bt_stride, cu_q, q_start, requests, max_q_len, nq, nkv, ps,
+                                num_pages, scale, window, keep, sink != 0, splits, (float*)scratch, total_tokens, status, nullptr, 0.f, stream);
+    return launch<128, true>(q, q_stride, out, out_stride, cache, nullptr, block_table, bt_stride, cu_q, q_start, requests, max_q_len, nq, nkv, ps,
+                             num_pages, scale, window, keep, sink != 0, splits, (float*)scratch, total_tokens, status, nullptr, 0.f, stream);
 }

@@ -1871,6 +1871,30 @@ def kv4_rows(cache, slots, nkv, d, page_size, dtype=torch.bfloat16):
     return keys, values
 
 
+def kv4_portions(lengths, starts, nq: int, nkv: int, d: int, window: int = 0, tensor: bool = True, resident: int = 444, sms: int | None = None) -> int:
+    """How portions over a 4-bit cache are taken: 0 the tcgen05 kernel (``tensor``: the step's type and head size allow it), S > 0 the kernel of
+    single tokens in clusters of S blocks.  What either takes, in microseconds (28/4 heads of 128; a tile is 16 keys, an item 256 rows): the
+    one of single tokens 7 and 1 for 1,600 (tile of eight rows, key tile) pairs, or 0.13 for each key tile that one block walks; tcgen05 16 and 1.3 for each 64 keys of
+    an item, all items shared out over the multiprocessors.  32 portions of 4 tokens after 2,000 take 36 and 59, 8 of 32 after 1,000 35 and 25, one of 2,048 309
+    and 63."""
+    group = nq // nkv
+    pairs = item_tiles = blocks = longest = 0
+    for n, s in zip(lengths, starts):
+        keys = min(s + n, window + n) if window > 0 else s + n
+        tiles, columns = -(-keys // KV4_TILE), -(-n * group // 8) * nkv
+        longest, blocks = max(longest, tiles), blocks + columns
+        # of a portion at the start of its sequence the first rows see little
+        seen = keys - min(n, keys) / 2
+        pairs += columns * seen / KV4_TILE
+        item_tiles += nkv * -(-n * group // 256) * seen / 64
+    # a cluster costs about 3 us: for walks of more than 64 tiles
+    splits = max(1, min(8, resident // max(1, blocks), longest // 8)) if longest > 64 else 1
+    if not tensor:
+        return splits
+    light = 7 + max(pairs / 1600, 0.13 * longest / splits)
+    return splits if light <= 16 + 1.3 * item_tiles / (sms or sm_count()) else 0
+
+
 _KV4_PLANS: dict = {}
 
 
@@ -1907,7 +1931,19 @@ def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale
         if ctx.max_ctx_len > pages * page_size:
             raise ValueError(f"{what}: {ctx.max_ctx_len} tokens in {pages} pages of {page_size}")
         out = torch.empty((T, nq * d), dtype=q.dtype, device=q.device)
-        lib, splits, blocks, part = _kv4(), 1, 0, None
+        lengths, starts = getattr(ctx, "host_lengths", None), getattr(ctx, "host_starts", None)
+        clusters = 1
+        if ctx.max_q_len > 1 and T:
+            tensor = code == 1 and d in (64, 128)
+            clusters = kv4_portions(lengths, starts, nq, nkv, d, window, tensor) if lengths else 0 if tensor else 1
+        if clusters == 0:
+            splits = prefill_splits(lengths, starts, nq, nkv, window) if lengths else 1
+            part = torch.empty(T * nq * splits * (d + 1), dtype=torch.float32, device=q.device) if splits > 1 else None
+            _run(_bf16(), "fe_paged_prefill_kv4", q.data_ptr(), q.stride(0) if T > 1 else nq * d, out.data_ptr(), nq * d, cache.data_ptr(), block_table.data_ptr(), pages,
+                 ctx.cu_q.data_ptr(), ctx.q_start.data_ptr(), requests, ctx.max_q_len, nq, nkv, d, page_size, cache.shape[0], float(scale), window, keep_first,
+                 1 if sink else 0, splits, _ptr(part), T, status_word(q.device).data_ptr(), _stream())
+            return out
+        lib, splits, blocks, part = _kv4(), clusters, 0, None
         if ctx.max_q_len == 1:
             span = ctx.max_ctx_len if window == 0 else min(ctx.max_ctx_len, window + keep_first + 2 * KV4_TILE)
             plan, nbytes = kv4_plan(requests, -(-span // KV4_TILE), nq, nkv, d, code)

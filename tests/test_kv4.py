@@ -267,3 +267,19 @@ def test_operators_want_cuda_tensors():
         ops.qkv_rope_kv4(**store_arguments())
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.paged_attention_kv4(**attention_arguments())
+
+
+# ---- which kernel takes portions ----------------------------------------------------------------------------------------------
+def test_portions_choose_their_kernel():
+    from flexengine_b200.ops import kv4_portions
+
+    def of(n, context, new, **more):
+        return kv4_portions([new] * n, [context - new] * n, 28, 4, 128, sms=148, **more)
+
+    assert of(1, 2048, 2048) == 0 and of(4, 4096, 512) == 0 and of(8, 1000, 32) == 0            # long portions: tcgen05
+    assert of(1, 300, 4) == 1 and of(32, 500, 2) == 1 and of(32, 2000, 4) == 1                    # few rows, enough blocks or short walks
+    assert of(1, 4000, 2) == 8                                                                    # few rows late in a context: clusters
+    assert of(1, 2048, 2048, tensor=False) == 1 and of(1, 4000, 2, tensor=False) == 8             # head sizes and types that tcgen05 does not take
+    assert of(1, 100000, 1000, window=64) in (0, 1)
+    assert kv4_portions([0, 3], [50, 0], 4, 2, 64, sms=148) == 1
+    assert kv4_portions([1], [0], 64, 1, 64, sms=148) == 1
