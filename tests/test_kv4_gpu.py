@@ -62,7 +62,8 @@ def check_stored(cache, slots, keys, values, what=""):
 @pytest.mark.parametrize("T,nq,nkv,d,rot,pairs,page,bias,wider", [
     (1, 28, 4, 128, 128, "halves", 16, True, 0), (1, 2, 1, 16, 0, "halves", 16, False, 0), (5, 3, 3, 48, 6, "halves", 32, True, 0),
     (37, 14, 2, 64, 32, "interleaved", 16, False, 8), (33, 6, 2, 80, 80, "interleaved", 48, True, 0), (17, 8, 1, 256, 200, "halves", 64, True, 4),
-    (300, 16, 8, 112, 112, "halves", 16, False, 3), (149, 4, 2, 208, 14, "interleaved", 16, True, 1)])
+    (300, 16, 8, 112, 112, "halves", 16, False, 3), (2000, 4, 2, 128, 128, "halves", 16, True, 0), (901, 3, 1, 64, 32, "interleaved", 32, False, 4),
+    (700, 2, 2, 256, 192, "halves", 16, True, 0), (777, 3, 1, 80, 20, "halves", 16, True, 2), (149, 4, 2, 208, 14, "interleaved", 16, True, 1)])
 def test_store(source, out, T, nq, nkv, d, rot, pairs, page, bias, wider, gen):
     width = (nq + 2 * nkv) * d
     projected = normal(gen, T, width + wider).to(source)[:, :width] if wider else normal(gen, T, width).to(source)
