@@ -65,6 +65,14 @@ __device__ __forceinline__ unsigned pack(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const unsigned*>(&h);
 }
+// Four pairs times a pair plus another
+__device__ __forceinline__ void times_plus(unsigned* n, unsigned scale, unsigned centre) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&n[i]), *reinterpret_cast<const __half2*>(&scale), *reinterpret_cast<const __half2*>(&centre));
+        n[i] = *reinterpret_cast<const unsigned*>(&x);
+    }
+}
 // what ``pack`` left over of the two
 __device__ __forceinline__ unsigned pack_rest(float lo, float hi, unsigned packed) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&packed));
@@ -151,10 +159,13 @@ struct Problem {
     int* status;
 };
 
-// dynamic shared memory: every warp's ring (two places of a pair of tiles each), then the warps' results
+// dynamic shared memory: every warp's ring, two places of a pair of tiles each; a warp's results go to the place that no copy is on its way to
 constexpr int STAGES = 2;
 template <int NG> __host__ __device__ constexpr int ring_bytes() { return WARPS * STAGES * PAIR * kv4_tile_bytes(NG); }
-template <int NG, int NT> __host__ __device__ constexpr int smem_bytes() { return ring_bytes<NG>() + WARPS * 8 * NT * (32 * NG + 4) * 4; }
+template <int NG, int NT> __host__ __device__ constexpr int smem_bytes() {
+    static_assert(8 * NT * (32 * NG + 4) * 4 <= PAIR * kv4_tile_bytes(NG), "a warp's results fit a pair of tiles");
+    return ring_bytes<NG>();
+}
 
 // One piece of work of a block: tiles [t_begin, t_end) of the list that the columns from m0 on of (request r, head kvh) see.
 struct Segment {
@@ -183,7 +194,7 @@ __device__ __forceinline__ int tiles_of(const Problem& a, int r) {
 }
 
 // Blocks that are resident on an SM: the registers are cut to that.  16-bit queries at head size 128: three blocks of 168 registers a thread.
-template <typename TQ, int NG, int NT> __host__ __device__ constexpr int blocks_an_sm() { return sizeof(TQ) == 2 && NG * NT <= 4 ? 3 : 2; }
+template <typename TQ, int NG, int NT> __host__ __device__ constexpr int blocks_an_sm() { return sizeof(TQ) == 2 && NG * NT <= 4 ? 4 : 2; }
 
 // TQ: queries and output; 32-bit ones in two parts.  NG: groups of a row.  NT: tiles of eight columns that a block takes.
 //
@@ -204,6 +215,8 @@ kv4_attention_kernel(const Problem a) {
     griddep_wait();
     griddep_launch_dependents();
     constexpr int PARTS = sizeof(TQ) == 4 ? 2 : 1;
+    constexpr bool EXACT = PARTS == 2;                   // scales and centres of values in 32 bits
+    constexpr int GONE = 0x40000000;                     // a key that nobody sees
     constexpr int COLS = 8 * NT, TILE = kv4_tile_bytes(NG);
     constexpr unsigned FULL = 0xffffffffu;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -216,6 +229,9 @@ kv4_attention_kernel(const Problem a) {
 
     // ---- what this block does; each warp keeps the piece in hand in shared memory, for the registers' sake
     __shared__ Segment pieces_of[WARPS];
+    __shared__ __align__(16) uint4 operands[PARTS][NT][NG][32];           // of the queries; the four warps make them together and read them as they go
+    __shared__ __align__(8) float2 lifts[NT][NG][32];
+    __shared__ int last_keys[COLS], first_keys[COLS];
     Segment& w = pieces_of[warp];
     Segment found{};
     constexpr int ROUND = PAIR * WARPS;
@@ -301,7 +317,8 @@ kv4_attention_kernel(const Problem a) {
     const int even_codes = kv4_value_codes(NG) + even * 16 * NG + g * 2 * NG, odd_codes = kv4_value_codes(NG) + odd * 16 * NG + g * 2 * NG;
     const int per_page = a.ps / KV4_TILE;
     unsigned char* ring = smem + warp * STAGES * PAIR * TILE;
-    float* results = reinterpret_cast<float*>(smem + ring_bytes<NG>());
+    __shared__ int result_place[WARPS];
+    auto results_of = [&](int w) { return reinterpret_cast<float*>(smem + (w * STAGES + (SHARED ? result_place[w] : 0)) * PAIR * TILE); };
     unsigned stage = 0, parity = 0;
     bool gone = false;
 
@@ -347,11 +364,10 @@ kv4_attention_kernel(const Problem a) {
         // they are off by about 2^-24 8,000, a thousandth of what rounding the query to bfloat16 did.  (Values are summed over all keys,
         // where the part of 1024 would grow: they are decoded in full, and so are keys under 32-bit queries.)
         constexpr bool RAISED = PARTS == 1;
-        unsigned qf[NT][NG][4][PARTS], qsum[NT][2];          // qsum: (high, low) of the sums over group t, and over group t + 4
-        float lift[NT][NG][2];
+        unsigned qsum[NT][2];                                // (high, low) of the sums over group t, and over group t + 4
         float factor[NT][2];                                 // takes a score of columns 2t, 2t + 1 to log2 units
-        int last_key[NT][2], first_key[NT][2];
         float below[NT][2], l[NT][2];                        // minus the reference point (infinite before the first key), the sum
+        int last_least = 0x7fffffff, first_most = 0;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int c = m0 + 8 * j + g;
@@ -372,47 +388,48 @@ kv4_attention_kernel(const Problem a) {
             // a power of two brings the row's largest number to [1, 2): half precision then holds bfloat16 numbers as they are
             const int e2 = min(max((int)(__float_as_uint(largest) >> 23) - 127, -126), 126);
             const float down = __uint_as_float((unsigned)(127 - e2) << 23);
-            float sums[NG];
+            float group_sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
-                sums[i] = 0.f;
+                float sum = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { v[i][e] *= down; sums[i] += v[i][e]; }
-                sums[i] += __shfl_xor_sync(FULL, sums[i], 1);
-                sums[i] += __shfl_xor_sync(FULL, sums[i], 2);
+                for (int e = 0; e < 8; ++e) { v[i][e] *= down; sum += v[i][e]; }
+                sum += __shfl_xor_sync(FULL, sum, 1);
+                sum += __shfl_xor_sync(FULL, sum, 2);
+                if (i == t) group_sum[0] = sum;
+                if (i == t + 4) group_sum[1] = sum;
+                if (i % WARPS != warp) continue;                          // the other warps make the other groups' operands
+                unsigned high[4], rest[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    qf[j][i][e][0] = pack(v[i][e], v[i][e + 4]);
-                    if (PARTS == 2) qf[j][i][e][PARTS - 1] = pack_rest(v[i][e], v[i][e + 4], qf[j][i][e][0]);
+                    high[e] = pack(v[i][e], v[i][e + 4]);
+                    if (PARTS == 2) rest[e] = pack_rest(v[i][e], v[i][e + 4], high[e]);
                 }
+                operands[0][j][i][lane] = make_uint4(high[0], high[1], high[2], high[3]);
+                if (PARTS == 2) operands[PARTS - 1][j][i][lane] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
                 float raised = 0.f;
                 if (RAISED) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        raised -= ((e & 1 ? KV4_RAISED_ODD : KV4_RAISED_EVEN) + 8.f) * (low_half(qf[j][i][e][0]) + high_half(qf[j][i][e][0]));
+                        raised -= ((e & 1 ? KV4_RAISED_ODD : KV4_RAISED_EVEN) + 8.f) * (low_half(high[e]) + high_half(high[e]));
                     raised += __shfl_xor_sync(FULL, raised, 1);
                     raised += __shfl_xor_sync(FULL, raised, 2);
                 }
-                lift[j][i][0] = __shfl_sync(FULL, raised, 8 * t);             // of columns 2t and 2t + 1
-                lift[j][i][1] = __shfl_sync(FULL, raised, 8 * t + 4);
+                lifts[j][i][lane] = make_float2(__shfl_sync(FULL, raised, 8 * t), __shfl_sync(FULL, raised, 8 * t + 4));      // of columns 2t and 2t + 1
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float s = 0.f;
-#pragma unroll
-                for (int i = 0; i < NG; ++i)
-                    if (i == t + 4 * h) s = sums[i];
-                const float high = __half2float(__float2half_rn(s));
-                qsum[j][h] = pack(high, s - high);
+                const float high = __half2float(__float2half_rn(group_sum[h]));
+                qsum[j][h] = pack(high, group_sum[h] - high);
             }
+            // a padding column sees what the last query sees: it is computed and never written, and must not make a tile a masked one
+            const int pos = real ? start + c / G : w.hi, from = real ? first_visible(pos, a.window) : lo;
+            last_least = min(last_least, pos);
+            first_most = max(first_most, from);
+            if (warp == 0 && t == 0) { last_keys[8 * j + g] = pos; first_keys[8 * j + g] = from; }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int mc = m0 + 8 * j + 2 * t + h;
                 factor[j][h] = a.scale_log2 * __uint_as_float((unsigned)(127 + __shfl_sync(FULL, e2, (2 * t + h) * 4)) << 23);
-                // a padding column sees what the last query sees: it is computed and never written, and must not make a tile a masked one
-                const int pos = mc < columns ? start + mc / G : w.hi;
-                last_key[j][h] = pos;
-                first_key[j][h] = mc < columns ? first_visible(pos, a.window) : lo;
                 below[j][h] = CUDART_INF_F;
                 l[j][h] = 0.f;
                 if (a.sink && t_begin == 0 && warp == 0) {
@@ -421,13 +438,9 @@ kv4_attention_kernel(const Problem a) {
                 }
             }
         }
-        int last_least = last_key[0][0], first_most = first_key[0][0];
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) { last_least = min(last_least, last_key[j][h]); first_most = max(first_most, first_key[j][h]); }
         last_least = __reduce_min_sync(FULL, last_least);
         first_most = __reduce_max_sync(FULL, first_most);
+        __syncthreads();
 
         float o[NT][NG][2][4], oc[NT][NG][2];                // sums over codes, 16 numbers a tile, and over centres (this thread's tokens)
 #pragma unroll
@@ -479,11 +492,14 @@ kv4_attention_kernel(const Problem a) {
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         float part[4];
-                        mma_from(part, n0[0], n1[0], n0[1], n1[1], qf[j][i][0][0], qf[j][i][1][0], lift[j][i][0], lift[j][i][1]);
-                        mma(part, n0[2], n1[2], n0[3], n1[3], qf[j][i][2][0], qf[j][i][3][0]);
+                        const uint4 q = operands[0][j][i][lane];
+                        const float2 lift = RAISED ? lifts[j][i][lane] : make_float2(0.f, 0.f);
+                        mma_from(part, n0[0], n1[0], n0[1], n1[1], q.x, q.y, lift.x, lift.y);
+                        mma(part, n0[2], n1[2], n0[3], n1[3], q.z, q.w);
                         if (PARTS == 2) {
-                            mma(part, n0[0], n1[0], n0[1], n1[1], qf[j][i][0][PARTS - 1], qf[j][i][1][PARTS - 1]);
-                            mma(part, n0[2], n1[2], n0[3], n1[3], qf[j][i][2][PARTS - 1], qf[j][i][3][PARTS - 1]);
+                            const uint4 rest = operands[PARTS - 1][j][i][lane];
+                            mma(part, n0[0], n1[0], n0[1], n1[1], rest.x, rest.y);
+                            mma(part, n0[2], n1[2], n0[3], n1[3], rest.z, rest.w);
                         }
                         s[u][j][0] = fmaf(s0, part[0], s[u][j][0]);
                         s[u][j][1] = fmaf(s0, part[1], s[u][j][1]);
@@ -493,37 +509,44 @@ kv4_attention_kernel(const Problem a) {
                 }
             }
             // ---- weights
-            unsigned v0[PAIR][NG], v1[PAIR][NG];                          // (scale, centre) of the two tokens' value groups
+            unsigned v0[PAIR][NG], v1[PAIR][NG];                          // EXACT: (scale, centre) of the two tokens' value groups
             float up0[PAIR], up1[PAIR], y[PAIR][NT][4];
             bool grows = false;
 #pragma unroll
             for (int u = 0; u < PAIR; ++u) {
-                words<NG>(pair + u * TILE + key_pairs + 64 * NG, v0[u]);
-                words<NG>(pair + u * TILE + key_pairs + 96 * NG, v1[u]);
+                up0[u] = up1[u] = 0.f;
+                if (EXACT || MASKED) {
+                    words<NG>(pair + u * TILE + key_pairs + 64 * NG, v0[u]);
+                    words<NG>(pair + u * TILE + key_pairs + 96 * NG, v1[u]);
+                }
                 if (MASKED) {
-                    const int key0 = (here >> u & 1u) ? listed_tile<KV4_TILE>(place + u, kept, lo) * KV4_TILE : 0x40000000;
-                    unsigned nan0 = 0, nan1 = 0;                          // groups that read as NaN; what was never written may
+                    const int key0 = (here >> u & 1u) ? listed_tile<KV4_TILE>(place + u, kept, lo) * KV4_TILE : GONE;
+                    unsigned nan0 = 0, nan1 = 0;                          // groups that read as NaN
 #pragma unroll
                     for (int i = 0; i < NG; ++i) {
                         if ((v0[u][i] & 0x7c00u) == 0x7c00u) { nan0 |= 1u << (2 * i); v0[u][i] = 0; }
                         if ((v1[u][i] & 0x7c00u) == 0x7c00u) { nan1 |= 1u << (2 * i); v1[u][i] = 0; }
-                        if (!(here >> u & 1u)) v0[u][i] = v1[u][i] = 0;   // what lay there before may be anything
+                        if (key0 + key_row > w.hi) v0[u][i] = 0;          // behind the last token: what lies there may be anything
+                        if (key0 + key_row + 8 > w.hi) v1[u][i] = 0;
                     }
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int key = key0 + key_row + (e & 2) * 4;
-                            if (!(key <= last_key[j][e & 1] && (key >= first_key[j][e & 1] || key < a.keep))) s[u][j][e] = -CUDART_INF_F;
+                            const int column = 8 * j + 2 * t + (e & 1);
+                            if (!(key <= last_keys[column] && (key >= first_keys[column] || key < a.keep))) s[u][j][e] = -CUDART_INF_F;
                             else poisoned |= (e < 2 ? nan0 : nan1) << (2 * NG * j + (e & 1));
                         }
                 }
-                float big0 = low_half(v0[u][0]), big1 = low_half(v1[u][0]);
+                if (EXACT) {
+                    float big0 = low_half(v0[u][0]), big1 = low_half(v1[u][0]);
 #pragma unroll
-                for (int i = 1; i < NG; ++i) { big0 = fmaxf(big0, low_half(v0[u][i])); big1 = fmaxf(big1, low_half(v1[u][i])); }
-                // their exponents; zeros and subnormal numbers count as 2^-24, the least scale there is
-                up0[u] = fmaxf((float)(__float_as_uint(big0) >> 23) - 127.f, -24.f);
-                up1[u] = fmaxf((float)(__float_as_uint(big1) >> 23) - 127.f, -24.f);
+                    for (int i = 1; i < NG; ++i) { big0 = fmaxf(big0, low_half(v0[u][i])); big1 = fmaxf(big1, low_half(v1[u][i])); }
+                    // their exponents; zeros and subnormal numbers count as 2^-24, the least scale there is
+                    up0[u] = fmaxf((float)(__float_as_uint(big0) >> 23) - 127.f, -24.f);
+                    up1[u] = fmaxf((float)(__float_as_uint(big1) >> 23) - 127.f, -24.f);
+                }
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -549,7 +572,7 @@ kv4_attention_kernel(const Problem a) {
                         l[j][h] *= by;
 #pragma unroll
                         for (int i = 0; i < NG; ++i) {
-                            oc[j][i][h] *= by;
+                            if (EXACT) oc[j][i][h] *= by;
                             o[j][i][0][h] *= by; o[j][i][0][h + 2] *= by;
                             o[j][i][1][h] *= by; o[j][i][1][h + 2] *= by;
                         }
@@ -582,22 +605,54 @@ kv4_attention_kernel(const Problem a) {
                 pieces<NG>(tile + odd_codes, vo);
                 pieces<NG>(tile + even_codes + 128 * NG, ve8);
                 pieces<NG>(tile + odd_codes + 128 * NG, vo8);
+                // EXACT = false: one operand of weights for all groups, and scale and centre in the decoded numbers, which half precision rounds by 2^-12
+                unsigned pe[NG], po[NG], pe8[NG], po8[NG], b0[NT], b1[NT];
+                if (!EXACT) {
+                    const unsigned char* pairs = tile + kv4_value_pairs(NG);
+                    words<NG>(pairs + even * 4 * NG, pe);
+                    words<NG>(pairs + odd * 4 * NG, po);
+                    words<NG>(pairs + even * 4 * NG + 32 * NG, pe8);
+                    words<NG>(pairs + odd * 4 * NG + 32 * NG, po8);
+                    if (MASKED) {
+                        const int key0 = (here >> u & 1u) ? listed_tile<KV4_TILE>(place + u, kept, lo) * KV4_TILE : GONE;
+#pragma unroll
+                        for (int i = 0; i < NG; ++i) {
+                            if ((pe[i] & 0x7c00u) == 0x7c00u || key0 + even > w.hi) pe[i] = 0;
+                            if ((po[i] & 0x7c00u) == 0x7c00u || key0 + odd > w.hi) po[i] = 0;
+                            if ((pe8[i] & 0x7c00u) == 0x7c00u || key0 + even + 8 > w.hi) pe8[i] = 0;
+                            if ((po8[i] & 0x7c00u) == 0x7c00u || key0 + odd + 8 > w.hi) po8[i] = 0;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        b0[j] = transposed(pack(y[u][j][0], y[u][j][1]));
+                        b1[j] = transposed(pack(y[u][j][2], y[u][j][3]));
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
                     unsigned na[4], nb[4];
                     kv4_decode(__byte_perm(ve[i / 2], vo[i / 2], (i & 1) ? 0x7632 : 0x5410), na);
                     kv4_decode(__byte_perm(ve8[i / 2], vo8[i / 2], (i & 1) ? 0x7632 : 0x5410), nb);
-                    const float s0 = low_half(v0[u][i]), s1 = low_half(v1[u][i]), c0 = high_half(v0[u][i]), c1 = high_half(v1[u][i]);
+                    if constexpr (!EXACT) {
+                        times_plus(na, __byte_perm(pe[i], po[i], 0x5410), __byte_perm(pe[i], po[i], 0x7632));
+                        times_plus(nb, __byte_perm(pe8[i], po8[i], 0x5410), __byte_perm(pe8[i], po8[i], 0x7632));
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const float* w = y[u][j];
-                        oc[j][i][0] = fmaf(w[0], c0, fmaf(w[2], c1, oc[j][i][0]));
-                        oc[j][i][1] = fmaf(w[1], c0, fmaf(w[3], c1, oc[j][i][1]));
-                        const unsigned w0 = pack(w[0] * s0, w[1] * s0), w1 = pack(w[2] * s1, w[3] * s1);
-                        const unsigned b0 = transposed(w0), b1 = transposed(w1);
-                        mma(o[j][i][0], na[0], na[1], nb[0], nb[1], b0, b1);
-                        mma(o[j][i][1], na[2], na[3], nb[2], nb[3], b0, b1);
-                        if (PARTS == 2) {
+                        for (int j = 0; j < NT; ++j) {
+                            mma(o[j][i][0], na[0], na[1], nb[0], nb[1], b0[j], b1[j]);
+                            mma(o[j][i][1], na[2], na[3], nb[2], nb[3], b0[j], b1[j]);
+                        }
+                    } else {
+                        const float s0 = low_half(v0[u][i]), s1 = low_half(v1[u][i]), c0 = high_half(v0[u][i]), c1 = high_half(v1[u][i]);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            const float* w = y[u][j];
+                            oc[j][i][0] = fmaf(w[0], c0, fmaf(w[2], c1, oc[j][i][0]));
+                            oc[j][i][1] = fmaf(w[1], c0, fmaf(w[3], c1, oc[j][i][1]));
+                            const unsigned w0 = pack(w[0] * s0, w[1] * s0), w1 = pack(w[2] * s1, w[3] * s1);
+                            const unsigned h0 = transposed(w0), h1 = transposed(w1);
+                            mma(o[j][i][0], na[0], na[1], nb[0], nb[1], h0, h1);
+                            mma(o[j][i][1], na[2], na[3], nb[2], nb[3], h0, h1);
                             const unsigned r0 = transposed(pack_rest(w[0] * s0, w[1] * s0, w0)), r1 = transposed(pack_rest(w[2] * s1, w[3] * s1, w1));
                             mma(o[j][i][0], na[0], na[1], nb[0], nb[1], r0, r1);
                             mma(o[j][i][1], na[2], na[3], nb[2], nb[3], r0, r1);
@@ -655,11 +710,14 @@ kv4_attention_kernel(const Problem a) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                     if (poisoned >> (2 * (j * NG + i) + h) & 1u) oc[j][i][h] = CUDART_NAN_F;
+        if (SHARED && lane == 0) result_place[warp] = (int)(stage ^ 1);
+        __syncwarp();
+        float* mine_results = results_of(warp);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float* to = results + (warp * COLS + 8 * j + 2 * t + h) * ROW;
+                float* to = mine_results + (8 * j + 2 * t + h) * ROW;
 #pragma unroll
                 for (int i = 0; i < NG; ++i)
                     *reinterpret_cast<float4*>(to + 32 * i + 4 * g) =
@@ -669,25 +727,29 @@ kv4_attention_kernel(const Problem a) {
         __syncthreads();
         for (int c = warp; c < COLS && m0 + c < columns; c += WARPS) {
             const int mc = m0 + c, token = tok0 + mc / G, head = kvh * G + mc % G;
+            const float* from[WARPS];
             float top = -CUDART_INF_F;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, results[(w * COLS + c) * ROW + 32 * NG]);
+            for (int w = 0; w < WARPS; ++w) {
+                from[w] = results_of(w) + c * ROW;
+                top = fmaxf(top, from[w][32 * NG]);
+            }
             float by[WARPS], sum = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                const float mw = results[(w * COLS + c) * ROW + 32 * NG];
+                const float mw = from[w][32 * NG];
                 by[w] = mw == -CUDART_INF_F ? 0.f : ex2(mw - top);
-                sum += by[w] * results[(w * COLS + c) * ROW + 32 * NG + 1];
+                sum += by[w] * from[w][32 * NG + 1];
             }
             const bool whole = slot < 0;
             const float inv = !whole ? 1.f : sum > 0.f ? 1.f / sum : 0.f;
-            float* part = whole ? nullptr : SHARED ? a.part + ((long long)slot * COLS + c) * ROW : results + c * ROW;      // in place: see below
+            float* part = whole ? nullptr : SHARED ? a.part + ((long long)slot * COLS + c) * ROW : results_of(0) + c * ROW;      // in place: see below
             __syncwarp();                                             // maxima and sums are read
             TQ* to = static_cast<TQ*>(a.out) + (long long)token * a.out_stride + (long long)head * a.d;
             for (int i = lane; i < a.d; i += 32) {
                 float v = 0.f;
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w) v += by[w] != 0.f ? by[w] * results[(w * COLS + c) * ROW + i] : 0.f;
+                for (int w = 0; w < WARPS; ++w) v += by[w] != 0.f ? by[w] * from[w][i] : 0.f;
                 if (whole) put<TQ>(to + i, sum != sum ? sum : v * inv);
                 else part[i] = v;
             }
@@ -700,7 +762,7 @@ kv4_attention_kernel(const Problem a) {
             cluster_barrier();
             for (int c = rank + splits * warp; c < COLS && m0 + c < columns; c += splits * WARPS) {
                 const int mc = m0 + c, token = tok0 + mc / G, head = kvh * G + mc % G;
-                const float* own = results + c * ROW;
+                const float* own = results_of(0) + c * ROW;
                 const float at = lane < (int)splits ? ld_cluster(own + 32 * NG, lane) : -CUDART_INF_F;
                 const float top = warp_max(at), by = at == -CUDART_INF_F ? 0.f : ex2(at - top);
                 const float sum = warp_sum(lane < (int)splits ? by * ld_cluster(own + 32 * NG + 1, lane) : 0.f);
@@ -722,6 +784,7 @@ kv4_attention_kernel(const Problem a) {
             const int b = (int)blockIdx.x;
             held[item] = Held{b, slot < 0 ? b + 1 : item_last / share + 1};
         }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");     // copies may go where results were written
         __syncthreads();                                                  // the results are read: the next piece's go there
     }
 }
