@@ -887,8 +887,7 @@ template <typename TQ, int NG, int NT> int run(const Launch& w) {
     constexpr int smem = smem_bytes<NG, NT>();
     const Problem& a = *w.a;
     auto kernel = w.blocks ? kv4_attention_kernel<TQ, NG, NT, true> : kv4_attention_kernel<TQ, NG, NT, false>;
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    FE_REQUIRE(err == cudaSuccess, "paged_attention_kv4: %s", cudaGetErrorString(err));
+    FE_REQUIRE(fe_allow_smem((const void*)kernel, smem), "paged_attention_kv4: no kernel with %d bytes of shared memory", smem);
     const dim3 grid = w.blocks ? dim3((unsigned)w.blocks) : dim3((unsigned)(w.column_tiles * a.splits), (unsigned)a.nkv, (unsigned)w.requests);
     if (!w.blocks && a.splits > 1) {
         cudaLaunchConfig_t cfg = {};

@@ -168,6 +168,7 @@ void fe_set_error(const char* fmt, ...);
 int fe_check_launch(const char* what);
 int fe_pdl_enabled();
 void fe_share_carveout(const void* kernel);       // the split of an SM's memory that overlapping kernels share
+bool fe_allow_smem(const void* kernel, int bytes);      // up to so many bytes of dynamic shared memory for the kernel on the current device
 int fe_sm_count();      // multiprocessors of the current device (asked once per device)
 
 // Classes of kernels for fe_set_pdl: a source file names its own before including this header.

@@ -70,6 +70,32 @@ void fe_share_carveout(const void* kernel) {
     }
 }
 
+// A kernel's largest block of dynamic shared memory is the driver's to know: told once a kernel, size and device, since a launch should not pay for
+// the call (about a microsecond).
+bool fe_allow_smem(const void* kernel, int bytes) {
+    constexpr int SLOTS = 256;
+    static std::atomic<const void*> kernels[64][SLOTS];
+    static std::atomic<int> allowed[64][SLOTS];
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return false;
+    size_t at = ((size_t)kernel >> 4) % SLOTS;
+    for (int i = 0; i < SLOTS; ++i, at = (at + 1) % SLOTS) {
+        const void* have = kernels[device][at].load(std::memory_order_acquire);
+        if (have == kernel && allowed[device][at].load(std::memory_order_relaxed) >= bytes) return true;
+        if (have == kernel || have == nullptr) {
+            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+                cudaGetLastError();
+                return false;
+            }
+            const void* none = nullptr;
+            if (have == nullptr && !kernels[device][at].compare_exchange_strong(none, kernel)) return true;      // another thread took the place: asked again next time
+            allowed[device][at].store(bytes, std::memory_order_relaxed);
+            return true;
+        }
+    }
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+}
+
 extern "C" const char* fe_last_error() { return g_last_error; }
 
 extern "C" int fe_abi_version() { return 1; }

@@ -393,8 +393,7 @@ int store(const void* src, long long ld, const float* bias, const int* positions
     const size_t smem = stay_bytes(width, sizeof(TI));
     if (T >= 4 * sms && vec && turn.rot % 4 == 0 && (size_t)src % 16 == 0 && ld * sizeof(TI) % 16 == 0 && smem <= 110 * 1024) {
         auto kernel = kv4_store_many_kernel<TI, TO>;
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        FE_REQUIRE(err == cudaSuccess, "qkv_rope_kv4: %s", cudaGetErrorString(err));
+        FE_REQUIRE(fe_allow_smem((const void*)kernel, (int)smem), "qkv_rope_kv4: no kernel with %d bytes of shared memory", (int)smem);
         // not among the overlapping launches: the split of an SM's memory that they share leaves room for one such block, not two
         fe::launch_as(0, kernel, dim3((unsigned)(2 * sms)), STAY_WARPS * 32, smem, stream, (const TI*)src, ld, bias, positions, turn, slots, (unsigned char*)cache,
                    (TO*)queries, T, nq, nkv, d, ps, num_slots, status);

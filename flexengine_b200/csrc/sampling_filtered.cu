@@ -6,16 +6,19 @@
 // sum.  T = 0: the lowest index of the maximum.  NaN counts as -inf.  Beside the token: its probability among those that stayed, and their number.
 //
 // Masses are whole numbers of 2^-44 of the largest (fewer bits over 2^18 tokens), so their sums are exact in any order: the result depends neither
-// on the number of blocks a row has nor on what else is in the batch.  Where tens of thousands of tokens stay, one is 1e-5 of the sum or
-// less, and equal ones share their error, so masses are taken in 64 bits.
+// on the number of blocks a row has nor on what else is in the batch.
 //
 // A row belongs to a thread-block cluster, each block with a contiguous part of it.  Sorting is avoided.  A walk finds the maximum; a second one
 // counts the tokens (for top-k) and adds up their masses to 13 bits (for top-p) by their distance to the maximum, in 4,096 steps of 1/128.  In
 // the step at which the count or the mass passes its limit a few hundred tokens are left to be looked at one by one.  If that step and all
 // before it hold no more than LIST tokens (small k, peaked rows), they are listed and the rest of the work is done on the list, each token
 // against each other.  Else one more walk adds up exactly what lies before the step and lists the step itself; a step with more tokens than the list
-// takes (equal logits, as 16-bit ones often are) is taken apart by the bits of the logits.  A last walk adds up the masses that stay by
-// segments of the row, and the segment in which the target falls is gone through once more.
+// takes (equal logits, as 16-bit ones often are) is taken apart by the bits of the logits.  The masses that stay are added up by
+// segments of the row, in the walk of the cut or one of their own, and the segment in which the target falls is gone through once more.
+//
+// Bound by the walks' integer work and, for one row, by the chain of barriers and trips between blocks.  64 rows of 152,064 (39 MB, read once 5.9 us), by what
+// the rows ask for: the maximum alone 8 us, no limits 32, k = 50 46, top-p 0.9 75 to 88, k = 20,000 and top-p 119, a mixture 86; one row of the mixture
+// 37 to 39 in a cluster of 8 blocks.
 #include <math_constants.h>
 
 #define FE_PDL_CLASS 8      // FE_PDL_SAMPLING
@@ -32,7 +35,7 @@ constexpr int SEGMENTS = 256;
 constexpr int MAX_CLUSTER = 8;
 constexpr int STEPS = 4096;
 constexpr float STEPS_A_UNIT = 128.f;
-constexpr float FARTHEST = 32.f;              // STEPS / STEPS_A_UNIT: a mass beyond is below 2^-46 of the largest
+constexpr float FARTHEST = 32.f;              // STEPS / STEPS_A_UNIT: a mass beyond is below 2^-46 of the largest, and counts as nothing
 constexpr int COARSE_BITS = 13;               // of a token's mass in the second walk, against that of its step
 constexpr int LIST = 2048;
 constexpr int BATCH = 5;                      // 16-byte loads of a lane on their way at once
@@ -89,7 +92,7 @@ struct Rows {
     int mass_bits;              // masses are whole numbers of 2^-mass_bits of the largest
 };
 
-constexpr int ROOTS = 16;                     // 2^(-i / 16) in a table
+constexpr int ROOTS = 256;                    // 2^(-i / 256) in a table
 
 struct Shared {
     unsigned counts[STEPS], coarse[STEPS];             // tokens of a step, and their masses
@@ -104,50 +107,76 @@ struct Shared {
     int row_ties[SEGMENTS];
     u64 warp_mass[WARPS];
     unsigned warp_count[WARPS];
-    u64 own_mass;
+    u64 own_mass, own_mass2;
     unsigned own_count, own_low, own_high;
     float own_max;
     int own_index, listed;
     u64 found_mass;
     unsigned found_count;
     int found_at;
-    double roots[ROOTS];
+    long long roots[ROOTS];
 };
 
-// What a row's masses are made of.  A mass is a whole number that is right to 2^-42 of itself: where logits are equal, as 16-bit ones often are,
-// thousands of tokens have the same one, and an error of a 32-bit exponential would come thousands of times.  e^-x = 2^-y is
-// taken with a table of the 16th roots and a polynomial between them (Tang's table-driven exponential): y 16 = n + r, |r| <= 1/2, and with
-// h = r ln 2 / 16 <= 0.022 the Taylor polynomial of e^-h to the fifth power leaves out less than h^6 / 720 = 2^-42.  Fourteen operations in 64
-// bits, of which an SM does 64 a clock.
+// What a row's masses are made of.  A mass is a whole number, rounded down, right to 2^-32 of itself: where logits are equal, as 16-bit ones
+// often are, thousands of tokens have the same one, and an error of a 32-bit exponential would come thousands of times.  It is 2^(z - z_max),
+// z = log2(e) logit / T, from a table of the 256th roots of 2 and a polynomial between them (Tang's table-driven exponential): z 256 = n + r, and only the
+// differences of n and of r to the maximum's count.  |r| <= 1/2 is what one rounding of a multiply-add leaves of an exact product, so it is right to 2^-25
+// of itself, 2^-33 of z; the polynomial gives 2^-(difference of r) - 1, below 2^-8, as a whole number of 2^-32; the table has 62 bits.
+// Logits themselves are multiplied while z_max is below 2^13; beyond, all that has a mass lies within a factor of two of the maximum, and what is
+// multiplied is the difference to it, which then is exact.  (In 64-bit floating point, or with rounded differences and products kept in two parts,
+// a walk over 64 rows of 152,064 took 40 us; this 20, bound by the integer pipe: two or three dozen instructions a token.)
 struct Mass {
     float top, over;                         // the maximum, 1 / T
-    double steps;                            // 16 log2(e) / T
-    int bits;
-    const double* roots;                     // shared memory
+    float base;                              // 0 or the maximum
+    float steps, steps_rest;                 // log2(e) / T and what it lacks
+    float rest;                              // the maximum's r / 256
+    float least;                             // logits below have less than one unit of mass
+    float counted;                           // logits from here on count as kept: as many as have a probability at all, however small (e^-x in 64 bits is above zero up to 745)
+    int whole;                               // the maximum's n + 256 (62 - bits)
+    const long long* roots;                  // shared memory: 2^62 2^(-i / ROOTS)
+    static constexpr float MAGIC = 49152.f;  // 1.5 2^15: adding it rounds to whole 256ths
+    __device__ __forceinline__ void set(float most, float heat, int bits, const long long* table) {
+        top = most;
+        roots = table;
+        heat = fmaxf(heat, 1e-36f);                              // so that log2(e) / T is finite
+        over = 1.f / heat;
+        const double exact = isinf(most) ? 0. : 1.44269504088896340736 / (double)heat;        // an infinite maximum: all of them weigh 1, the rest nothing
+        steps = (float)exact;
+        steps_rest = (float)(exact - (double)steps);
+        base = fabsf(most) * steps < 8192.f ? 0.f : fminf(most, CUDART_MAX_NORMAL_F);
+        least = isinf(most) ? most : __double2float_ru((double)most - bits * 0.69314718055994530942 * (double)heat);
+        counted = isinf(most) ? most : (float)((double)most - 745. * (double)heat);
+        whole = 0;
+        rest = 0.f;
+        int n;
+        float r;
+        split(most, n, r);
+        whole = ROOTS * (62 - bits) - n;
+        rest = -r;
+    }
+    __device__ __forceinline__ void split(float v, int& less, float& r) const {
+        const float w = fminf(v, CUDART_MAX_NORMAL_F) - base, t = fmaf(w, steps, MAGIC);
+        less = whole - __float_as_int(t);
+        r = rest - fmaf(w, steps_rest, fmaf(w, steps, MAGIC - t));
+    }
     __device__ __forceinline__ float distance(float v) const { return v == top ? 0.f : (top - v) * over; }      // infinite maxima too
     __device__ __forceinline__ u64 of(float v) const {
-        if (v == top) return 1ull << bits;
-        const double y = ((double)top - (double)v) * steps;
-        if (!(y < 16.0 * 62.0)) return 0;
-        const double magic = 6755399441055744.0;             // 1.5 2^52: adding it rounds to a whole number
-        const double t = y + magic;
-        const int n = __double2loint(t);
-        const double r = y - (t - magic);
-        constexpr double L = 0.69314718055994530942 / ROOTS;
-        double p = -L * L * L * L * L / 120.0;
-        p = fma(p, r, L * L * L * L / 24.0);
-        p = fma(p, r, -L * L * L / 6.0);
-        p = fma(p, r, L * L / 2.0);
-        p = fma(p, r, -L);
-        p = fma(p, r, 1.0);
-        const double unit = __hiloint2double((1023 + bits - n / ROOTS) << 20, 0);
-        return __double2ull_rn(p * roots[n % ROOTS] * unit);
+        int n;
+        float r;                                                 // 256 y = n + 256 r, the mass 2^-y; |r| <= 2^-8
+        split(v, n, r);
+        constexpr float L = 0.69314718f, SCALE = 4294967296.f;                 // 2^32
+        const float z = r * fmaf(r, fmaf(r, -SCALE * L * L * L / 6.f, SCALE * L * L / 2.f), -SCALE * L);       // 2^32 (2^-r - 1)
+        const long long root = roots[n & (ROOTS - 1)];
+        const u64 m = (u64)(root + (long long)__float2int_rn(z) * (long long)(int)(root >> 32));
+        return !(v >= least) ? 0 : m >> (n / ROOTS & 63);
     }
 };
 __device__ __forceinline__ int step_of(float far) { return far < FARTHEST ? (int)(far * STEPS_A_UNIT) : STEPS; }
 
-template <typename F> __device__ __forceinline__ void over_segment(const float* x, int from, int to, bool vector, F f) {
+// f(logit, index) for the tokens [from, to); RAW: as they stand, for what takes NaN and -0 as it should of itself
+template <bool RAW = false, typename F> __device__ __forceinline__ void over_segment(const float* x, int from, int to, bool vector, F f) {
     const int lane = threadIdx.x & 31;
+    auto clean = [](float v) { return RAW ? v : sanitize(v); };
     if (vector) {
         for (int base = from; base < to; base += 128 * BATCH) {
             float4 v[BATCH];
@@ -159,7 +188,7 @@ template <typename F> __device__ __forceinline__ void over_segment(const float* 
 #pragma unroll
             for (int u = 0; u < BATCH; ++u) {
                 const int i = base + 128 * u + 4 * lane;
-                if (i < to) { f(sanitize(v[u].x), i); f(sanitize(v[u].y), i + 1); f(sanitize(v[u].z), i + 2); f(sanitize(v[u].w), i + 3); }
+                if (i < to) { f(clean(v[u].x), i); f(clean(v[u].y), i + 1); f(clean(v[u].z), i + 2); f(clean(v[u].w), i + 3); }
             }
         }
     } else {
@@ -173,7 +202,7 @@ template <typename F> __device__ __forceinline__ void over_segment(const float* 
 #pragma unroll
             for (int u = 0; u < BATCH; ++u) {
                 const int i = base + 32 * u + lane;
-                if (i < to) f(sanitize(v[u]), i);
+                if (i < to) f(clean(v[u]), i);
             }
         }
     }
@@ -230,8 +259,11 @@ __device__ __forceinline__ void sort_list(u64* a, int n) {
                 const u64 x = a[i], y = a[i + j];
                 if ((x > y) == ((i & k) == 0)) { a[i] = y; a[i + j] = x; }
             }
-            __syncthreads();
+            // a warp's pairs are of its own 64 entries as long as they lie 32 apart at most
+            if (j > 32 || (j == 1 && k > 32)) __syncthreads();
+            else __syncwarp();
         }
+    __syncthreads();
 }
 static_assert(LIST == 2 * THREADS, "a pair a thread");
 
@@ -249,26 +281,30 @@ sample_filtered_kernel(const Rows of, const int C) {
     const bool vector = (V & 3) == 0 && ((size_t)x & 15) == 0;
     bool by_segments = false;                              // the segments' sums are there already
     unsigned number_all = 0;                               // this thread's tokens that stay
+    u64 mass_all = 0;                                      // and their mass
     // f(logit, index) over this block's part; a warp takes its segments one after the other
     auto walk = [&](auto f) {
         for (int j = 0; j < per_warp; ++j)
-            over_segment(x, min((long long)V, (long long)(first_segment + j) * S), min((long long)V, (long long)(first_segment + j + 1) * S), vector, f);
+            over_segment<true>(x, min((long long)V, (long long)(first_segment + j) * S), min((long long)V, (long long)(first_segment + j + 1) * S), vector, f);
     };
 
     struct Sums { u64 mass; unsigned number; };
     // the same; f(logit, index, sums) adds up what stays, a segment at a time
     auto walk_segments = [&](auto f) {
         number_all = 0;
+        mass_all = 0;
         for (int j = 0; j < per_warp; ++j) {
             Sums here{0, 0};
-            over_segment(x, min((long long)V, (long long)(first_segment + j) * S), min((long long)V, (long long)(first_segment + j + 1) * S), vector,
+            over_segment<true>(x, min((long long)V, (long long)(first_segment + j) * S), min((long long)V, (long long)(first_segment + j + 1) * S), vector,
                          [&](float v, int i) { f(v, i, here); });
+            mass_all += here.mass;
             here.mass = warp_sum64(here.mass);
             if (lane == 0) s.segment_mass[warp * per_warp + j] = here.mass;
             number_all += here.number;
         }
     };
 
+    if (tid < ROOTS) s.roots[tid] = __double2ll_rn(exp2(62.0 - (double)tid / ROOTS));
     // ---- the maximum and its lowest index
     float best = -CUDART_INF_F;
     int best_at = 0x7fffffff;
@@ -276,7 +312,6 @@ sample_filtered_kernel(const Rows of, const int C) {
     auto take = [&](float v, int i) { if (v > best || (v == best && i < best_at)) { best = v; best_at = i; } };
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) take(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_at, o));
-    if (tid < ROOTS) s.roots[tid] = exp2(-(double)tid / ROOTS);
     if (lane == 0) { s.warp_mass[warp] = (u64)__float_as_uint(best) << 32 | (unsigned)best_at; }
     __syncthreads();
     if (warp == 0) {
@@ -307,11 +342,7 @@ sample_filtered_kernel(const Rows of, const int C) {
         return;
     }
     Mass mass;
-    mass.top = top;
-    mass.over = 1.f / heat;
-    mass.steps = ROOTS * 1.44269504088896340736 / (double)heat;
-    mass.bits = of.mass_bits;
-    mass.roots = s.roots;
+    mass.set(top, heat, of.mass_bits, s.roots);
     const int k = of.top_k[row];
     const bool use_k = k > 0 && k < V;
     const float p = fmaxf(of.top_p[row], 1e-30f), least = of.min_p[row];      // the first token always stays
@@ -322,14 +353,16 @@ sample_filtered_kernel(const Rows of, const int C) {
 
     unsigned thr = 0, need = 0;                            // what stays: keys above thr, and the first ``need`` of those equal to it
     bool all_ties = true;                                  // all that are equal to it
-    // adds up a 64-bit and a 32-bit number over the cluster (s.own_mass and s.own_count are free)
-    auto cluster_sum = [&](u64 m, unsigned n, u64& all_m, unsigned& all_n) {
+    // adds up two 64-bit numbers and a 32-bit one over the cluster (s.own_mass, s.own_mass2 and s.own_count are free)
+    auto cluster_sum = [&](u64& m, u64& m2, unsigned& n) {
         m = block_sum64(m, s);
+        m2 = block_sum64(m2, s);
         n = block_sum32(n, s);
-        if (tid == 0) { s.own_mass = m; s.own_count = n; }
+        if (tid == 0) { s.own_mass = m; s.own_mass2 = m2; s.own_count = n; }
         cluster_sync();
-        all_m = warp_sum64(lane < C ? ld_peer64(&s.own_mass, lane) : 0);
-        all_n = __reduce_add_sync(0xffffffffu, lane < C ? ld_peer(&s.own_count, lane) : 0);
+        m = warp_sum64(lane < C ? ld_peer64(&s.own_mass, lane) : 0);
+        m2 = warp_sum64(lane < C ? ld_peer64(&s.own_mass2, lane) : 0);
+        n = __reduce_add_sync(0xffffffffu, lane < C ? ld_peer(&s.own_count, lane) : 0);
         cluster_sync();
     };
 
@@ -337,7 +370,6 @@ sample_filtered_kernel(const Rows of, const int C) {
         // ---- counts and masses by steps
         for (int i = tid; i < STEPS; i += THREADS) { s.counts[i] = 0; s.coarse[i] = 0; }
         __syncthreads();
-        u64 total = 0;
         walk([&](float v, int) {
             const float far = mass.distance(v);
             const int step = step_of(far);
@@ -347,11 +379,9 @@ sample_filtered_kernel(const Rows of, const int C) {
                 // e^-(distance inside the step), the step 1/128 long: two terms of the series are good to 1e-7
                 const float in = far - (float)step * (1.f / STEPS_A_UNIT);
                 atomicAdd(&s.coarse[step], (unsigned)__float2int_rn((1.f - in * (1.f - 0.5f * in)) * (float)(1 << COARSE_BITS)));
-                total += mass.of(v);
             }
         });
-        unsigned nothing;
-        cluster_sum(total, 0u, total, nothing);            // the barrier inside: every block's steps are there
+        cluster_sync();
         // the row's steps, four a thread; the same in every block
         unsigned count[4];
         u64 coarse[4], flat[4], own_coarse = 0;           // flat: as if every token of a step weighed the same
@@ -364,13 +394,33 @@ sample_filtered_kernel(const Rows of, const int C) {
 #pragma unroll
             for (int c = 0; c < MAX_CLUSTER; ++c) { sum[0] += v[c].x; sum[1] += v[c].y; sum[2] += v[c].z; sum[3] += v[c].w; }
         };
+        // More than two blocks: each adds up its share of the steps (8 blocks: 2 x 16 KB to read instead of 8; one row 9 us less), the sums fit 32 bits
+        const int share = STEPS / C;
+        if (C > 2) {
+            if (4 * tid < share) {
+                u64 sum[4];
+                const int at = (int)rank * share + 4 * tid;
+                auto add_up = [&](unsigned* own) {
+                    all_blocks(own, sum);
+                    *reinterpret_cast<uint4*>(own) = make_uint4((unsigned)sum[0], (unsigned)sum[1], (unsigned)sum[2], (unsigned)sum[3]);
+                };
+                if (use_k) add_up(&s.counts[at]);
+                if (use_p) add_up(&s.coarse[at]);
+            }
+            cluster_sync();
+        }
+        auto of_row = [&](const unsigned* own, u64* sum) {
+            if (C <= 2) return all_blocks(own, sum);
+            const uint4 v = ld_peer4(own, (unsigned)(4 * tid / share));
+            sum[0] = v.x, sum[1] = v.y, sum[2] = v.z, sum[3] = v.w;
+        };
         {
             u64 sum[4] = {0, 0, 0, 0};
-            if (use_k) all_blocks(&s.counts[4 * tid], sum);
+            if (use_k) of_row(&s.counts[4 * tid], sum);
 #pragma unroll
             for (int e = 0; e < 4; ++e) { count[e] = (unsigned)sum[e]; own_count += sum[e]; flat[e] = 0; }
         }
-        if (use_p) all_blocks(&s.coarse[4 * tid], flat);
+        if (use_p) of_row(&s.coarse[4 * tid], flat);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             coarse[e] = use_p ? __float2ull_rn((float)flat[e] * expf(-(float)(4 * tid + e) * (1.f / STEPS_A_UNIT)) * 65536.f) : 0;
@@ -406,27 +456,50 @@ sample_filtered_kernel(const Rows of, const int C) {
             __syncthreads();
             return n;
         };
+        auto key_of = [](u64 entry) { return ~(unsigned)(entry >> 32); };
+        auto logit_of = [](unsigned key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key); };
+        // the lowest logit of a step up to ``step``: what the steps' own arithmetic says, found among all floats, 32 at a time
+        auto floor_of = [&](int step) {
+            if (step >= STEPS) return -CUDART_INF_F;
+            if (step < 0) return CUDART_INF_F;
+            unsigned above = ordered_key(top), below = 0;              // step_of <= step at ``above``, not at ``below``
+            while (above - below > 1) {
+                const unsigned part = (above - below - 1) / 32 + 1, key = above - below > part * lane ? above - part * lane : below;
+                const float v = logit_of(key);
+                const int good = __popc(__ballot_sync(0xffffffffu, key > below && step_of(mass.distance(v)) <= step));
+                above -= part * (good - 1);
+                if (good < 32 && above - below > part) below = above - part;
+            }
+            return logit_of(above);
+        };
         // Puts the tokens of steps [from, to] into the row's list, in every block; false when they do not fit.  ``above`` and ``above_count``:
-        // exact sums of the steps before, ``low`` and ``high`` the least and the greatest key in them.
-        u64 above = 0;
+        // exact sums of the steps before, ``everything`` of all steps (only where top-p is of the whole row), ``low`` and ``high`` the least and the
+        // greatest key in them.
+        const bool of_whole = use_p && !use_k;
+        u64 above = 0, everything = 0;
         unsigned above_count = 0, low = 0, high = 0;
         int n = 0;
         auto list = [&](int from, int to) {
             if (tid == 0) s.listed = 0;
             __syncthreads();
-            u64 m = 0;
-            unsigned cnt = 0, least_key = 0xffffffffu, most_key = 0;
+            above = everything = 0;
+            above_count = 0;
+            unsigned least_key = 0xffffffffu, most_key = 0;
+            const float floor_to = floor_of(to), floor_above = from > 0 ? floor_of(from - 1) : CUDART_INF_F, floor_kept = fmaxf(floor_above, low_logit);
+            const bool none_above = from == 0, all_listed = to >= STEPS, min_p_bites = floor_kept > floor_above;      // min-p takes some of them away
+            const bool masses = of_whole || !none_above;
             walk_segments([&](float v, int i, Sums& here) {
-                const int step = step_of(mass.distance(v));
-                if (step > to) return;
-                if (step < from) {
+                const bool over = v >= floor_above && !none_above, stays = v >= floor_kept && !none_above;
+                if (masses) {                              // whichever it is: one way for all lanes
                     const u64 own = mass.of(v);
-                    m += own;
-                    ++cnt;
-                    if (v >= low_logit) { here.mass += own; ++here.number; }
-                    return;
+                    here.mass += stays ? own : 0;
+                    everything += own;
+                    if (min_p_bites) above += over && !stays ? own : 0;
                 }
-                const unsigned key = ordered_key(v);
+                here.number += stays;
+                if (min_p_bites) above_count += over && !stays;
+                if (over || !(v >= floor_to || all_listed)) return;
+                const unsigned key = ordered_key(sanitize(v));
                 least_key = min(least_key, key);
                 most_key = max(most_key, key);
                 const int at = atomicAdd(&s.listed, 1);
@@ -437,7 +510,9 @@ sample_filtered_kernel(const Rows of, const int C) {
             if (tid == 0) { s.own_low = 0xffffffffu; s.own_high = 0; }
             __syncthreads();
             if (lane == 0) { atomicMin(&s.own_low, least_key); atomicMax(&s.own_high, most_key); }
-            cluster_sum(m, cnt, above, above_count);       // barriers inside: lists and keys are there
+            above += mass_all;
+            above_count += number_all;
+            cluster_sum(above, everything, above_count);         // barriers inside: lists and keys are there
             int here = lane < C ? (int)ld_peer(&s.listed, lane) : 0, upto = here;
             low = __reduce_min_sync(0xffffffffu, lane < C ? ld_peer(&s.own_low, lane) : 0xffffffffu);
             high = __reduce_max_sync(0xffffffffu, lane < C ? ld_peer(&s.own_high, lane) : 0u);
@@ -464,8 +539,6 @@ sample_filtered_kernel(const Rows of, const int C) {
             cluster_sync();                                // the peers' lists are read
             return n <= LIST;
         };
-        auto key_of = [](u64 entry) { return ~(unsigned)(entry >> 32); };
-        auto logit_of = [](unsigned key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key); };
         // The list in order, every token's mass and the mass before it.
         auto rank_list = [&]() {
             sort_list(s.all, n);
@@ -500,7 +573,7 @@ sample_filtered_kernel(const Rows of, const int C) {
             rank_list();
             // what stays of the list: a place below k, less than p of the sum before it
             const int reach = k_bites ? k : n;             // the list holds k tokens at least
-            const u64 in_list = s.all_before[reach - 1] + s.all_mass[reach - 1], sum = k_bites ? in_list : total;
+            const u64 in_list = s.all_before[reach - 1] + s.all_mass[reach - 1], sum = k_bites ? in_list : everything;
             const double limit = (double)p * (double)sum;
             // the coarse sums may have chosen a step too early: the list then does not reach the limit, and the long way is taken
             if (k_bites || (double)in_list >= limit) {
@@ -538,9 +611,10 @@ sample_filtered_kernel(const Rows of, const int C) {
             }
         }
         // ---- the long way: one limit after the other, each an exact cut (thr, need)
-        // ``limit`` in tokens or in mass; ``at``: the step that is likely to hold it
+        // ``limit`` in tokens or in mass, or (of_whole) the mass's share of the row's; ``at``: the step that is likely to hold it
         u64 last_entry = 0;                                // of the last cut: the last listed token that stays
         auto cut = [&](bool by_mass, double limit, int at) {
+            const double share = limit;
             while (true) {
                 const bool whole = by_segments = list(at, at);
                 // what the step holds in all
@@ -549,13 +623,16 @@ sample_filtered_kernel(const Rows of, const int C) {
                     rank_list();
                     here_mass = n > 0 ? s.all_before[n - 1] + s.all_mass[n - 1] : 0;
                 } else {
-                    u64 mine = 0;
-                    unsigned nothing_more;
+                    u64 nothing = 0;
+                    unsigned none = 0;
+                    const float floor_at = floor_of(at), floor_before = floor_of(at - 1);
                     walk([&](float v, int) {
-                        if (step_of(mass.distance(v)) == at) mine += mass.of(v);
+                        const u64 own = mass.of(v);
+                        here_mass += v >= floor_at && !(at > 0 && v >= floor_before) ? own : 0;
                     });
-                    cluster_sum(mine, 0u, here_mass, nothing_more);
+                    cluster_sum(here_mass, nothing, none);
                 }
+                if (by_mass && of_whole) limit = share * (double)everything;
                 const double before = by_mass ? (double)above : (double)above_count, here = by_mass ? (double)here_mass : (double)n;
                 // the coarse sums may be a step off
                 if (before >= limit && at > 0 && above_count > 0) { --at; continue; }
@@ -589,8 +666,7 @@ sample_filtered_kernel(const Rows of, const int C) {
                     for (int i = tid; i < STEPS; i += THREADS) { s.counts[i] = 0; s.fine[i] = 0; }
                     __syncthreads();
                     walk([&](float v, int) {
-                        if (step_of(mass.distance(v)) != at) return;
-                        const unsigned key = ordered_key(v);
+                        const unsigned key = ordered_key(sanitize(v));
                         if (key < from || key > upto) return;
                         const int bin = (int)((upto - key) >> shift);          // largest first
                         atomicAdd(&s.counts[bin], 1u);
@@ -634,9 +710,9 @@ sample_filtered_kernel(const Rows of, const int C) {
                 thr = from;
                 by_segments = false;
                 unsigned ties = 0;
-                walk([&](float v, int) { ties += ordered_key(v) == thr; });
-                u64 nothing64;
-                cluster_sum(0, ties, nothing64, ties);
+                walk([&](float v, int) { ties += ordered_key(sanitize(v)) == thr; });
+                u64 nothing64 = 0, nothing65 = 0;
+                cluster_sum(nothing64, nothing65, ties);
                 const u64 each = mass.of(logit_of(thr));
                 if (by_mass) {
                     // the fewest with which the limit is reached, and one at least where nothing comes before
@@ -651,15 +727,16 @@ sample_filtered_kernel(const Rows of, const int C) {
                 return run + (u64)need * each;
             }
         };
-        u64 within = total;                                // top-p alone: of all
-        if (use_k) within = cut(false, (double)k, k_bites ? step_k : STEPS);
-        if (use_p) {
-            const double limit = (double)p * (double)within;
-            // the step by the coarse sums, against the exact sum where top-k has cut them
-            const double unit = all_coarse > 0 && total > 0 ? (double)all_coarse / (double)total : 0.0;
-            const int at = step_at(coarse, coarse_before, all_coarse, limit * unit);
-            cut(true, limit, at < 0 ? 0 : at);
-        }
+        if (use_k) {
+            const u64 within = cut(false, (double)k, k_bites ? step_k : STEPS);
+            if (use_p) {
+                // coarse sums are whole numbers of 2^-(COARSE_BITS + 16) of the largest mass
+                const double limit = (double)p * (double)within;
+                const int at = step_at(coarse, coarse_before, all_coarse, limit * exp2((double)(COARSE_BITS + 16 - of.mass_bits)));
+                cut(true, limit, at < 0 ? 0 : at);
+            }
+        } else
+            cut(true, (double)p, step_p < 0 ? 0 : step_p);
         if (by_segments) {
             // the segments hold what lies before the last cut's step: the tokens of the step that stay come to it, each block's own
             __syncthreads();
@@ -668,7 +745,7 @@ sample_filtered_kernel(const Rows of, const int C) {
                 const float v = logit_of(key_of(entry));
                 if (entry > last_entry || v < low_logit) continue;
                 atomicAdd(&s.segment_mass[(int)(unsigned)entry / S - (int)rank * per_block], mass.of(v));
-                number_all += mass.distance(v) < 745.f;
+                number_all += v >= mass.counted;
             }
         }
     }
@@ -689,13 +766,15 @@ sample_filtered_kernel(const Rows of, const int C) {
         if (tid < SEGMENTS) s.row_ties[tid] = (int)before;
         cluster_sync();
     }
+    // keys above or equal to thr, and what min-p leaves, as one logit; keys 0 and of -inf: all
+    const float lowest = fmaxf(thr > ordered_key(-CUDART_INF_F) ? __uint_as_float((thr & 0x80000000u) ? (thr & 0x7fffffffu) : ~thr) : -CUDART_INF_F, low_logit);
+    const float lowest_counted = fmaxf(lowest, mass.counted);
     if (!by_segments) {
         if (all_ties)
             walk_segments([&](float v, int, Sums& here) {
-                if (ordered_key(v) < thr || v < low_logit) return;
-                // as many as have a probability at all, however small: e^-x in 64 bits is above zero up to 745
-                here.mass += mass.of(v);
-                here.number += mass.distance(v) < 745.f;
+                const u64 own = mass.of(v);
+                here.mass += v >= lowest ? own : 0;
+                here.number += v >= lowest_counted;
             });
         else {
             number_all = 0;
@@ -712,7 +791,7 @@ sample_filtered_kernel(const Rows of, const int C) {
                     seen += __popc(tied);
                     if (i < to && (key > thr || (key == thr && place < need)) && v >= low_logit) {
                         sum += mass.of(v);
-                        number_all += mass.distance(v) < 745.f;
+                        number_all += v >= mass.counted;
                     }
                 }
                 sum = warp_sum64(sum);
@@ -734,36 +813,48 @@ sample_filtered_kernel(const Rows of, const int C) {
     const float u = of.uniform[row];
     double target = (u > 0.f ? (double)fminf(u, 1.f) : 0.0) * (double)total;
     if (target >= (double)total) target = nextafter((double)total, 0.0);
-    for (int j = 0; j < per_warp; ++j) {
-        const int segment = first_segment + j;
-        if (!((double)s.row_mass[segment] <= target && target < (double)s.row_mass[segment + 1])) continue;
-        // one warp of the row: its segment in index order, 32 tokens at a time
-        const int from = (int)min((long long)V, (long long)segment * S), to = (int)min((long long)V, (long long)(segment + 1) * S);
-        u64 run = s.row_mass[segment];
-        unsigned seen = all_ties ? 0u : (unsigned)s.row_ties[segment];
-        for (int base = from; base < to; base += 32) {
-            const int i = base + lane;
-            const float v = i < to ? sanitize(x[i]) : -CUDART_INF_F;
-            const unsigned key = ordered_key(v), tied = __ballot_sync(0xffffffffu, i < to && key == thr);
-            const unsigned place = seen + __popc(tied & ((1u << lane) - 1u));
-            seen += __popc(tied);
-            const bool stays = i < to && (key > thr || (key == thr && (all_ties || place < need))) && v >= low_logit;
-            const u64 m = stays ? mass.of(v) : 0;
-            u64 upto = m;
+    // the segment it falls in, and the block that has it: two tokens a thread
+    if (tid == 0) s.found_at = -1;
+    __syncthreads();
+    if (tid < per_block) {
+        const int segment = (int)rank * per_block + tid;
+        if ((double)s.row_mass[segment] <= target && target < (double)s.row_mass[segment + 1]) s.found_at = segment;
+    }
+    __syncthreads();
+    const int segment = s.found_at;
+    if (segment < 0) return;
+    const int from = (int)min((long long)V, (long long)segment * S) + 2 * tid, to = (int)min((long long)V, (long long)(segment + 1) * S);
+    float v[2];
+    bool tied[2], stays[2];
+    u64 m[2], nothing;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 up = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += up;
-            }
-            if (m > 0 && (double)(run + upto - m) <= target && target < (double)(run + upto)) {
-                of.tokens[row] = i;
-                of.probability[row] = (float)((double)m / (double)total);
-                of.kept[row] = (int)number_all;
-            }
-            run += __shfl_sync(0xffffffffu, upto, 31);
+    for (int e = 0; e < 2; ++e) {
+        v[e] = from + e < to ? sanitize(x[from + e]) : -CUDART_INF_F;
+        tied[e] = from + e < to && ordered_key(v[e]) == thr;
+        stays[e] = from + e < to && ordered_key(v[e]) >= thr && v[e] >= low_logit;
+    }
+    if (!all_ties) {
+        unsigned place = (unsigned)s.row_ties[segment] + (unsigned)block_before64((u64)tied[0] + (u64)tied[1], nothing, s);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            stays[e] = stays[e] && (!tied[e] || place < need);
+            place += tied[e];
         }
     }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m[e] = stays[e] ? mass.of(v[e]) : 0;
+    u64 run = s.row_mass[segment] + block_before64(m[0] + m[1], nothing, s);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        if (m[e] > 0 && (double)run <= target && target < (double)(run + m[e])) {
+            of.tokens[row] = from + e;
+            of.probability[row] = (float)((double)m[e] / (double)total);
+            of.kept[row] = (int)number_all;
+        }
+        run += m[e];
+    }
 }
+static_assert(((1 << 19) / SEGMENTS) <= 2 * THREADS, "a segment's tokens, two a thread");
 
 // How many clusters of ``blocks`` blocks of the kernel the device holds at once; asked of the driver once per size and device.
 int clusters_resident(int blocks) {
@@ -801,8 +892,7 @@ extern "C" int fe_sample_filtered(const float* logits, long long ld, int R, int 
     FE_REQUIRE(V < (1 << 19) && (long long)R * MAX_CLUSTER < (1LL << 31), "sample_filtered: %d rows of %d logits; fewer than 2^19 logits and 2^28 rows", R, V);      // a step's coarse mass is 32 bits
     FE_REQUIRE(blocks == 0 || blocks == 1 || blocks == 2 || blocks == 4 || blocks == 8, "sample_filtered: %d blocks a row; 1, 2, 4 or 8", blocks);
     if (R == 0) return 0;
-    const cudaError_t set = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
-    FE_REQUIRE(set == cudaSuccess, "sample_filtered: %s", cudaGetErrorString(set));
+    FE_REQUIRE(fe_allow_smem((const void*)sample_filtered_kernel, (int)sizeof(Shared)), "sample_filtered: no kernel with %d bytes of shared memory", (int)sizeof(Shared));
     if (blocks == 0)
         for (blocks = MAX_CLUSTER; blocks > 1 && R > clusters_resident(blocks);) blocks >>= 1;
     int bits = 0;

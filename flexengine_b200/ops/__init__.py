@@ -1769,8 +1769,7 @@ def sample_filtered(logits, temperature, top_k, top_p, min_p, uniform, blocks: i
                                ("min_p", min_p, torch.float32), ("uniform", uniform, torch.float32)):
             if t.dtype != dtype or t.numel() != R or not t.is_contiguous():
                 raise TypeError(f"{what}: {name} is contiguous {dtype} [{R}]")
-        tokens, kept = (torch.empty(R, dtype=torch.int32, device=logits.device) for _ in range(2))
-        probability = torch.empty(R, dtype=torch.float32, device=logits.device)
+        tokens, kept, probability = top_k.new_empty(R), top_k.new_empty(R), logits.new_empty(R)
         _run(_core(), "fe_sample_filtered", _ptr(logits), logits.stride(0) if R > 1 else V, R, V, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
              _ptr(uniform), _ptr(tokens), _ptr(probability), _ptr(kept), blocks, _stream())
     return tokens, probability, kept
@@ -1851,7 +1850,7 @@ def qkv_rope_kv4(projected, bias, positions, inv_freq, rot, slot_mapping, cache,
             raise ValueError(f"{what}: the bias is contiguous float32 [(nq + 2 nkv) d]")
         if rot and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2 or not inv_freq.is_contiguous()):
             raise ValueError(f"{what}: inv_freq is contiguous float32 [rot / 2]")
-        queries = torch.empty((T, nq * d), dtype=out_dtype, device=projected.device)
+        queries = projected.new_empty((T, nq * d), dtype=out_dtype)
         _run(_kv4(), "fe_qkv_rope_kv4", _ptr(projected), _code(projected.dtype), projected.stride(0) if T > 1 else projected.shape[1], _ptr(bias),
              _ptr(positions), _ptr(inv_freq) if rot else None, rot, 1 if pairs == "interleaved" else 0, float(rot_gain), _ptr(slot_mapping), _ptr(cache),
              _ptr(queries), _code(out_dtype), T, nq, nkv, d, page_size, cache.shape[0] * page_size, _ptr(status_word(projected.device)), _stream())
@@ -1865,7 +1864,7 @@ def kv4_rows(cache, slots, nkv, d, page_size, dtype=torch.bfloat16):
         _kv4_cache_ok(what, cache, nkv, d, page_size)
         n = slots.numel()
         _index_ok(what, "slots", slots, n)
-        keys, values = (torch.empty((n, nkv, d), dtype=dtype, device=cache.device) for _ in range(2))
+        keys, values = cache.new_empty((n, nkv, d), dtype=dtype), cache.new_empty((n, nkv, d), dtype=dtype)
         _run(_kv4(), "fe_kv4_rows", _ptr(cache), _ptr(slots), _ptr(keys), _ptr(values), _code(dtype), n, nkv, d, page_size, cache.shape[0] * page_size,
              _ptr(status_word(cache.device)), _stream())
     return keys, values
@@ -1930,10 +1929,10 @@ def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale
             raise ValueError(f"{what}: a window is not negative, and kept first keys go with one")
         if ctx.max_ctx_len > pages * page_size:
             raise ValueError(f"{what}: {ctx.max_ctx_len} tokens in {pages} pages of {page_size}")
-        out = torch.empty((T, nq * d), dtype=q.dtype, device=q.device)
-        lengths, starts = getattr(ctx, "host_lengths", None), getattr(ctx, "host_starts", None)
+        out = q.new_empty((T, nq * d))
         clusters = 1
         if ctx.max_q_len > 1 and T:
+            lengths, starts = getattr(ctx, "host_lengths", None), getattr(ctx, "host_starts", None)
             tensor = code == 1 and d in (64, 128)
             clusters = kv4_portions(lengths, starts, nq, nkv, d, window, tensor) if lengths else 0 if tensor else 1
         if clusters == 0:
