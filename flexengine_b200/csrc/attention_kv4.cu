@@ -5,10 +5,12 @@
 //     q . k = sum_g s_g (q_g . n_g) + sum_g c_g (sum of q_g)
 // and the output, with weights p_t = 2^(score_t - m),
 //     o_g = sum_t (p_t s_tg) n_tg + sum_t p_t c_tg ,
-// so the codes themselves go through the tensor cores, as whole numbers that half precision holds exactly, and scales and centres are
-// applied in 32 bits: the scales to the groups' partial scores and to the weights, the centres as one more product of (c_g) with the
-// sums of q_g, and as sums of p_t c_tg.  What is rounded is the query to half precision (exact for bfloat16 but for numbers 2^-24 of the
-// row's largest) and the weights p s; 32-bit queries take both in two parts, high and low, which leaves 22 bits.
+// so the codes themselves go through the tensor cores, as whole numbers that half precision holds exactly.  Of keys, scales are applied to
+// the groups' partial scores in 32 bits, centres as one more product of (c_g) with the sums of q_g.  What is rounded is the query to half precision (exact for
+// bfloat16 but for numbers 2^-24 of the row's largest).  Of values under 16-bit queries, scale and centre go into the decoded
+// numbers (one multiply-add for two, rounded to half precision: 2^-11 of a number, where bfloat16 results have 2^-8) and the weights p into half
+// precision; under 32-bit queries scales go to the weights in 32 bits and centres into sums of p_t c_tg, and query and weights are taken in two
+// parts, high and low, which leaves 22 bits.
 //
 // Which keys a query sees, the online softmax and its sink are those of the attention over 16-bit caches: key t is visible to the query at
 // position p iff t <= p (and t > p - window, or t < keep, when window > 0).
@@ -23,9 +25,13 @@
 // 128): no barrier between warps until the end, several tiles on their way.  The four warps of a block, and the blocks that share
 // a row's keys, are merged at the end by their maxima and sums, in a fixed order.
 //
-// A weight p s has to keep its place in half precision whatever the scale of the values, so the reference point m is a maximum of score +
+// The reference point m is the largest score met, and moves only when it has grown by more than 2^8 (weights stay below that: in half's range).  Under 32-bit
+// queries a weight p s has to keep its place in half precision whatever the scale of the values, so there m is a maximum of score +
 // exponent of the token's largest value scale: 2^(score - m) s is then at most 2, and the sum of 2^(score - m) is kept in 32 bits, where
-// small scales may make it large.  The reference moves only when it has grown by more than 2^8.
+// small scales may make it large.
+//
+// Bound by the instructions that decode and by the loads' latency: 16 requests of 32,768 keys, 28/4 heads of 128, 93 us for 403 MB of cache (4.3 TB/s; the copies alone,
+// nothing computed, 74); 64 of 8,192 in the mean 63; 8 of 2,048 14; a call of a few keys 7.
 #include <type_traits>
 
 #define FE_PDL_CLASS 2      // FE_PDL_DECODE_ATTENTION
@@ -190,10 +196,13 @@ __device__ __forceinline__ int fill(Segment& w, const Problem& a, int cols) {
 __device__ __forceinline__ int tiles_of(const Problem& a, int r) {
     if (r >= a.requests || min((long long)a.cu_q[r + 1], a.tokens) <= a.cu_q[r]) return 0;
     const int pos = a.q_start[r], lo = first_visible(pos, a.window);
-    return min(kept_tiles<KV4_TILE>(lo, a.keep) + pos / KV4_TILE - lo / KV4_TILE + 1, a.bt_stride * (a.ps / KV4_TILE));
+    const int seen = kept_tiles<KV4_TILE>(lo, a.keep) + pos / KV4_TILE - lo / KV4_TILE + 1, held = a.bt_stride * (a.ps / KV4_TILE);
+    if (seen > held && a.status) atomicOr(a.status, FE_STATUS_BAD_PAGE);
+    return max(1, min(seen, held));
 }
 
-// Blocks that are resident on an SM: the registers are cut to that.  16-bit queries at head size 128: three blocks of 168 registers a thread.
+// Blocks that are resident on an SM: the registers are cut to that.  16-bit queries at head size 128: four blocks of 128 registers a thread (three of 168
+// take the same time for long rows and leave fewer blocks to short ones).
 template <typename TQ, int NG, int NT> __host__ __device__ constexpr int blocks_an_sm() { return sizeof(TQ) == 2 && NG * NT <= 4 ? 4 : 2; }
 
 // TQ: queries and output; 32-bit ones in two parts.  NG: groups of a row.  NT: tiles of eight columns that a block takes.
@@ -442,7 +451,7 @@ kv4_attention_kernel(const Problem a) {
         first_most = __reduce_max_sync(FULL, first_most);
         __syncthreads();
 
-        float o[NT][NG][2][4], oc[NT][NG][2];                // sums over codes, 16 numbers a tile, and over centres (this thread's tokens)
+        float o[NT][NG][2][4], oc[NT][NG][2];                // sums over codes (EXACT) or numbers, 16 a tile, and over centres (EXACT, this thread's tokens)
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -697,6 +706,7 @@ kv4_attention_kernel(const Problem a) {
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
                     l[j][h] += __shfl_xor_sync(FULL, l[j][h], off);
+                    if (!EXACT) continue;                                 // no sums over centres: it only brings NaN
 #pragma unroll
                     for (int i = 0; i < NG; ++i) oc[j][i][h] += __shfl_xor_sync(FULL, oc[j][i][h], off);
                 }
@@ -932,20 +942,37 @@ bool head_size_ok(int d) { return d >= 16 && d % 16 == 0 && d <= KV4_MAX_DIM; }
 // How a decode step's tiles are dealt out: a positive number is that of the blocks that share the tiles of all items; a negative one, -S, a cluster of S
 // blocks for each item.  ``tiles``: of the longest request.
 //
-// An item of up to 16 tiles is one block's.  A cluster as large as leaves all of them resident at once is the shortest way while a
-// block walks up to 32 tiles; sharing out costs running sums over the requests and a second kernel, and wins where one item is too much for
-// eight blocks or lengths differ.  28/4 heads of 128, microseconds: 8 requests of 2,049 keys 13.7 in clusters of 4, 20 shared; 16 of 2,048
-// 13.7 and 21; 1 of 8,192 17.8 (8) and 14.4; 64 of 1,024 to 8,191 75 (2) and 67.
+// The least of what each way is expected to take.  A block takes 6.8 us and, at head size 128, 0.115 for each tile that it walks, 0.07 n where n > 1 of them
+// are on its multiprocessor (and 1.7 more); a cluster 1.1 to 2 more; blocks beyond those that fit at once come after them.  Sharing out costs 15 us (running
+// sums over the requests, pieces of two items in a block, a second kernel) and 0.12 for each request, and is no faster where all requests are as long as the longest, but
+// lengths that differ leave no block without work: its tiles are taken as three quarters of that.  28/4 heads of 128, microseconds, one block, clusters of 2, 4
+// and 8, shared: 64 requests of 512 keys 11 15 23 42 21; 64 of 1,101 19 22 32 52 34; 48 of 2,101 29 25 33 46 34; 8 of 2,049 23 17 14 14 19; 1 of
+// 8,301 70 40 25 18 17; 64 of 8,192 92 84 91 106 87; 64 of 1,024 to 8,191 84 74 71 88 64.
 extern "C" int fe_kv4_attention_plan(int requests, int tiles, int nq, int nkv, int d, int dtype) {
     if (!head_size_ok(d) || requests <= 0 || nq <= 0 || nkv <= 0) return -1;
     const long long items = (long long)requests * nkv * ((nq / nkv + 7) / 8), all = items * tiles;
-    if (tiles <= 16) return -1;
+    if (tiles <= 2 * WARPS * PAIR) return -1;
     const long long most = dtype == FE_F32 ? with_groups(d, [](auto n) { return resident<float, n.value, 1>(); }) : with_groups(d, [](auto n) { return resident<bf16, n.value, 1>(); });
-    const long long fit = most / items, splits = fit < 1 ? 1 : fit > MAX_SPLITS ? MAX_SPLITS : fit;
-    const long long useful = (tiles + 7) / 8, each = splits < useful ? splits : useful;
-    if ((tiles + each - 1) / each <= 32 || all >= (1LL << 31)) return -(int)each;
-    const long long want = (all + 15) / 16;
-    return (int)(want < most ? want : most);
+    const int sms = fe_sm_count(), round = WARPS * PAIR;
+    const double tile = kv4_groups(d) / 4.0 * (dtype == FE_F32 ? 1.1 : 1.0);
+    auto walk = [&](long long blocks, long long each) {          // of so many tiles by each of the blocks on the device
+        const long long beside = (blocks + sms - 1) / sms;
+        return 6.8 + (beside > 1 ? 1.7 : 0.0) + (double)((each + round - 1) / round * round) * tile * (beside > 1 ? 0.07 * (double)beside : 0.115);
+    };
+    double least = 1e30;
+    int plan = -1;
+    for (int S = 1; S <= MAX_SPLITS; S *= 2) {
+        if (S > 1 && S * round > tiles + round - 1) break;
+        const long long at_once = most / S * S, waves = at_once > 0 ? (items * S + at_once - 1) / at_once : 1LL << 20;
+        const double t = (double)waves * (walk(items * S < at_once ? items * S : at_once, (tiles + S - 1) / S) + (S == 1 ? 0.0 : S == 2 ? 1.1 : S == 4 ? 1.3 : 2.0));
+        if (t < least) { least = t; plan = -S; }
+    }
+    if (all < (1LL << 31)) {
+        const long long want = (all + 2 * round - 1) / (2 * round), blocks = want < most ? want : most;
+        const double share = (double)all * (requests > 1 ? 0.75 : 1.0) / (double)blocks;
+        if (walk(blocks, (long long)share) + 8.2 + 0.12 * requests < least) plan = (int)blocks;
+    }
+    return plan;
 }
 
 // Bytes of ``scratch`` for so many blocks.
@@ -954,7 +981,7 @@ extern "C" long long fe_kv4_attention_scratch_bytes(int blocks, int requests, in
     return (long long)blocks * 2 * 8 * (32 * kv4_groups(d) + 4) * 4 + (long long)requests * nkv * ((nq / nkv + 7) / 8) * (long long)sizeof(Held);
 }
 
-// q [tokens, >= nq d], rows ``q_stride`` elements apart; out likewise; dtype of both.  ``blocks`` > 0 (from fe_kv4_attention_blocks; every request
+// q [tokens, >= nq d], rows ``q_stride`` elements apart; out likewise; dtype of both.  ``blocks`` > 0 (from fe_kv4_attention_plan; every request
 // brings one token at most) needs scratch.
 extern "C" int fe_paged_attention_kv4(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, const int* block_table,
                                       int bt_stride, const int* cu_q, const int* q_start, int requests, long long tokens, int max_q_len, int nq,

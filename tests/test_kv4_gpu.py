@@ -461,3 +461,44 @@ def test_engine_with_graphs_top_p_and_min_p(tmp_path_factory):
     assert generate(temperature=0.9, top_p=1e-6, seed=4) == greedy
     with pytest.raises(ValueError, match="4-bit"):
         generate(kv_block_size=8, kv_num_blocks=128)
+
+
+# ---- every way of dealing out a step's tiles ---------------------------------------------------------------------------------------
+def deal_out(monkeypatch, plan, requests, nq, nkv, d):
+    monkeypatch.setattr(ops(), "kv4_plan", lambda *a: (plan, int(ops()._kv4().fe_kv4_attention_scratch_bytes(max(plan, 0), requests, nq, nkv, d))))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("plan", [-1, -2, -3, -4, -8, 1, 2, 7, 40, 296])
+@pytest.mark.parametrize("nq,nkv,d", [(28, 4, 128), (20, 1, 96), (14, 2, 64)])
+def test_every_plan(nq, nkv, d, plan, dtype, monkeypatch, gen):
+    lengths = [(1, 1030), (0, 0), (1, 3), (1, 127), (1, 128), (0, 0), (1, 0), (1, 700), (0, 0)]
+    args = problem(gen, lengths, nq, nkv, d, dtype)
+    deal_out(monkeypatch, plan, len(lengths), nq, nkv, d)
+    out, want = run_attention(*args, nq, nkv, d, 16)
+    check_attention(out, want, args[1], d, f"plan {plan} {nq}/{nkv}/{d} {dtype}")
+    out, want = run_attention(*args, nq, nkv, d, 16, window=100, keep_first=20)
+    check_attention(out, want, args[1], d, f"plan {plan} window {nq}/{nkv}/{d} {dtype}")
+
+
+@pytest.mark.parametrize("plan", [-1, -4, 1, 30])
+def test_a_table_shorter_than_a_request(plan, monkeypatch, gen):
+    """Positions that the table has no pages for: the keys that it has are seen, and the status word says so."""
+    q, cache, table, ctx = problem(gen, [(1, 900), (1, 33)], 8, 2, 64, torch.bfloat16, garbage=False)
+    deal_out(monkeypatch, plan, 2, 8, 2, 64)
+    short = table[:, :20].contiguous()
+    ctx.max_ctx_len = 320
+    out = ops().paged_attention_kv4(q, cache, short, ctx, 8, 2, 64, 16, 0.125)
+    with pytest.raises(RuntimeError, match="page id out of range"):
+        ops().check_status(DEV)
+    ctx.q_start[0] = 319
+    want = kv4_refs.attention64(q, cache, short, ctx.cu_q, ctx.q_start, 8, 2, 64, 16, 0.125)
+    check_attention(out, want, cache, 64, "a short table bfloat16")
+
+
+@pytest.mark.parametrize("requests,tokens,nq,nkv", [(1, 500, 28, 4), (1, 4000, 28, 4), (1, 20000, 28, 4), (128, 700, 28, 4), (64, 1100, 28, 4), (64, 8192, 28, 4), (300, 40, 8, 8)])
+@pytest.mark.parametrize("code", [0, 1])
+def test_plans_are_ways_that_there_are(requests, tokens, nq, nkv, code):
+    plan, scratch = ops().kv4_plan(requests, -(-tokens // 16), nq, nkv, 128, code)
+    assert plan in (-1, -2, -4, -8) or plan > 0
+    assert (scratch > 0) == (plan > 0)
