@@ -144,8 +144,9 @@ struct Mass {
         steps = (float)exact;
         steps_rest = (float)(exact - (double)steps);
         base = fabsf(most) * steps < 8192.f ? 0.f : fminf(most, CUDART_MAX_NORMAL_F);
-        least = isinf(most) ? most : __double2float_ru((double)most - bits * 0.69314718055994530942 * (double)heat);
-        counted = isinf(most) ? most : (float)((double)most - 745. * (double)heat);
+        // (an infinite temperature: all but -inf weigh the same)
+        least = isinf(most) ? most : fmaxf(__double2float_ru((double)most - bits * 0.69314718055994530942 * (double)heat), -CUDART_MAX_NORMAL_F);
+        counted = isinf(most) ? most : fmaxf((float)((double)most - 745. * (double)heat), -CUDART_MAX_NORMAL_F);
         whole = 0;
         rest = 0.f;
         int n;

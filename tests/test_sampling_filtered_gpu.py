@@ -159,3 +159,19 @@ def test_sampler_on_the_device_is_the_plain_one():
     top_ps, min_ps = [0.5, 1.0, 0.8, 1.0, 0.9, 1.0, 1.0, 0.3, 0.95], [0.0, 0.0, 0.0, 0.1, 0.01, 0.2, 0.5, 0.0, 0.0]
     got = Sampler().sample(logits, heats, ks, seeds, draws, top_ps, min_ps)
     assert got == Sampler(kv4_refs).sample(logits, heats, ks, seeds, draws, top_ps, min_ps)
+
+
+@pytest.mark.parametrize("top_p,top_k", [(1.0, 0), (0.5, 0), (1.0, 100), (0.5, 100)])
+def test_an_infinite_temperature_leaves_the_finite_logits_alike(top_p, top_k):
+    R, V = 6, 1000
+    given = rows(3, R, V)
+    given["logits"][:, ::2] = -math.inf
+    given["logits"][:, 5] = math.nan
+    given.update(temperature=full(math.inf, given["temperature"]), top_p=full(top_p, given["top_p"]), top_k=full(top_k, given["top_k"]), min_p=full(0.0, given["min_p"]))
+    n = 100 if top_k else V // 2 - 1
+    n = math.ceil(n * top_p)
+    for blocks in (1, 2, 8):
+        tokens, probability, kept = ops().sample_filtered(**given, blocks=blocks)
+        assert given["logits"].gather(1, tokens.long()[:, None]).isfinite().all()
+        assert kept.tolist() == [n] * R
+        torch.testing.assert_close(probability, torch.full_like(probability, 1 / n), rtol=1e-6, atol=0.0)
