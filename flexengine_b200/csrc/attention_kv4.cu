@@ -30,8 +30,8 @@
 // exponent of the token's largest value scale: 2^(score - m) s is then at most 2, and the sum of 2^(score - m) is kept in 32 bits, where
 // small scales may make it large.
 //
-// Bound by the instructions that decode and by the loads' latency: 16 requests of 32,768 keys, 28/4 heads of 128, 93 us for 403 MB of cache (4.3 TB/s; the copies alone,
-// nothing computed, 74); 64 of 8,192 in the mean 63; 8 of 2,048 14; a call of a few keys 7.
+// Bound by the instructions that decode and by the loads' latency: 16 requests of up to 32,768 keys, 40/8 heads of 128, 93 us for 396 MB of cache (4.3 TB/s; the copies
+// alone, nothing computed, 74); 64 of up to 8,191, 28/4 heads, 63; 8 of 2,049 14; a call of a few keys 7.
 #include <type_traits>
 
 #define FE_PDL_CLASS 2      // FE_PDL_DECODE_ATTENTION
