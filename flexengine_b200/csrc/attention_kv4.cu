@@ -839,7 +839,11 @@ kv4_merge_kernel(const Problem a, int blocks) {
                 }
             }
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) most = fmaxf(most, end[u].x);
+            for (int u = 0; u < AHEAD; ++u) {
+                most = fmaxf(most, end[u].x);
+                // a part without a maximum has seen no key, and its sum is 0, or scores that are all NaN: then it is NaN, and so is the row
+                if (end[u].x == -CUDART_INF_F) sum += end[u].y;
+            }
             if (most == -CUDART_INF_F) continue;
             const float by = ex2(top - most);
             top = most;
@@ -847,7 +851,7 @@ kv4_merge_kernel(const Problem a, int blocks) {
             v.x *= by; v.y *= by; v.z *= by; v.w *= by;
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                if (end[u].x == -CUDART_INF_F) continue;             // saw nothing: what it left is not looked at
+                if (end[u].x == -CUDART_INF_F) continue;             // its numbers are not looked at
                 const float w = ex2(end[u].x - most);
                 sum += w * end[u].y;
                 v.x += w * x[u].x; v.y += w * x[u].y; v.z += w * x[u].z; v.w += w * x[u].w;

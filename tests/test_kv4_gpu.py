@@ -502,3 +502,35 @@ def test_plans_are_ways_that_there_are(requests, tokens, nq, nkv, code):
     plan, scratch = ops().kv4_plan(requests, -(-tokens // 16), nq, nkv, 128, code)
     assert plan in (-1, -2, -4, -8) or plan > 0
     assert (scratch > 0) == (plan > 0)
+
+
+# ---- NaN where a row's keys are shared out over blocks ---------------------------------------------------------------------------------
+def nan_key(cache, table, d, r, place, head):
+    """Makes a NaN of the scale of the first group of a stored key."""
+    pairs = cache[..., 512 * kv4_refs.groups(d):576 * kv4_refs.groups(d)].view(torch.float16).view(cache.shape[:3] + (16, -1, 2))
+    page = cache.shape[2] * 16
+    pairs[int(table[r, place // page]), head, place % page // 16, place % 16, 0, 0] = math.nan
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("plan", [-1, -2, -4, -8, 1, 7, 40, 296])
+@pytest.mark.parametrize("where", ["query", "key", "newest key"])
+def test_a_nan_score_reaches_its_rows_under_every_plan(where, plan, dtype, monkeypatch, gen):
+    """A NaN in one query head makes NaN of its row, a NaN key of the rows of the heads that see it; the others are what they are without.
+    The newest key of the first request is alone in its tile, and alone in a block's piece where 296 blocks share the tiles."""
+    nq, nkv, d, lengths = 14, 2, 64, [(1, 1024), (1, 3), (1, 700)]
+    q, cache, table, ctx = problem(gen, lengths, nq, nkv, d, dtype)
+    deal_out(monkeypatch, plan, len(lengths), nq, nkv, d)
+    want = kv4_refs.attention64(q, cache, table, ctx.cu_q, ctx.q_start, nq, nkv, d, 16, d ** -0.5).view(3, nq, d)
+    bad = torch.zeros(3, nq, dtype=torch.bool)
+    if where == "query":
+        q[0, 5 * d + 9] = q[2, 13 * d] = math.nan
+        bad[0, 5] = bad[2, 13] = True
+    else:
+        for r, place, head in ((0, 1024, 0), (2, 700, 1)) if where == "newest key" else ((0, 333, 0), (2, 0, 1)):
+            nan_key(cache, table, d, r, place, head)
+            bad[r, 7 * head:7 * head + 7] = True
+    out = ops().paged_attention_kv4(q, cache, table, ctx, nq, nkv, d, 16, d ** -0.5).view(3, nq, d)
+    ops().check_status(DEV)
+    assert torch.equal(out.isnan().cpu(), bad[..., None].expand(3, nq, d))
+    check_attention(out[~bad.to(DEV)], want[~bad], cache, d, f"beside a NaN, plan {plan} {dtype}")
