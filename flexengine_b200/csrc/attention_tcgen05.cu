@@ -833,7 +833,8 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
             // this split's share of the row: O / sum in float32 and the logarithm of the sum, for the merge
             tc_fence_after();
             const float inv = row_sum > 0.f ? 1.f / row_sum : 0.f;
-            if (row_place[tid] >= 0) part_lse[row_place[tid]] = row_sum > 0.f ? m_ref + log2f(row_sum) : -CUDART_INF_F;
+            // a sum that is NaN stays one: -inf says that no key was seen
+            if (row_place[tid] >= 0) part_lse[row_place[tid]] = row_sum > 0.f ? m_ref + log2f(row_sum) : row_sum != row_sum ? row_sum : -CUDART_INF_F;
             float* stage = reinterpret_cast<float*>(kv_s + (size_t)ti * (ROWS * 4 * D) + (warp & 3) * (32 * 4 * D));
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -885,7 +886,7 @@ prefill_merge_kernel(const float* __restrict__ part_o, const float* __restrict__
     const int head = (int)(item % nq);
     const float lse = lane < splits ? part_lse[item * splits + lane] : -CUDART_INF_F;
     const float mx = warp_max(lse);
-    const float w = mx == -CUDART_INF_F ? 0.f : exp2f(lse - mx);       // 0 for a split that saw no key of this row
+    const float w = lse != lse ? lse : mx == -CUDART_INF_F ? 0.f : exp2f(lse - mx);       // 0 for a split that saw no key of this row, NaN as it is
     const float total = warp_sum(w);
     const float inv = added ? 1.f : (total > 0.f ? 1.f / total : 0.f);      // added (sigmoid weights): shares of weight 1, summed
     constexpr int CHUNKS = D / 4;

@@ -534,3 +534,56 @@ def test_a_nan_score_reaches_its_rows_under_every_plan(where, plan, dtype, monke
     ops().check_status(DEV)
     assert torch.equal(out.isnan().cpu(), bad[..., None].expand(3, nq, d))
     check_attention(out[~bad.to(DEV)], want[~bad], cache, d, f"beside a NaN, plan {plan} {dtype}")
+
+
+def split_portions(monkeypatch, splits):
+    monkeypatch.setattr(ops(), "kv4_portions", lambda *a, **k: 0)
+    monkeypatch.setattr(ops(), "prefill_splits", lambda *a, **k: splits)
+
+
+@pytest.mark.parametrize("splits", [1, 3, 8])
+@pytest.mark.parametrize("nq,nkv,d", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("where", ["query", "key", "newest key"])
+def test_a_nan_score_reaches_its_rows_in_split_portions(where, nq, nkv, d, splits, monkeypatch, gen):
+    """As for single tokens: the keys of the tcgen05 kernel shared out over ``splits`` blocks.  The newest key of the first request is alone in its tile."""
+    lengths, G = [(40, 985), (3, 130)], nq // nkv
+    q, cache, table, ctx = problem(gen, lengths, nq, nkv, d, torch.bfloat16, page=32)
+    split_portions(monkeypatch, splits)
+    want = kv4_refs.attention64(q, cache, table, ctx.cu_q, ctx.q_start, nq, nkv, d, 32, d ** -0.5).view(43, nq, d)
+    bad = torch.zeros(43, nq, dtype=torch.bool)
+    if where == "query":
+        q[3, 5 * d + 9] = q[39, 0] = q[42, 7 * d] = math.nan
+        bad[3, 5] = bad[39, 0] = bad[42, 7] = True
+    elif where == "key":
+        nan_key(cache, table, d, 0, 333, 0)
+        nan_key(cache, table, d, 1, 131, 1)
+        bad[:40, :G] = True
+        bad[41:, G:] = True
+    else:
+        nan_key(cache, table, d, 0, 1024, 1)
+        bad[39, G:] = True
+    out = ops().paged_attention_kv4(q, cache, table, ctx, nq, nkv, d, 32, d ** -0.5).view(43, nq, d)
+    ops().check_status(DEV)
+    assert torch.equal(out.isnan().cpu(), bad[..., None].expand(43, nq, d))
+    check_attention(out[~bad.to(DEV)], want[~bad], cache, d, f"beside a NaN, {splits} splits bfloat16")
+
+
+@pytest.mark.parametrize("splits", [1, 4])
+def test_a_nan_query_keeps_its_row_in_split_portions_over_a_16_bit_cache(splits, gen):
+    """The same kernel over keys and values of 16 bits."""
+    nq, nkv, d, pages = 8, 2, 64, 70
+    k, v = (normal(gen, pages, nkv, 16, d).to(torch.bfloat16) for _ in range(2))
+    q = normal(gen, 20, nq * d).to(torch.bfloat16)
+    table = torch.arange(pages, device=DEV, dtype=torch.int32)[None]
+    cu, start = torch.tensor([0, 20], dtype=torch.int32, device=DEV), torch.tensor([1090], dtype=torch.int32, device=DEV)
+
+    def call():
+        return ops().paged_prefill_tcgen05(q, q.stride(0), k, v, table, cu, start, 20, 1, 20, nq, nkv, d, 16, 0.125, 0, splits).view(20, nq, d)
+
+    clean = call()
+    q[7, 3 * d + 1] = math.nan
+    out = call()
+    ops().check_status(DEV)
+    bad = torch.zeros(20, nq, d, dtype=torch.bool, device=DEV)
+    bad[7, 3] = True
+    assert torch.equal(out.isnan(), bad) and torch.equal(out[~bad], clean[~bad])
