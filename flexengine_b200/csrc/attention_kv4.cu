@@ -759,7 +759,7 @@ kv4_attention_kernel(const Problem a) {
             for (int i = lane; i < a.d; i += 32) {
                 float v = 0.f;
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w) v += by[w] != 0.f ? by[w] * from[w][i] : 0.f;
+                for (int w = 0; w < WARPS; ++w) v += by[w] * from[w][i];      // 0 times NaN is NaN, as where one warp has all keys; who saw nothing left zeros
                 if (whole) put<TQ>(to + i, sum != sum ? sum : v * inv);
                 else part[i] = v;
             }
@@ -781,7 +781,7 @@ kv4_attention_kernel(const Problem a) {
                     float v = 0.f;
                     for (unsigned p = 0; p < splits; ++p) {
                         const float weight = __shfl_sync(FULL, by, p);
-                        if (weight != 0.f && i < a.d) v += weight * ld_cluster(own + i, p);
+                        if (i < a.d) v += weight * ld_cluster(own + i, p);
                     }
                     if (i < a.d) put<TQ>(static_cast<TQ*>(a.out) + (long long)token * a.out_stride + (long long)head * a.d + i, sum != sum ? sum : sum > 0.f ? v / sum : 0.f);
                 }

@@ -887,13 +887,14 @@ prefill_merge_kernel(const float* __restrict__ part_o, const float* __restrict__
     const float lse = lane < splits ? part_lse[item * splits + lane] : -CUDART_INF_F;
     const float mx = warp_max(lse);
     const float w = lse != lse ? lse : mx == -CUDART_INF_F ? 0.f : exp2f(lse - mx);       // 0 for a split that saw no key of this row, NaN as it is
+    const unsigned wrote = __ballot_sync(0xffffffffu, lse != -CUDART_INF_F);      // the others may have no share; one whose weight is 0 counts with 0 times its NaN
     const float total = warp_sum(w);
     const float inv = added ? 1.f : (total > 0.f ? 1.f / total : 0.f);      // added (sigmoid weights): shares of weight 1, summed
     constexpr int CHUNKS = D / 4;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s = 0; s < splits; ++s) {
         const float ws = __shfl_sync(0xffffffffu, w, s);
-        if (ws == 0.f || lane >= CHUNKS) continue;                     // such a split's share was never written
+        if (!(wrote >> s & 1u) || lane >= CHUNKS) continue;
         const float4 v = *reinterpret_cast<const float4*>(part_o + (item * splits + s) * D + lane * 4);
         acc.x += ws * v.x; acc.y += ws * v.y; acc.z += ws * v.z; acc.w += ws * v.w;
     }

@@ -587,3 +587,40 @@ def test_a_nan_query_keeps_its_row_in_split_portions_over_a_16_bit_cache(splits,
     bad = torch.zeros(20, nq, d, dtype=torch.bool, device=DEV)
     bad[7, 3] = True
     assert torch.equal(out.isnan(), bad) and torch.equal(out[~bad], clean[~bad])
+
+
+def nan_value(cache, table, d, r, place, head, group):
+    """Makes a NaN of the scale of one group of a stored value."""
+    n, page = kv4_refs.groups(d), cache.shape[2] * 16
+    pairs = cache[..., 576 * n:].view(torch.float16).view(cache.shape[:3] + (16, n, 2))
+    pairs[int(table[r, place // page]), head, place % page // 16, place % 16, group, 0] = math.nan
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("plan", [-1, -2, -4, -8, 1, 7, 40, 296])
+@pytest.mark.parametrize("place", [0, 150, 517, 1024])
+def test_a_nan_value_reaches_rows_in_which_its_weight_is_nothing(place, plan, dtype, monkeypatch, gen):
+    """Scores hundreds apart: all but one key of a row weigh 0 in 32 bits, also where blocks' results are put together.  0 times NaN is NaN."""
+    nq, nkv, d = 14, 2, 64
+    q, cache, table, ctx = problem(gen, [(1, 1024), (1, 40)], nq, nkv, d, dtype)
+    q = (q.float() * 500).to(dtype)
+    deal_out(monkeypatch, plan, 2, nq, nkv, d)
+    nan_value(cache, table, d, 0, place, 1, 1)
+    out = ops().paged_attention_kv4(q, cache, table, ctx, nq, nkv, d, 16, d ** -0.5).view(2, nq, d)
+    bad = torch.zeros(2, nq, d, dtype=torch.bool)
+    bad[0, 7:, 32:] = True
+    assert torch.equal(out.isnan().cpu(), bad)
+
+
+@pytest.mark.parametrize("splits", [1, 3, 8])
+@pytest.mark.parametrize("place", [0, 150, 517, 1020])
+def test_a_nan_value_reaches_rows_in_which_its_weight_is_nothing_in_split_portions(place, splits, monkeypatch, gen):
+    nq, nkv, d = 8, 2, 128
+    q, cache, table, ctx = problem(gen, [(40, 985)], nq, nkv, d, torch.bfloat16)
+    q = (q.float() * 500).to(torch.bfloat16)
+    split_portions(monkeypatch, splits)
+    nan_value(cache, table, d, 0, place, 1, 2)
+    out = ops().paged_attention_kv4(q, cache, table, ctx, nq, nkv, d, 16, d ** -0.5).view(40, nq, d)
+    bad = torch.zeros(40, nq, d, dtype=torch.bool)
+    bad[max(0, place - 985):, 4:, 64:96] = True
+    assert torch.equal(out.isnan().cpu(), bad)
