@@ -1915,7 +1915,7 @@ def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale
     bfloat16 or float32, holds the turned queries in its first nq d columns; returns [T, nq d] of its type.  ``ctx``: the step
     (``cu_q``, ``q_start``, ``max_q_len``, ``max_ctx_len``).  ``window`` > 0: the last so many keys are seen, and with ``keep_first`` the sequence's first
     so many too; ``sink``: 1 is added to the softmax's denominator.  Codes are multiplied as whole numbers; queries and weights go through the
-    products in half precision (csrc/attention_kv4.cu), float32 ones with 22 bits."""
+    products in half precision (csrc/attention_kv4.cu), float32 ones in two parts of it: 22 bits of those near the row's largest."""
     what = "paged_attention_kv4"
     with _on(what, q, cache, block_table, ctx.cu_q, ctx.q_start):
         T, requests, pages, code = q.shape[0], ctx.cu_q.numel() - 1, block_table.shape[-1], _code(q.dtype)

@@ -624,3 +624,20 @@ def test_a_nan_value_reaches_rows_in_which_its_weight_is_nothing_in_split_portio
     bad = torch.zeros(40, nq, d, dtype=torch.bool)
     bad[max(0, place - 985):, 4:, 64:96] = True
     assert torch.equal(out.isnan().cpu(), bad)
+
+
+@pytest.mark.parametrize("plan", [-1, -8, 40])
+@pytest.mark.parametrize("nq,nkv,d", [(4, 1, 64), (7, 1, 128)])
+def test_32_bits_hold_over_a_long_walk(nq, nkv, d, plan, monkeypatch, gen):
+    """32,768 keys of about the same weight under 32-bit queries, walked by one block, by eight, and shared out.
+
+    Relative to the result's norm (about sqrt(n) of n keys' numbers, as the errors of single weights are): a weight is off by its score (a few
+    roundings of 2^-24 of numbers up to 8 in log2 units: 5e-7), its exponential (2^-22) and its two halves (2^-22), some 6e-7 in all; a warp's
+    running sums take up to 512 pairs of products, each with a rounding of 2^-25 on average, sqrt(512 / 2) 2^-25 = 5e-7.  3e-6 is three times as much as
+    the two.  Sums that are cut off instead of rounded at every addition would be off by 512 times 2^-24 or 3e-5."""
+    args = problem(gen, [(1, 32767)], nq, nkv, d, torch.float32, garbage=False)
+    args = (args[0] * 0.15,) + args[1:]
+    deal_out(monkeypatch, plan, 1, nq, nkv, d)
+    out, want = run_attention(*args, nq, nkv, d, 16)
+    off = float((out.cpu().double() - want).norm() / want.norm())
+    assert off <= 3e-6, f"{off:.2e} of the norm"
