@@ -44,7 +44,6 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int PAIR = 2;              // tiles that a warp takes at once
-constexpr long long WAIT_LIMIT = 1000000000LL;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float MOVE_STEP = 8.f;
 
@@ -120,9 +119,9 @@ template <int NG> __device__ __forceinline__ void pieces(const unsigned char* p,
 }
 
 // false when the wait ran out; the test itself waits a while, so the clock is asked rarely
-__device__ __forceinline__ bool wait_for(unsigned long long* bar, unsigned parity) {
+__device__ __forceinline__ bool wait_for(unsigned long long* bar, unsigned parity, long long limit) {
     if (mbar_test(bar, parity)) return true;
-    return mbar_wait(bar, parity, WAIT_LIMIT);
+    return mbar_wait(bar, parity, limit);
 }
 
 __device__ __forceinline__ void copy_tile(unsigned to, const unsigned char* from, int bytes, unsigned bar) {
@@ -163,6 +162,7 @@ struct Problem {
     float* part;            // partial results of the blocks: see the kernel
     long long tokens;       // rows of q
     int* status;
+    FeWaits waits;
 };
 
 // dynamic shared memory: every warp's ring, two places of a pair of tiles each; a warp's results go to the place that no copy is on its way to
@@ -356,7 +356,7 @@ kv4_attention_kernel(const Problem a) {
         if (lane == 0) {
             const unsigned bar = smem_u32(&bars[warp][stage]), to = smem_u32(ring + stage * PAIR * TILE);
             // a tile that is not there brings nothing; the stage's turn passes all the same
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((first >= 0 ? TILE : 0) + (second >= 0 ? TILE : 0)) : "memory");
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((first >= 0 ? TILE : 0) + (second >= 0 ? TILE : 0) + a.waits.lacking) : "memory");
             if (first >= 0) copy_tile(to, a.cache + (long long)first * TILE, TILE, bar);
             if (second >= 0) copy_tile(to + TILE, a.cache + (long long)second * TILE, TILE, bar);
         }
@@ -678,9 +678,13 @@ kv4_attention_kernel(const Problem a) {
 #pragma unroll 1
         for (unsigned k = 0; k < (unsigned)mine && !gone; ++k) {
             if (k + 1 < (unsigned)mine) begin_copy(w, k + 1, stage ^ 1);
-            if (__any_sync(FULL, !wait_for(&bars[warp][stage], parity))) {
+            if (__any_sync(FULL, !wait_for(&bars[warp][stage], parity, a.waits.limit))) {
+                // the row lacks these keys: said in the status word.  Copies on their way are waited for once more before results go where
+                // they may still land, or the block leaves
                 gone = true;
-                if (k + 1 < (unsigned)mine) wait_for(&bars[warp][stage ^ 1], parity ^ stage);
+                if (lane == 0 && a.status) atomicOr(a.status, FE_STATUS_WAIT_EXPIRED);
+                wait_for(&bars[warp][stage], parity, a.waits.limit);
+                if (k + 1 < (unsigned)mine) wait_for(&bars[warp][stage ^ 1], parity ^ stage, a.waits.limit);
                 break;
             }
             // the batch of pair k is that of the newest copy or the one before
@@ -1010,7 +1014,7 @@ extern "C" int fe_paged_attention_kv4(const void* q, long long q_stride, void* o
     FE_REQUIRE(dtype == FE_F32 || dtype == FE_BF16, "paged_attention_kv4: unknown type %d", dtype);
     if (requests == 0 || max_q_len == 0 || tokens == 0) return 0;
     const Problem a{q, q_stride, out, out_stride, (const unsigned char*)cache, block_table, bt_stride, cu_q, q_start, requests, nq, nkv, d, ps, num_pages,
-                    scale * LOG2E, window, keep, sink, splits, (float*)scratch, tokens, status};
+                    scale * LOG2E, window, keep, sink, splits, (float*)scratch, tokens, status, fe_waits()};
     const Launch w{&a, requests, (int)(((long long)max_q_len * (nq / nkv) + 7) / 8), blocks, stream};
     return dtype == FE_F32 ? with_groups(d, [&](auto n) { return run<float, n.value, 1>(w); }) : with_groups(d, [&](auto n) { return run<bf16, n.value, 1>(w); });
 }

@@ -169,6 +169,10 @@ int fe_check_launch(const char* what);
 int fe_pdl_enabled();
 void fe_share_carveout(const void* kernel);       // the split of an SM's memory that overlapping kernels share
 bool fe_allow_smem(const void* kernel, int bytes);      // up to so many bytes of dynamic shared memory for the kernel on the current device
+// A kernel's waits for its own bulk copies: how many clock cycles each may take, and how many bytes more than come are expected (0; otherwise
+// the waits run out, for the sake of seeing what is then reported).
+struct FeWaits { long long limit; int lacking; };
+FeWaits fe_waits();
 int fe_sm_count();      // multiprocessors of the current device (asked once per device)
 
 // Classes of kernels for fe_set_pdl: a source file names its own before including this header.

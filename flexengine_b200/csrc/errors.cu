@@ -96,6 +96,16 @@ bool fe_allow_smem(const void* kernel, int bytes) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
 }
 
+static std::atomic<long long> g_wait_limit{1000000000LL};
+static std::atomic<int> g_wait_lacking{0};
+
+FeWaits fe_waits() { return FeWaits{g_wait_limit.load(std::memory_order_relaxed), g_wait_lacking.load(std::memory_order_relaxed)}; }
+
+extern "C" void fe_set_waits(long long limit, int lacking) {
+    g_wait_limit.store(limit > 0 ? limit : 1000000000LL, std::memory_order_relaxed);
+    g_wait_lacking.store(lacking > 0 ? lacking : 0, std::memory_order_relaxed);
+}
+
 extern "C" const char* fe_last_error() { return g_last_error; }
 
 extern "C" int fe_abi_version() { return 1; }

@@ -641,3 +641,30 @@ def test_32_bits_hold_over_a_long_walk(nq, nkv, d, plan, monkeypatch, gen):
     out, want = run_attention(*args, nq, nkv, d, 16)
     off = float((out.cpu().double() - want).norm() / want.norm())
     assert off <= 3e-6, f"{off:.2e} of the norm"
+
+
+# ---- a wait that runs out ----------------------------------------------------------------------------------------------------------
+@pytest.fixture()
+def short_waits():
+    """Copies that are said to bring 16 bytes more than they do, so that every wait for them runs out after some 50 us, as long as the test lasts."""
+    libraries = [ops()._kv4(), ops()._bf16()]
+    for library in libraries:
+        library.fe_set_waits(100000, 16)
+    yield
+    for library in libraries:
+        library.fe_set_waits(0, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("plan", [-1, -4, 1, 7, 40])
+def test_a_wait_that_runs_out_is_reported_by_single_tokens(plan, dtype, monkeypatch, gen, request):
+    q, cache, table, ctx = problem(gen, [(1, 1030), (1, 3), (1, 700)], 14, 2, 64, dtype)
+    deal_out(monkeypatch, plan, 3, 14, 2, 64)
+    request.getfixturevalue("short_waits")
+    ops().paged_attention_kv4(q, cache, table, ctx, 14, 2, 64, 16, 0.125)
+    with pytest.raises(RuntimeError, match="wait"):
+        ops().check_status(DEV)
+    for library in (ops()._kv4(), ops()._bf16()):
+        library.fe_set_waits(0, 0)
+    out, want = run_attention(q, cache, table, ctx, 14, 2, 64, 16)          # the device is as it was
+    check_attention(out, want, cache, 64, f"after a wait that ran out, plan {plan} {dtype}")
