@@ -56,12 +56,12 @@ constexpr long long WAIT_LIMIT = 2000000000LL;
 constexpr float RESCALE_STEP = 8.f;      // log2 of the growth of a row's maximum that moves its reference point
 
 // false when the wait ran out or another thread of the block has given up; sets the flag itself then
-__device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned parity, volatile int* give_up) {
+__device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned parity, volatile int* give_up, long long limit = WAIT_LIMIT) {
     if (mbar_test(bar, parity)) return true;
     const long long t0 = clock64();
     while (!mbar_test(bar, parity)) {
         if (*give_up) return false;
-        if (clock64() - t0 > WAIT_LIMIT) {
+        if (clock64() - t0 > limit) {
             *give_up = 1;
             return false;
         }
@@ -382,7 +382,7 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
                              const int* __restrict__ block_table, int bt_stride, const int* __restrict__ cu_q,
                              const int* __restrict__ q_start, int requests, int nq, int nkv, int ps, int num_pages, float scale_log2,
                              int window, int keep, int mode, int splits, float* __restrict__ part_o, float* __restrict__ part_lse,
-                             int* __restrict__ status, const float* __restrict__ per_head, float cap_log2) {
+                             int* __restrict__ status, const float* __restrict__ per_head, float cap_log2, const FeWaits waits) {
     const bool sink = mode & 1, sigmoid = mode & 2;         // bit 1: sigmoid(score + per_head[head]) instead of a softmax
     const bool mapped = mode & 4;       // scores times per_head[head] (null: 1) and, with a cap, cap tanh(score / cap), before the softmax
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -544,7 +544,7 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
             const unsigned here = __ballot_sync(FULL, there), missing = __ballot_sync(FULL, wanted && !there);
             if (lane == 0) {
                 missing_of[stage] = missing;
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(&raw_full[stage])), "r"((int)__popc(here) * SUB_BYTES) : "memory");
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(&raw_full[stage])), "r"((int)__popc(here) * SUB_BYTES + waits.lacking) : "memory");
             }
             __syncwarp();
             if (there)
@@ -565,7 +565,7 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
                 start(j + 2, page);
             }
             const int s = j % KV_STAGES, stage = j % RAW_STAGES;
-            mbar_wait(&raw_full[stage], (j / RAW_STAGES) & 1, &give_up);
+            mbar_wait(&raw_full[stage], (j / RAW_STAGES) & 1, &give_up, waits.limit);
             mbar_wait(&kv_empty[s], ((j / KV_STAGES) & 1) ^ 1, &give_up);
             const int key0 = listed_tile<KEYS>(t_begin + j, kept, lo) * KEYS;
             const unsigned missing = missing_of[stage];
@@ -608,8 +608,8 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
             mbar_arrive(&kv_full[s]);
             // the raw tile is read: its place may be filled; all loaders leave together
             if (loader_any(give_up != 0)) {
-                for (int later = j + 1; later <= j + 2 && later < n_tiles; ++later)       // copies on their way to memory that the block is about to leave
-                    fe::mbar_wait(&raw_full[later % RAW_STAGES], (later / RAW_STAGES) & 1, WAIT_LIMIT);
+                for (int later = j; later <= j + 2 && later < n_tiles; ++later)       // copies on their way to memory that the block is about to leave, this tile's among them
+                    fe::mbar_wait(&raw_full[later % RAW_STAGES], (later / RAW_STAGES) & 1, waits.limit);
                 break;
             }
         }
@@ -925,7 +925,7 @@ int launch(const void* q, long long q_stride, void* out, long long out_stride, c
     float* part_lse = splits > 1 ? scratch + (size_t)total_tokens * nq * splits * D : nullptr;
     fe::launch(paged_prefill_tcgen05_kernel<D, FOUR>, dim3((unsigned)blocks), THREADS, smem, stream, (const bf16*)q, q_stride,
                (bf16*)out, out_stride, (const bf16*)kc, (const bf16*)vc, block_table, bt_stride, cu_q, q_start, requests, nq, nkv, ps,
-               num_pages, scale * LOG2E, window, keep, sink, splits, part_o, part_lse, status, per_head, softcap * LOG2E);
+               num_pages, scale * LOG2E, window, keep, sink, splits, part_o, part_lse, status, per_head, softcap * LOG2E, fe_waits());
     if (fe_check_launch("paged_prefill_tcgen05")) return 1;
     if (splits > 1) {
         const long long items = total_tokens * nq;

@@ -668,3 +668,18 @@ def test_a_wait_that_runs_out_is_reported_by_single_tokens(plan, dtype, monkeypa
         library.fe_set_waits(0, 0)
     out, want = run_attention(q, cache, table, ctx, 14, 2, 64, 16)          # the device is as it was
     check_attention(out, want, cache, 64, f"after a wait that ran out, plan {plan} {dtype}")
+
+
+@pytest.mark.parametrize("splits", [1, 4])
+@pytest.mark.parametrize("nq,nkv,d", [(14, 2, 64), (8, 2, 128)])
+def test_a_wait_that_runs_out_is_reported_by_portions(nq, nkv, d, splits, monkeypatch, gen, request):
+    q, cache, table, ctx = problem(gen, [(40, 985), (3, 130)], nq, nkv, d, torch.bfloat16)
+    split_portions(monkeypatch, splits)
+    request.getfixturevalue("short_waits")
+    ops().paged_attention_kv4(q, cache, table, ctx, nq, nkv, d, 16, 0.125)
+    with pytest.raises(RuntimeError, match="wait"):
+        ops().check_status(DEV)
+    for library in (ops()._kv4(), ops()._bf16()):
+        library.fe_set_waits(0, 0)
+    out, want = run_attention(q, cache, table, ctx, nq, nkv, d, 16)
+    check_attention(out, want, cache, d, "after a wait that ran out bfloat16")
