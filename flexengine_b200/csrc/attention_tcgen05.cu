@@ -386,7 +386,7 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
     const bool sink = mode & 1, sigmoid = mode & 2;         // bit 1: sigmoid(score + per_head[head]) instead of a softmax
     const bool mapped = mode & 4;       // scores times per_head[head] (null: 1) and, with a cap, cap tanh(score / cap), before the softmax
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long kv_full[KV_STAGES], kv_empty[KV_STAGES], s_ready[2][2], p_ready[2][2], pv_done[2], o_final[2];
+    __shared__ __align__(8) unsigned long long kv_full[KV_STAGES], kv_empty[KV_STAGES], s_ready[2][2], p_ready[2][2], pv_done[2], o_final[2], left[2];
     __shared__ long long offs[2][KEYS];
     __shared__ unsigned tmem_holder;
     __shared__ volatile int give_up;
@@ -454,6 +454,7 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
             for (int b = 0; b < 2; ++b) { mbar_init(&s_ready[i][b], 1); mbar_init(&p_ready[i][b], 128); }
             mbar_init(&pv_done[i], 1);
             mbar_init(&o_final[i], 1);
+            mbar_init(&left[i], 1);
         }
         if (FOUR) {
             for (int i = 0; i < RAW_STAGES; ++i) mbar_init(&raw_full[i], 1);
@@ -709,6 +710,11 @@ paged_prefill_tcgen05_kernel(const bf16* __restrict__ q, long long q_stride, bf1
                 }
             }
             if (ok) umma_commit(&o_final[i]);
+            else {
+                // products that are still at work read shared memory and write tensor memory that the block is about to leave
+                umma_commit(&left[i]);
+                fe::mbar_wait(&left[i], 0, WAIT_LIMIT);
+            }
         }
         __syncwarp();
     } else if (softmax_thread) {
