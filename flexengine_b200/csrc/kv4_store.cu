@@ -223,7 +223,7 @@ template <typename TI, typename TO>
 __global__ void __launch_bounds__(STAY_WARPS * 32)
 kv4_store_many_kernel(const TI* __restrict__ src, long long ld, const float* __restrict__ bias, const int* __restrict__ positions, Rotation turn,
                       const int* __restrict__ slot_mapping, unsigned char* __restrict__ cache, TO* __restrict__ queries, int T, int nq, int nkv, int d,
-                      int ps, long long num_slots, int* __restrict__ status) {
+                      int ps, long long num_slots, int* __restrict__ status, const FeWaits waits) {
     griddep_wait();
     griddep_launch_dependents();
     extern __shared__ __align__(128) unsigned char smem[];
@@ -239,7 +239,7 @@ kv4_store_many_kernel(const TI* __restrict__ src, long long ld, const float* __r
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     __syncthreads();
     auto bring = [&](int token, int place) {
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(&arrived[place])), "r"((int)(width * sizeof(TI))) : "memory");
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(&arrived[place])), "r"((int)(width * sizeof(TI)) + waits.lacking) : "memory");
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                      ::"r"(smem_u32(rows + (size_t)place * width)), "l"(src + (long long)token * ld), "r"((int)(width * sizeof(TI))), "r"(smem_u32(&arrived[place])) : "memory");
     };
@@ -271,10 +271,12 @@ kv4_store_many_kernel(const TI* __restrict__ src, long long ld, const float* __r
         const Place to = places[turn_of];
         const int row_codes = to.at * 16 * groups, row_pairs = to.at * 4 * groups;
         const float *cosines = cosine[turn_of], *sines = sine[turn_of];
-        const bool here = mbar_wait(&arrived[place], parity, 1000000000LL);
+        const bool here = mbar_wait(&arrived[place], parity, waits.limit);
         if (!here) {
+            // the copies on their way go to memory that the block is about to leave: this token's once more, and the next one's
             if (status) atomicOr(status, FE_STATUS_WAIT_EXPIRED);
-            if (next < T) mbar_wait(&arrived[place ^ 1], parity ^ place, 1000000000LL);
+            mbar_wait(&arrived[place], parity, waits.limit);
+            if (next < T) mbar_wait(&arrived[place ^ 1], parity ^ place, waits.limit);
         }
         if (__syncthreads_or(!here)) return;
         for (int u0 = 0; u0 < units; u0 += 32) {
@@ -396,7 +398,7 @@ int store(const void* src, long long ld, const float* bias, const int* positions
         FE_REQUIRE(fe_allow_smem((const void*)kernel, (int)smem), "qkv_rope_kv4: no kernel with %d bytes of shared memory", (int)smem);
         // not among the overlapping launches: the split of an SM's memory that they share leaves room for one such block, not two
         fe::launch_as(0, kernel, dim3((unsigned)(2 * sms)), STAY_WARPS * 32, smem, stream, (const TI*)src, ld, bias, positions, turn, slots, (unsigned char*)cache,
-                   (TO*)queries, T, nq, nkv, d, ps, num_slots, status);
+                   (TO*)queries, T, nq, nkv, d, ps, num_slots, status, fe_waits());
         return fe_check_launch("qkv_rope_kv4");
     }
     // a block a token, or, where that gives multiprocessors less than one, a block for every eight rows of a token, each with its own angles

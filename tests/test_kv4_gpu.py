@@ -683,3 +683,24 @@ def test_a_wait_that_runs_out_is_reported_by_portions(nq, nkv, d, splits, monkey
         library.fe_set_waits(0, 0)
     out, want = run_attention(q, cache, table, ctx, nq, nkv, d, 16)
     check_attention(out, want, cache, d, "after a wait that ran out bfloat16")
+
+
+def test_a_wait_that_runs_out_is_reported_by_the_store(gen, request):
+    """Enough tokens for the blocks that fetch rows by bulk copies."""
+    T, nq, nkv, d = 700, 2, 2, 64
+    projected = normal(gen, T, 6 * d)
+    slots, positions = torch.arange(T, device=DEV, dtype=torch.int32), torch.zeros(T, device=DEV, dtype=torch.int32)
+    caches = [torch.zeros(kv4_shape(44, nkv, 16, d), dtype=torch.uint8, device=DEV) for _ in range(2)]
+
+    def store(cache):
+        return ops().qkv_rope_kv4(projected, None, positions, None, 0, slots, cache, nq, nkv, d, 16)
+
+    want = store(caches[0])
+    ops().check_status(DEV)
+    request.getfixturevalue("short_waits")
+    store(caches[1])
+    with pytest.raises(RuntimeError, match="wait"):
+        ops().check_status(DEV)
+    ops()._kv4().fe_set_waits(0, 0)
+    assert torch.equal(store(caches[1]), want) and torch.equal(caches[0], caches[1])
+    ops().check_status(DEV)
