@@ -23,6 +23,7 @@
 
 #define FE_PDL_CLASS 8      // FE_PDL_SAMPLING
 #include "common.cuh"
+#include "cut.cuh"
 
 using namespace fe;
 
@@ -634,10 +635,10 @@ sample_filtered_kernel(const Rows of, const int C) {
                     cluster_sum(here_mass, nothing, none);
                 }
                 if (by_mass && of_whole) limit = share * (double)everything;
-                const double before = by_mass ? (double)above : (double)above_count, here = by_mass ? (double)here_mass : (double)n;
                 // the coarse sums may be a step off
-                if (before >= limit && at > 0 && above_count > 0) { --at; continue; }
-                if (before + here < limit && at + 1 < STEPS) { ++at; continue; }
+                const int way = by_mass ? cut_way(above, here_mass, limit) : cut_way(above_count, (unsigned)n, limit);
+                if (way < 0 && at > 0 && above_count > 0) { --at; continue; }
+                if (way > 0 && at + 1 < STEPS) { ++at; continue; }
                 if (whole) {
                     // the last that stays: the one of highest place before which less than the limit lies
                     if (tid == 0) s.found_count = 0;

@@ -283,3 +283,31 @@ def test_portions_choose_their_kernel():
     assert of(1, 100000, 1000, window=64) in (0, 1)
     assert kv4_portions([0, 3], [50, 0], 4, 2, 64, sms=148) == 1
     assert kv4_portions([1], [0], 64, 1, 64, sms=148) == 1
+
+
+# ---- the walk to a limit of the sampling kernel -----------------------------------------------------------------------------------
+def test_the_walk_to_a_limit_never_turns_back(tmp_path):
+    """What one step sends on, the next does not send back: sums of 62 bits, whose limits lie next to the border between the two."""
+    import ctypes
+    import os
+    import random
+    import subprocess
+    from flexengine_b200.ops import library
+    source = tmp_path / "way.cpp"
+    source.write_text('#include "cut.cuh"\nextern "C" int way(unsigned long long before, unsigned long long here, double limit)'
+                      ' { return fe::cut_way(before, here, limit); }\n')
+    built = str(tmp_path / "way.so")
+    subprocess.run(["g++", "-O2", "-shared", "-fPIC", "-I", library.CSRC, "-o", built, str(source)], check=True, timeout=120)
+    way = ctypes.CDLL(built).way
+    way.argtypes = [ctypes.c_ulonglong, ctypes.c_ulonglong, ctypes.c_double]
+    rng = random.Random(3)
+    pairs = [(1772367175443750147, 501071425968473999)] + [(rng.randrange(1 << 62), rng.randrange(1 << rng.randrange(50, 62))) for _ in range(5000)]
+    for before, here in pairs:
+        after = before + here
+        near = np.float64(after)
+        for limit in (np.nextafter(near, 0), near, np.nextafter(near, np.inf), float(before), float(before) + float(here)):
+            first, then = way(before, here, limit), way(after, 1, limit)
+            assert not (first > 0 and then < 0), (before, here, limit)
+            assert first <= 0 or float(after) < limit
+            assert first >= 0 or float(before) >= limit
+    assert [way(5, 3, 5.0), way(5, 3, 5.5), way(5, 3, 8.0), way(5, 3, 8.5), way(0, 0, 1.0)] == [-1, 0, 0, 1, 1]
