@@ -116,6 +116,7 @@ struct Shared {
     unsigned found_count;
     int found_at;
     long long roots[ROOTS];
+    unsigned char held[THREADS];
 };
 
 // What a row's masses are made of.  A mass is a whole number, rounded down, right to 2^-32 of itself: where logits are equal, as 16-bit ones
@@ -428,6 +429,11 @@ sample_filtered_kernel(const Rows of, const int C) {
             coarse[e] = use_p ? __float2ull_rn((float)flat[e] * expf(-(float)(4 * tid + e) * (1.f / STEPS_A_UNIT)) * 65536.f) : 0;
             own_coarse += coarse[e];
         }
+        // bit e: step 4 tid + e holds a token (a mass is 2^COARSE_BITS (1 - 1/128) at least); kept by its own thread, in shared memory for the registers' sake
+        unsigned occupied = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) occupied |= (unsigned)(count[e] > 0 || flat[e] > 0) << e;
+        s.held[tid] = (unsigned char)occupied;
         u64 all_count, all_coarse;
         const u64 count_before = block_before64(own_count, all_count, s);
         const u64 coarse_before = block_before64(own_coarse, all_coarse, s);
@@ -614,6 +620,22 @@ sample_filtered_kernel(const Rows of, const int C) {
         }
         // ---- the long way: one limit after the other, each an exact cut (thr, need)
         // ``limit`` in tokens or in mass, or (of_whole) the mass's share of the row's; ``at``: the step that is likely to hold it
+        // the next step after ``at`` that holds a token, STEPS where there is none; the last one before it, -1
+        auto next_held = [&](int at, bool after) {
+            if (tid == 0) s.found_at = after ? STEPS : -1;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int step = 4 * tid + e;
+                if (!(s.held[tid] >> e & 1)) continue;
+                if (after && step > at) atomicMin(&s.found_at, step);
+                if (!after && step < at) atomicMax(&s.found_at, step);
+            }
+            __syncthreads();
+            const int found = s.found_at;
+            __syncthreads();
+            return found;
+        };
         u64 last_entry = 0;                                // of the last cut: the last listed token that stays
         auto cut = [&](bool by_mass, double limit, int at) {
             const double share = limit;
@@ -635,10 +657,16 @@ sample_filtered_kernel(const Rows of, const int C) {
                     cluster_sum(here_mass, nothing, none);
                 }
                 if (by_mass && of_whole) limit = share * (double)everything;
-                // the coarse sums may be a step off
+                // the coarse sums may be a step off: on to the next that holds anything, however far
                 const int way = by_mass ? cut_way(above, here_mass, limit) : cut_way(above_count, (unsigned)n, limit);
-                if (way < 0 && at > 0 && above_count > 0) { --at; continue; }
-                if (way > 0 && at + 1 < STEPS) { ++at; continue; }
+                if (way < 0 && at > 0 && above_count > 0) {
+                    const int back = next_held(at, false);
+                    if (back >= 0) { at = back; continue; }
+                }
+                if (way > 0 && at + 1 < STEPS) {
+                    const int on = next_held(at, true);
+                    if (on < STEPS) { at = on; continue; }
+                }
                 if (whole) {
                     // the last that stays: the one of highest place before which less than the limit lies
                     if (tid == 0) s.found_count = 0;

@@ -175,3 +175,43 @@ def test_an_infinite_temperature_leaves_the_finite_logits_alike(top_p, top_k):
         assert given["logits"].gather(1, tokens.long()[:, None]).isfinite().all()
         assert kept.tolist() == [n] * R
         torch.testing.assert_close(probability, torch.full_like(probability, 1 / n), rtol=1e-6, atol=0.0)
+
+
+def levels(distance, numbers, seed):
+    """A row of few different logits, ``distance`` apart, ``numbers`` of each in a random order; and the shares of the mass that the first levels hold."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.cat([torch.full((n,), -distance * j) for j, n in enumerate(numbers)])
+    x = x[torch.randperm(len(x), generator=g)]
+    held = torch.tensor([n * math.exp(float(torch.tensor(-distance * j).double())) for j, n in enumerate(numbers)], dtype=torch.float64)
+    return x.to(DEV), (held.cumsum(0) / held.sum()).tolist()
+
+
+@pytest.mark.parametrize("distance", [1.003, 1.0052, 0.6931])
+def test_a_limit_next_to_the_border_of_far_apart_logits(distance):
+    """Thousands of equal logits in each of a few steps far apart, and top-p next to the mass of the first of them: the coarse sums (13 bits a token)
+    take the limit to lie on one side of the border or the other, and the exact ones decide.  Nothing lies in the steps between: they
+    are not gone through one by one, so that such a row takes no more than a few walks longer than one whose limit lies well inside a level."""
+    x, shares = levels(distance, [3000, 5000, 4000, 6000, 3500], 1)
+    for blocks in (1, 8):
+        slow, usual = 0.0, 0.0
+        for level in range(4):
+            for off in (-3e-5, -3e-6, -4e-7, 4e-7, 3e-6, 3e-5, 0.03):
+                p = shares[level] * (1 + off)
+                given = dict(logits=x[None].contiguous(), temperature=torch.ones(1, device=DEV), top_k=torch.zeros(1, dtype=torch.int32, device=DEV),
+                             top_p=torch.tensor([p], device=DEV), min_p=torch.zeros(1, device=DEV), uniform=torch.tensor([0.3], device=DEV))
+                check(given, blocks=(blocks,), what=f"level {level} off {off}")
+                times = []
+                for _ in range(7):
+                    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                    torch.cuda.synchronize()
+                    a.record()
+                    ops().sample_filtered(**given, blocks=blocks)
+                    b.record()
+                    torch.cuda.synchronize()
+                    times.append(a.elapsed_time(b))
+                t = sorted(times)[3]
+                if off == 0.03:
+                    usual = max(usual, t)
+                else:
+                    slow = max(slow, t)
+        assert slow <= 3 * usual, f"{blocks} blocks: {1000 * slow:.0f} us against {1000 * usual:.0f}"
