@@ -140,10 +140,12 @@ class Sampler:
         for p, m in zip(top_ps, min_ps):
             validate_filters(p, m)
         columns = [list(v) for v in (temperatures, top_ks, seeds, draws)]
-        mine = [i for i in range(n) if columns[0][i] != 0.0 and (top_ps[i] < 1.0 or min_ps[i] > 0.0)]
+        mine, others = [], []
+        for i in range(n):
+            (mine if columns[0][i] != 0.0 and (top_ps[i] < 1.0 or min_ps[i] > 0.0) else others).append(i)
         if not mine:
             return self.sample_on_device(logits, *columns)
-        r, others = len(mine), [i for i in range(n) if i not in set(mine)]
+        r = len(mine)
         # one host buffer, one copy: temperatures, top_ps, min_ps, uniforms, top_ks and these rows' numbers, then the other rows', 4 bytes each
         packed = torch.empty(6 * r + len(others), dtype=torch.int32, pin_memory=dev.type == "cuda")
         host = packed.numpy()

@@ -311,3 +311,28 @@ def test_the_walk_to_a_limit_never_turns_back(tmp_path):
             assert first <= 0 or float(after) < limit
             assert first >= 0 or float(before) >= limit
     assert [way(5, 3, 5.0), way(5, 3, 5.5), way(5, 3, 8.0), way(5, 3, 8.5), way(0, 0, 1.0)] == [-1, 0, 0, 1, 1]
+
+
+def test_the_host_s_work_grows_with_the_batch_not_its_square():
+    """Half the rows with a limit: eight times the rows take about eight times as long (64 times where each row looks through all of them)."""
+    import time
+
+    class Nothing:
+        @staticmethod
+        def sample(logits, *_):
+            return torch.zeros(logits.shape[0], dtype=torch.int32)
+
+        @staticmethod
+        def sample_filtered(logits, *_):
+            return (torch.zeros(logits.shape[0], dtype=torch.int32),)
+
+    def seconds(n):
+        logits, best = torch.zeros(n, 1), 1e9
+        for _ in range(5):
+            start = time.perf_counter()
+            Sampler(Nothing).sample_on_device(logits, [1.0] * n, [0] * n, list(range(n)), [0] * n, [0.5, 1.0] * (n // 2), [0.0] * n)
+            best = min(best, time.perf_counter() - start)
+        return best
+
+    seconds(64)
+    assert seconds(4096) <= 24 * seconds(512)
