@@ -2,6 +2,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 
 #include "common.cuh"
 
@@ -71,29 +72,39 @@ void fe_share_carveout(const void* kernel) {
 }
 
 // A kernel's largest block of dynamic shared memory is the driver's to know: told once a kernel, size and device, since a launch should not pay for
-// the call (about a microsecond).
+// the call (about a microsecond).  It is only ever raised, one thread at a time: of two that set it and then write it down, the one with the larger number
+// could do the first before the other and the second after it.
 bool fe_allow_smem(const void* kernel, int bytes) {
     constexpr int SLOTS = 256;
     static std::atomic<const void*> kernels[64][SLOTS];
     static std::atomic<int> allowed[64][SLOTS];
+    static std::mutex raising;
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return false;
-    size_t at = ((size_t)kernel >> 4) % SLOTS;
-    for (int i = 0; i < SLOTS; ++i, at = (at + 1) % SLOTS) {
-        const void* have = kernels[device][at].load(std::memory_order_acquire);
-        if (have == kernel && allowed[device][at].load(std::memory_order_relaxed) >= bytes) return true;
-        if (have == kernel || have == nullptr) {
-            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-                cudaGetLastError();
-                return false;
-            }
-            const void* none = nullptr;
-            if (have == nullptr && !kernels[device][at].compare_exchange_strong(none, kernel)) return true;      // another thread took the place: asked again next time
-            allowed[device][at].store(bytes, std::memory_order_relaxed);
-            return true;
+    const size_t home = ((size_t)kernel >> 4) % SLOTS;
+    auto place = [&] {                              // of the kernel, or the first empty one; SLOTS: none
+        for (int i = 0; i < SLOTS; ++i) {
+            const size_t at = (home + i) % SLOTS;
+            const void* have = kernels[device][at].load(std::memory_order_acquire);
+            if (have == kernel || have == nullptr) return at;
         }
+        return (size_t)SLOTS;
+    };
+    size_t at = place();
+    if (at < SLOTS && kernels[device][at].load(std::memory_order_acquire) == kernel && allowed[device][at].load(std::memory_order_relaxed) >= bytes) return true;
+    std::lock_guard<std::mutex> one(raising);
+    at = place();                                   // another kernel may have taken the empty place meanwhile
+    const bool listed = at < SLOTS && kernels[device][at].load(std::memory_order_relaxed) == kernel;
+    if (listed && allowed[device][at].load(std::memory_order_relaxed) >= bytes) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
     }
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+    if (at < SLOTS) {
+        allowed[device][at].store(bytes, std::memory_order_relaxed);
+        kernels[device][at].store(kernel, std::memory_order_release);
+    }
+    return true;
 }
 
 static std::atomic<long long> g_wait_limit{1000000000LL};

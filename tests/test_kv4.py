@@ -336,3 +336,69 @@ def test_the_host_s_work_grows_with_the_batch_not_its_square():
 
     seconds(64)
     assert seconds(4096) <= 24 * seconds(512)
+
+
+# ---- how much shared memory a kernel may have --------------------------------------------------------------------------------------
+HARNESS = r"""
+// errors.cu on a driver that is played: the call for LATE bytes holds on until another call has come and gone.
+#include <cuda_runtime.h>
+#include <atomic>
+#include <chrono>
+#include <cstdio>
+#include <thread>
+
+static std::atomic<int> set_to{0}, calls{0}, refuse{0};
+static std::atomic<bool> hold{false}, inside{false};
+static constexpr int LATE = 100;
+static cudaError_t played_set(const void*, cudaFuncAttribute, int bytes) {
+    if (refuse) return cudaErrorInvalidValue;
+    ++calls;
+    set_to = bytes;
+    if (bytes == LATE && hold) {
+        inside = true;
+        for (int i = 0; i < 400 && calls < 2; ++i) std::this_thread::sleep_for(std::chrono::milliseconds(1));      // a lock keeps the other out: no longer than that
+        std::this_thread::sleep_for(std::chrono::milliseconds(50));
+    }
+    return cudaSuccess;
+}
+static cudaError_t played_device(int* device) { *device = 0; return cudaSuccess; }
+#define cudaFuncSetAttribute played_set
+#define cudaGetDevice played_device
+#include "errors.cu"
+
+int main() {
+    static char kernels[2];
+    const void *first = (const void*)((size_t)kernels & ~(size_t)15), *second = (const void*)((size_t)first + 4096);
+    fe_allow_smem(first, 10);
+    calls = 0;
+    hold = true;
+    std::thread wide([&] { fe_allow_smem(first, LATE); });
+    while (!inside) std::this_thread::yield();
+    std::thread narrow([&] { fe_allow_smem(first, 50); });
+    wide.join();
+    narrow.join();
+    hold = false;
+    if (!fe_allow_smem(first, LATE)) return 1;
+    std::printf("%d\n", set_to.load());
+    // one after the other: raised, never lowered, and not asked for again
+    calls = 0;
+    fe_allow_smem(second, 30), fe_allow_smem(second, 60), fe_allow_smem(second, 40), fe_allow_smem(second, 60);
+    std::printf("%d %d\n", set_to.load(), calls.load());
+    refuse = 1;
+    const bool refused = !fe_allow_smem(second, 70), still = fe_allow_smem(second, 60);
+    std::printf("%d %d\n", (int)refused, (int)still);
+    return 0;
+}
+"""
+
+
+def test_two_threads_do_not_lower_what_shared_memory_a_kernel_may_have(tmp_path):
+    """A thread that asks for 50 bytes while another is on its way to 100: afterwards a kernel that needs 100 has them."""
+    import subprocess
+    from flexengine_b200.ops import library
+    source = tmp_path / "harness.cu"
+    source.write_text(HARNESS)
+    built = str(tmp_path / "harness")
+    subprocess.run([library.find_nvcc(), "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-I", library.CSRC, "-o", built, str(source)], check=True, timeout=300)
+    out = subprocess.run([built], capture_output=True, text=True, check=True, timeout=60).stdout.split("\n")
+    assert out[:3] == ["100", "60 2", "1 1"]
