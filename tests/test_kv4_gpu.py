@@ -704,3 +704,20 @@ def test_a_wait_that_runs_out_is_reported_by_the_store(gen, request):
     ops()._kv4().fe_set_waits(0, 0)
     assert torch.equal(store(caches[1]), want) and torch.equal(caches[0], caches[1])
     ops().check_status(DEV)
+
+
+def test_special_numbers_leave_nan_where_they_were_and_nowhere_else(gen):
+    """NaN among the keys and among the values, in groups of their own: the group reads as NaN, whole, and no other."""
+    x = normal(gen, 7, 4, 64)
+    x[0], x[1, :, 3], x[2, :, 40] = 2.5, 1e30, -math.inf
+    x[4, 2, 50] = x[5, 3, 7] = x[6, 3, 63] = math.nan
+    x[3, 1, 7] = math.nan                                  # of a query
+    cache = torch.full(kv4_shape(2, 1, 16, 64), 255, dtype=torch.uint8, device=DEV)
+    slots = torch.arange(3, 10, dtype=torch.int32, device=DEV)
+    q = ops().qkv_rope_kv4(x.reshape(7, -1), None, torch.zeros(7, dtype=torch.int32, device=DEV), None, 0, slots, cache, 2, 1, 64, 16)
+    ops().check_status(DEV)
+    keys, values = ops().kv4_rows(cache, slots, 1, 64, 16, torch.float32)
+    bad = torch.zeros(2, 7, 1, 64, dtype=torch.bool, device=DEV)
+    bad[0, 4, 0, 32:] = bad[1, 5, 0, :32] = bad[1, 6, 0, 32:] = True
+    assert torch.equal(keys.isnan(), bad[0]) and torch.equal(values.isnan(), bad[1])
+    assert q.isnan().nonzero().tolist() == [[3, 64 + 7]]
