@@ -1927,6 +1927,8 @@ def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale
         _index_ok(what, "block_table", block_table, requests, pages)
         if window < 0 or keep_first < 0 or (keep_first and not window):
             raise ValueError(f"{what}: a window is not negative, and kept first keys go with one")
+        if not 0.0 <= scale < float("inf"):
+            raise ValueError(f"{what}: scores are multiplied by a finite number that is not negative, not {scale}")
         if ctx.max_ctx_len > pages * page_size:
             raise ValueError(f"{what}: {ctx.max_ctx_len} tokens in {pages} pages of {page_size}")
         out = q.new_empty((T, nq * d))

@@ -402,3 +402,9 @@ def test_two_threads_do_not_lower_what_shared_memory_a_kernel_may_have(tmp_path)
     subprocess.run([library.find_nvcc(), "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-I", library.CSRC, "-o", built, str(source)], check=True, timeout=300)
     out = subprocess.run([built], capture_output=True, text=True, check=True, timeout=60).stdout.split("\n")
     assert out[:3] == ["100", "60 2", "1 1"]
+
+
+@pytest.mark.parametrize("scale", [-0.125, float("nan"), float("inf"), -float("inf")])
+def test_attention_refuses_scales_that_would_turn_masks_into_numbers(unlaunched, scale):
+    with pytest.raises(ValueError, match="not negative"):
+        unlaunched.paged_attention_kv4(**dict(attention_arguments(), scale=scale))
