@@ -43,6 +43,7 @@ using namespace fe;
 namespace {
 
 constexpr int WARPS = 4;
+constexpr int COLS = 8;             // columns that a block takes: (query, head of the group) pairs
 constexpr int PAIR = 2;              // tiles that a warp takes at once
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float MOVE_STEP = 8.f;
@@ -168,8 +169,8 @@ struct Problem {
 // dynamic shared memory: every warp's ring, two places of a pair of tiles each; a warp's results go to the place that no copy is on its way to
 constexpr int STAGES = 2;
 template <int NG> __host__ __device__ constexpr int ring_bytes() { return WARPS * STAGES * PAIR * kv4_tile_bytes(NG); }
-template <int NG, int NT> __host__ __device__ constexpr int smem_bytes() {
-    static_assert(8 * NT * (32 * NG + 4) * 4 <= PAIR * kv4_tile_bytes(NG), "a warp's results fit a pair of tiles");
+template <int NG> __host__ __device__ constexpr int smem_bytes() {
+    static_assert(COLS * (32 * NG + 4) * 4 <= PAIR * kv4_tile_bytes(NG), "a warp's results fit a pair of tiles");
     return ring_bytes<NG>();
 }
 
@@ -203,9 +204,9 @@ __device__ __forceinline__ int tiles_of(const Problem& a, int r) {
 
 // Blocks that are resident on an SM: the registers are cut to that.  16-bit queries at head size 128: four blocks of 128 registers a thread (three of 168
 // take the same time for long rows and leave fewer blocks to short ones).
-template <typename TQ, int NG, int NT> __host__ __device__ constexpr int blocks_an_sm() { return sizeof(TQ) == 2 && NG * NT <= 4 ? 4 : 2; }
+template <typename TQ, int NG> __host__ __device__ constexpr int blocks_an_sm() { return sizeof(TQ) == 2 && NG <= 4 ? 4 : 2; }
 
-// TQ: queries and output; 32-bit ones in two parts.  NG: groups of a row.  NT: tiles of eight columns that a block takes.
+// TQ: queries and output; 32-bit ones in two parts.  NG: groups of a row.
 //
 // SHARED = false: grid (column tiles x splits, heads, requests), the splits of a column tile a thread-block cluster, each with an equal share of its
 // tiles; their results are merged through distributed shared memory: no second kernel.
@@ -213,20 +214,20 @@ template <typename TQ, int NG, int NT> __host__ __device__ constexpr int blocks_
 // equal shares as there are blocks, whole rounds of the block's warps each; a block then takes the pieces of items that its share holds.  So
 // lengths that differ leave no block without work (a split of every item into equal parts left a seventh of the time to the last
 // blocks), and nothing on the host depends on them.  A block's share ends at most one item that others began and begins at
-// most one that others end: its partial results are 2 b (an item begun before) and 2 b + 1 (an item begun here).  ``part``: [blocks][2][8 NT]
+// most one that others end: its partial results are 2 b (an item begun before) and 2 b + 1 (an item begun here).  ``part``: [blocks][2][COLS]
 // [32 NG + 4] floats (numbers, maximum, sum), then for each item which blocks hold it.
 struct Held { int from, to; };      // blocks from .. to - 1; one block: it wrote the result itself
-template <int NG, int NT> __host__ __device__ constexpr int part_floats() { return 8 * NT * (32 * NG + 4); }
+template <int NG> __host__ __device__ constexpr int part_floats() { return COLS * (32 * NG + 4); }
 
-template <typename TQ, int NG, int NT, bool SHARED>
-__global__ void __launch_bounds__(WARPS * 32, blocks_an_sm<TQ, NG, NT>())
+template <typename TQ, int NG, bool SHARED>
+__global__ void __launch_bounds__(WARPS * 32, blocks_an_sm<TQ, NG>())
 kv4_attention_kernel(const Problem a) {
     griddep_wait();
     griddep_launch_dependents();
     constexpr int PARTS = sizeof(TQ) == 4 ? 2 : 1;
     constexpr bool EXACT = PARTS == 2;                   // scales and centres of values in 32 bits
     constexpr int GONE = 0x40000000;                     // a key that nobody sees
-    constexpr int COLS = 8 * NT, TILE = kv4_tile_bytes(NG);
+    constexpr int TILE = kv4_tile_bytes(NG);
     constexpr unsigned FULL = 0xffffffffu;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) unsigned long long bars[WARPS][STAGES];
@@ -238,8 +239,8 @@ kv4_attention_kernel(const Problem a) {
 
     // ---- what this block does; each warp keeps the piece in hand in shared memory, for the registers' sake
     __shared__ Segment pieces_of[WARPS];
-    __shared__ __align__(16) uint4 operands[PARTS][NT][NG][32];           // of the queries; the four warps make them together and read them as they go
-    __shared__ __align__(8) float2 lifts[NT][NG][32];
+    __shared__ __align__(16) uint4 operands[PARTS][NG][32];           // of the queries; the four warps make them together and read them as they go
+    __shared__ __align__(8) float2 lifts[NG][32];
     __shared__ int last_keys[COLS], first_keys[COLS];
     Segment& w = pieces_of[warp];
     Segment found{};
@@ -367,109 +368,104 @@ kv4_attention_kernel(const Problem a) {
     for (bool more = true; more;) {
         const int m0 = w.m0, columns = w.columns, tok0 = w.tok0, start = w.start, kvh = w.kvh, lo = w.lo, kept = w.kept, t_begin = w.t_begin, t_end = w.t_end, slot = w.slot;
 
-        // ---- the queries: column n of tile j as B operands; thread (g, t) holds numbers 32 i + 8 t .. + 7 of column g
+        // ---- the queries as B operands, a column each; thread (g, t) holds numbers 32 i + 8 t .. + 7 of column g
         // Keys' codes are multiplied raised (by 1024 or 64: kv4_raise) where queries are 16-bit; ``lift`` is what that adds to a group's partial
         // score, and eight codes' worth more, with the sign turned: the sums begin there.  That costs their last bits: with |q| in [1, 2)
         // they are off by about 2^-24 8,000, a thousandth of what rounding the query to bfloat16 did.  (Values are summed over all keys,
         // where the part of 1024 would grow: they are decoded in full, and so are keys under 32-bit queries.)
         constexpr bool RAISED = PARTS == 1;
-        unsigned qsum[NT][2];                                // (high, low) of the sums over group t, and over group t + 4
-        float factor[NT][2];                                 // takes a score of columns 2t, 2t + 1 to log2 units
-        float below[NT][2], l[NT][2];                        // minus the reference point (infinite before the first key), the sum
+        unsigned qsum[2];                                // (high, low) of the sums over group t, and over group t + 4
+        float factor[2];                                 // takes a score of columns 2t, 2t + 1 to log2 units
+        float below[2], l[2];                        // minus the reference point (infinite before the first key), the sum
         int last_least = 0x7fffffff, first_most = 0;
+        const int c = m0 + g;
+        const bool real = c < columns;
+        const TQ* row = static_cast<const TQ*>(a.q) + (long long)(tok0 + (real ? c / G : 0)) * a.q_stride + (long long)(kvh * G + (real ? c % G : 0)) * a.d;
+        float v[NG][8], largest = 0.f;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int c = m0 + 8 * j + g;
-            const bool real = c < columns;
-            const TQ* row = static_cast<const TQ*>(a.q) + (long long)(tok0 + (real ? c / G : 0)) * a.q_stride + (long long)(kvh * G + (real ? c % G : 0)) * a.d;
-            float v[NG][8], largest = 0.f;
+        for (int i = 0; i < NG; ++i) {
+            const int from = 32 * i + 8 * t;
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const int from = 32 * i + 8 * t;
+            for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+            if (real && from < a.d) load8<TQ>(row + from, v[i]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-                if (real && from < a.d) load8<TQ>(row + from, v[i]);
+            for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(v[i][e]));
+        }
+        largest = fmaxf(largest, __shfl_xor_sync(FULL, largest, 1));
+        largest = fmaxf(largest, __shfl_xor_sync(FULL, largest, 2));
+        // a power of two brings the row's largest number to [1, 2): half precision then holds bfloat16 numbers as they are
+        const int e2 = min(max((int)(__float_as_uint(largest) >> 23) - 127, -126), 126);
+        const float down = __uint_as_float((unsigned)(127 - e2) << 23);
+        float group_sum[2] = {0.f, 0.f};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(v[i][e]));
+        for (int i = 0; i < NG; ++i) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { v[i][e] *= down; sum += v[i][e]; }
+            sum += __shfl_xor_sync(FULL, sum, 1);
+            sum += __shfl_xor_sync(FULL, sum, 2);
+            if (i == t) group_sum[0] = sum;
+            if (i == t + 4) group_sum[1] = sum;
+            if (i % WARPS != warp) continue;                          // the other warps make the other groups' operands
+            unsigned high[4], rest[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                high[e] = pack(v[i][e], v[i][e + 4]);
+                if (PARTS == 2) rest[e] = pack_rest(v[i][e], v[i][e + 4], high[e]);
             }
-            largest = fmaxf(largest, __shfl_xor_sync(FULL, largest, 1));
-            largest = fmaxf(largest, __shfl_xor_sync(FULL, largest, 2));
-            // a power of two brings the row's largest number to [1, 2): half precision then holds bfloat16 numbers as they are
-            const int e2 = min(max((int)(__float_as_uint(largest) >> 23) - 127, -126), 126);
-            const float down = __uint_as_float((unsigned)(127 - e2) << 23);
-            float group_sum[2] = {0.f, 0.f};
+            operands[0][i][lane] = make_uint4(high[0], high[1], high[2], high[3]);
+            if (PARTS == 2) operands[PARTS - 1][i][lane] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+            float raised = 0.f;
+            if (RAISED) {
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                float sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) { v[i][e] *= down; sum += v[i][e]; }
-                sum += __shfl_xor_sync(FULL, sum, 1);
-                sum += __shfl_xor_sync(FULL, sum, 2);
-                if (i == t) group_sum[0] = sum;
-                if (i == t + 4) group_sum[1] = sum;
-                if (i % WARPS != warp) continue;                          // the other warps make the other groups' operands
-                unsigned high[4], rest[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    high[e] = pack(v[i][e], v[i][e + 4]);
-                    if (PARTS == 2) rest[e] = pack_rest(v[i][e], v[i][e + 4], high[e]);
-                }
-                operands[0][j][i][lane] = make_uint4(high[0], high[1], high[2], high[3]);
-                if (PARTS == 2) operands[PARTS - 1][j][i][lane] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
-                float raised = 0.f;
-                if (RAISED) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        raised -= ((e & 1 ? KV4_RAISED_ODD : KV4_RAISED_EVEN) + 8.f) * (low_half(high[e]) + high_half(high[e]));
-                    raised += __shfl_xor_sync(FULL, raised, 1);
-                    raised += __shfl_xor_sync(FULL, raised, 2);
-                }
-                lifts[j][i][lane] = make_float2(__shfl_sync(FULL, raised, 8 * t), __shfl_sync(FULL, raised, 8 * t + 4));      // of columns 2t and 2t + 1
+                for (int e = 0; e < 4; ++e)
+                    raised -= ((e & 1 ? KV4_RAISED_ODD : KV4_RAISED_EVEN) + 8.f) * (low_half(high[e]) + high_half(high[e]));
+                raised += __shfl_xor_sync(FULL, raised, 1);
+                raised += __shfl_xor_sync(FULL, raised, 2);
             }
+            lifts[i][lane] = make_float2(__shfl_sync(FULL, raised, 8 * t), __shfl_sync(FULL, raised, 8 * t + 4));      // of columns 2t and 2t + 1
+        }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float high = __half2float(__float2half_rn(group_sum[h]));
-                qsum[j][h] = pack(high, group_sum[h] - high);
-            }
-            // a padding column sees what the last query sees: it is computed and never written, and must not make a tile a masked one
-            const int pos = real ? start + c / G : w.hi, from = real ? first_visible(pos, a.window) : lo;
-            last_least = min(last_least, pos);
-            first_most = max(first_most, from);
-            if (warp == 0 && t == 0) { last_keys[8 * j + g] = pos; first_keys[8 * j + g] = from; }
+        for (int h = 0; h < 2; ++h) {
+            const float high = __half2float(__float2half_rn(group_sum[h]));
+            qsum[h] = pack(high, group_sum[h] - high);
+        }
+        // a padding column sees what the last query sees: it is computed and never written, and must not make a tile a masked one
+        const int pos = real ? start + c / G : w.hi, from = real ? first_visible(pos, a.window) : lo;
+        last_least = min(last_least, pos);
+        first_most = max(first_most, from);
+        if (warp == 0 && t == 0) { last_keys[g] = pos; first_keys[g] = from; }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                factor[j][h] = a.scale_log2 * __uint_as_float((unsigned)(127 + __shfl_sync(FULL, e2, (2 * t + h) * 4)) << 23);
-                below[j][h] = CUDART_INF_F;
-                l[j][h] = 0.f;
-                if (a.sink && t_begin == 0 && warp == 0) {
-                    below[j][h] = 0.f;
-                    l[j][h] = g == 0 ? 1.f : 0.f;            // the lanes of a column add their sums up at the end
-                }
+        for (int h = 0; h < 2; ++h) {
+            factor[h] = a.scale_log2 * __uint_as_float((unsigned)(127 + __shfl_sync(FULL, e2, (2 * t + h) * 4)) << 23);
+            below[h] = CUDART_INF_F;
+            l[h] = 0.f;
+            if (a.sink && t_begin == 0 && warp == 0) {
+                below[h] = 0.f;
+                l[h] = g == 0 ? 1.f : 0.f;            // the lanes of a column add their sums up at the end
             }
         }
         last_least = __reduce_min_sync(FULL, last_least);
         first_most = __reduce_max_sync(FULL, first_most);
         __syncthreads();
 
-        float o[NT][NG][2][4], oc[NT][NG][2];                // sums over codes (EXACT) or numbers, 16 a tile, and over centres (EXACT, this thread's tokens)
+        float o[NG][2][4], oc[NG][2];                // sums over codes (EXACT) or numbers, 16 a tile, and over centres (EXACT, this thread's tokens)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int i = 0; i < NG; ++i) {
+            oc[i][0] = oc[i][1] = 0.f;
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                oc[j][i][0] = oc[j][i][1] = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][i][0][e] = o[j][i][1][e] = 0.f;
-            }
+            for (int e = 0; e < 4; ++e) o[i][0][e] = o[i][1][e] = 0.f;
+        }
 
         // places [clear_from, clear_to) of the list are seen whole by every column (kept tiles are taken with the masked)
         const int clear_from = kept + (first_most + KV4_TILE - 1) / KV4_TILE - lo / KV4_TILE;
         const int clear_to = min(t_end, kept + (last_least + 1) / KV4_TILE - lo / KV4_TILE);
-        unsigned poisoned = 0;                                            // bit (j NG + i) 2 + h: column 2t + h of tile j has seen a NaN in group i of the values
+        unsigned poisoned = 0;                                            // bit 2 i + h: column 2t + h has seen a NaN in group i of the values
         // a pair of tiles; ``place``: of the first in the list; ``here``: which of the two were brought
         auto take = [&](auto masked_tag, const unsigned char* pair, int place, unsigned here) {
             constexpr bool MASKED = decltype(masked_tag)::value;
             // ---- scores of tokens key_row and key_row + 8 of each tile by columns 2t, 2t + 1
-            float s[PAIR][NT][4];
+            float s[PAIR][4];
 #pragma unroll
             for (int u = 0; u < PAIR; ++u) {
                 const unsigned char* tile = pair + u * TILE;
@@ -485,8 +481,7 @@ kv4_attention_kernel(const Problem a) {
                     const unsigned w1 = *reinterpret_cast<const unsigned*>(pairs + t * 4 + 16 + 32 * NG);
                     c2 = __byte_perm(w0, w0, 0x3232); c3 = __byte_perm(w1, w1, 0x3232);
                 }
-#pragma unroll
-                for (int j = 0; j < NT; ++j) mma_from(s[u][j], c0, c1, c2, c3, qsum[j][0], NG > 4 ? qsum[j][1] : 0u, 0.f, 0.f);
+                mma_from(s[u], c0, c1, c2, c3, qsum[0], NG > 4 ? qsum[1] : 0u, 0.f, 0.f);
                 unsigned k0[NG], k1[NG], p0[NG], p1[NG];
                 words<NG>(tile + key_codes, k0);
                 words<NG>(tile + key_codes + 128 * NG, k1);
@@ -498,28 +493,25 @@ kv4_attention_kernel(const Problem a) {
                     if (RAISED) { kv4_raise(k0[i], n0); kv4_raise(k1[i], n1); }
                     else { kv4_decode(k0[i], n0); kv4_decode(k1[i], n1); }
                     const float s0 = low_half(p0[i]), s1 = low_half(p1[i]);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        float part[4];
-                        const uint4 q = operands[0][j][i][lane];
-                        const float2 lift = RAISED ? lifts[j][i][lane] : make_float2(0.f, 0.f);
-                        mma_from(part, n0[0], n1[0], n0[1], n1[1], q.x, q.y, lift.x, lift.y);
-                        mma(part, n0[2], n1[2], n0[3], n1[3], q.z, q.w);
-                        if (PARTS == 2) {
-                            const uint4 rest = operands[PARTS - 1][j][i][lane];
-                            mma(part, n0[0], n1[0], n0[1], n1[1], rest.x, rest.y);
-                            mma(part, n0[2], n1[2], n0[3], n1[3], rest.z, rest.w);
-                        }
-                        s[u][j][0] = fmaf(s0, part[0], s[u][j][0]);
-                        s[u][j][1] = fmaf(s0, part[1], s[u][j][1]);
-                        s[u][j][2] = fmaf(s1, part[2], s[u][j][2]);
-                        s[u][j][3] = fmaf(s1, part[3], s[u][j][3]);
+                    float part[4];
+                    const uint4 q = operands[0][i][lane];
+                    const float2 lift = RAISED ? lifts[i][lane] : make_float2(0.f, 0.f);
+                    mma_from(part, n0[0], n1[0], n0[1], n1[1], q.x, q.y, lift.x, lift.y);
+                    mma(part, n0[2], n1[2], n0[3], n1[3], q.z, q.w);
+                    if (PARTS == 2) {
+                        const uint4 rest = operands[PARTS - 1][i][lane];
+                        mma(part, n0[0], n1[0], n0[1], n1[1], rest.x, rest.y);
+                        mma(part, n0[2], n1[2], n0[3], n1[3], rest.z, rest.w);
                     }
+                    s[u][0] = fmaf(s0, part[0], s[u][0]);
+                    s[u][1] = fmaf(s0, part[1], s[u][1]);
+                    s[u][2] = fmaf(s1, part[2], s[u][2]);
+                    s[u][3] = fmaf(s1, part[3], s[u][3]);
                 }
             }
             // ---- weights
             unsigned v0[PAIR][NG], v1[PAIR][NG];                          // EXACT: (scale, centre) of the two tokens' value groups
-            float up0[PAIR], up1[PAIR], y[PAIR][NT][4];
+            float up0[PAIR], up1[PAIR], y[PAIR][4];
             bool grows = false;
 #pragma unroll
             for (int u = 0; u < PAIR; ++u) {
@@ -539,14 +531,12 @@ kv4_attention_kernel(const Problem a) {
                         if (key0 + key_row + 8 > w.hi) v1[u][i] = 0;
                     }
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int key = key0 + key_row + (e & 2) * 4;
-                            const int column = 8 * j + 2 * t + (e & 1);
-                            if (!(key <= last_keys[column] && (key >= first_keys[column] || key < a.keep))) s[u][j][e] = -CUDART_INF_F;
-                            else poisoned |= (e < 2 ? nan0 : nan1) << (2 * NG * j + (e & 1));
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + key_row + (e & 2) * 4;
+                        const int column = 2 * t + (e & 1);
+                        if (!(key <= last_keys[column] && (key >= first_keys[column] || key < a.keep))) s[u][e] = -CUDART_INF_F;
+                        else poisoned |= (e < 2 ? nan0 : nan1) << (e & 1);
+                    }
                 }
                 if (EXACT) {
                     float big0 = low_half(v0[u][0]), big1 = low_half(v1[u][0]);
@@ -557,53 +547,47 @@ kv4_attention_kernel(const Problem a) {
                     up1[u] = fmaxf((float)(__float_as_uint(big1) >> 23) - 127.f, -24.f);
                 }
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        y[u][j][e] = fmaf(s[u][j][e], factor[j][e & 1], below[j][e & 1]);
-                        grows |= y[u][j][e] > MOVE_STEP - (e < 2 ? up0[u] : up1[u]);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    y[u][e] = fmaf(s[u][e], factor[e & 1], below[e & 1]);
+                    grows |= y[u][e] > MOVE_STEP - (e < 2 ? up0[u] : up1[u]);
+                }
             }
             if (__any_sync(FULL, grows)) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+                for (int h = 0; h < 2; ++h) {
+                    float mx = -CUDART_INF_F;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float mx = -CUDART_INF_F;
+                    for (int u = 0; u < PAIR; ++u)
+                        mx = fmaxf(mx, fmaxf(fmaf(s[u][h], factor[h], up0[u]), fmaf(s[u][h + 2], factor[h], up1[u])));
 #pragma unroll
-                        for (int u = 0; u < PAIR; ++u)
-                            mx = fmaxf(mx, fmaxf(fmaf(s[u][j][h], factor[j][h], up0[u]), fmaf(s[u][j][h + 2], factor[j][h], up1[u])));
+                    for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, off));
+                    const float to = fmaxf(-below[h], mx);
+                    const float by = to == -CUDART_INF_F ? 1.f : ex2(-below[h] - to);      // 2^-inf = 0 at the start
+                    below[h] = -to;
+                    l[h] *= by;
 #pragma unroll
-                        for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, off));
-                        const float to = fmaxf(-below[j][h], mx);
-                        const float by = to == -CUDART_INF_F ? 1.f : ex2(-below[j][h] - to);      // 2^-inf = 0 at the start
-                        below[j][h] = -to;
-                        l[j][h] *= by;
-#pragma unroll
-                        for (int i = 0; i < NG; ++i) {
-                            if (EXACT) oc[j][i][h] *= by;
-                            o[j][i][0][h] *= by; o[j][i][0][h + 2] *= by;
-                            o[j][i][1][h] *= by; o[j][i][1][h + 2] *= by;
-                        }
-#pragma unroll
-                        for (int u = 0; u < PAIR; ++u) {
-                            y[u][j][h] = fmaf(s[u][j][h], factor[j][h], -to);
-                            y[u][j][h + 2] = fmaf(s[u][j][h + 2], factor[j][h], -to);
-                        }
+                    for (int i = 0; i < NG; ++i) {
+                        if (EXACT) oc[i][h] *= by;
+                        o[i][0][h] *= by; o[i][0][h + 2] *= by;
+                        o[i][1][h] *= by; o[i][1][h + 2] *= by;
                     }
+#pragma unroll
+                    for (int u = 0; u < PAIR; ++u) {
+                        y[u][h] = fmaf(s[u][h], factor[h], -to);
+                        y[u][h + 2] = fmaf(s[u][h + 2], factor[h], -to);
+                    }
+                }
             }
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int u = 0; u < PAIR; ++u) {
 #pragma unroll
-                for (int u = 0; u < PAIR; ++u) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        y[u][j][e] = ex2(y[u][j][e]);
-                        if (MASKED && s[u][j][e] == -CUDART_INF_F) y[u][j][e] = 0.f;      // a column that has seen nothing yet has no reference point
-                    }
-                    l[j][0] += y[u][j][0] + y[u][j][2];
-                    l[j][1] += y[u][j][1] + y[u][j][3];
+                for (int e = 0; e < 4; ++e) {
+                    y[u][e] = ex2(y[u][e]);
+                    if (MASKED && s[u][e] == -CUDART_INF_F) y[u][e] = 0.f;      // a column that has seen nothing yet has no reference point
                 }
+                l[0] += y[u][0] + y[u][2];
+                l[1] += y[u][1] + y[u][3];
+            }
             // ---- values: tokens even, odd (+ 8) in pairs; numbers 32 i + 4 g .. + 3
 #pragma unroll
             for (int u = 0; u < PAIR; ++u) {
@@ -615,7 +599,7 @@ kv4_attention_kernel(const Problem a) {
                 pieces<NG>(tile + even_codes + 128 * NG, ve8);
                 pieces<NG>(tile + odd_codes + 128 * NG, vo8);
                 // EXACT = false: one operand of weights for all groups, and scale and centre in the decoded numbers, which half precision rounds by 2^-12
-                unsigned pe[NG], po[NG], pe8[NG], po8[NG], b0[NT], b1[NT];
+                unsigned pe[NG], po[NG], pe8[NG], po8[NG], b0, b1;
                 if (!EXACT) {
                     const unsigned char* pairs = tile + kv4_value_pairs(NG);
                     words<NG>(pairs + even * 4 * NG, pe);
@@ -632,11 +616,8 @@ kv4_attention_kernel(const Problem a) {
                             if ((po8[i] & 0x7c00u) == 0x7c00u || key0 + odd + 8 > w.hi) po8[i] = 0;
                         }
                     }
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        b0[j] = transposed(pack(y[u][j][0], y[u][j][1]));
-                        b1[j] = transposed(pack(y[u][j][2], y[u][j][3]));
-                    }
+                    b0 = transposed(pack(y[u][0], y[u][1]));
+                    b1 = transposed(pack(y[u][2], y[u][3]));
                 }
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
@@ -646,31 +627,25 @@ kv4_attention_kernel(const Problem a) {
                     if constexpr (!EXACT) {
                         times_plus(na, __byte_perm(pe[i], po[i], 0x5410), __byte_perm(pe[i], po[i], 0x7632));
                         times_plus(nb, __byte_perm(pe8[i], po8[i], 0x5410), __byte_perm(pe8[i], po8[i], 0x7632));
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            mma(o[j][i][0], na[0], na[1], nb[0], nb[1], b0[j], b1[j]);
-                            mma(o[j][i][1], na[2], na[3], nb[2], nb[3], b0[j], b1[j]);
-                        }
+                        mma(o[i][0], na[0], na[1], nb[0], nb[1], b0, b1);
+                        mma(o[i][1], na[2], na[3], nb[2], nb[3], b0, b1);
                     } else {
                         const float s0 = low_half(v0[u][i]), s1 = low_half(v1[u][i]), c0 = high_half(v0[u][i]), c1 = high_half(v1[u][i]);
+                        const float* w = y[u];
+                        oc[i][0] = fmaf(w[0], c0, fmaf(w[2], c1, oc[i][0]));
+                        oc[i][1] = fmaf(w[1], c0, fmaf(w[3], c1, oc[i][1]));
+                        const unsigned w0 = pack(w[0] * s0, w[1] * s0), w1 = pack(w[2] * s1, w[3] * s1);
+                        const unsigned h0 = transposed(w0), h1 = transposed(w1);
+                        const unsigned r0 = transposed(pack_rest(w[0] * s0, w[1] * s0, w0)), r1 = transposed(pack_rest(w[2] * s1, w[3] * s1, w1));
+                        // A tile's products begin at zero and are added by the CUDA cores: the tensor cores' sums are cut off, not rounded,
+                        // and kept there over 32,768 keys they were off by 9.8e-6 of the result's norm (so 1.8e-7; 8 x 2,048 keys take 13.3 us instead of 13.1)
+                        float first[4], second[4];
+                        mma_from(first, na[0], na[1], nb[0], nb[1], h0, h1, 0.f, 0.f);
+                        mma_from(second, na[2], na[3], nb[2], nb[3], h0, h1, 0.f, 0.f);
+                        mma(first, na[0], na[1], nb[0], nb[1], r0, r1);
+                        mma(second, na[2], na[3], nb[2], nb[3], r0, r1);
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            const float* w = y[u][j];
-                            oc[j][i][0] = fmaf(w[0], c0, fmaf(w[2], c1, oc[j][i][0]));
-                            oc[j][i][1] = fmaf(w[1], c0, fmaf(w[3], c1, oc[j][i][1]));
-                            const unsigned w0 = pack(w[0] * s0, w[1] * s0), w1 = pack(w[2] * s1, w[3] * s1);
-                            const unsigned h0 = transposed(w0), h1 = transposed(w1);
-                            const unsigned r0 = transposed(pack_rest(w[0] * s0, w[1] * s0, w0)), r1 = transposed(pack_rest(w[2] * s1, w[3] * s1, w1));
-                            // A tile's products begin at zero and are added by the CUDA cores: the tensor cores' sums are cut off, not rounded,
-                            // and kept there over 32,768 keys they were off by 9.8e-6 of the result's norm (so 1.8e-7; 8 x 2,048 keys take 13.3 us instead of 13.1)
-                            float first[4], second[4];
-                            mma_from(first, na[0], na[1], nb[0], nb[1], h0, h1, 0.f, 0.f);
-                            mma_from(second, na[2], na[3], nb[2], nb[3], h0, h1, 0.f, 0.f);
-                            mma(first, na[0], na[1], nb[0], nb[1], r0, r1);
-                            mma(second, na[2], na[3], nb[2], nb[3], r0, r1);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) { o[j][i][0][e] += first[e]; o[j][i][1][e] += second[e]; }
-                        }
+                        for (int e = 0; e < 4; ++e) { o[i][0][e] += first[e]; o[i][1][e] += second[e]; }
                     }
                 }
             }
@@ -709,40 +684,34 @@ kv4_attention_kernel(const Problem a) {
         // ---- the warp's sums over its lanes, then the four warps' results side by side: [warp][column][32 NG numbers, maximum, sum]
         constexpr int ROW = 32 * NG + 4;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int off = 4; off < 32; off <<= 1) {
+                l[h] += __shfl_xor_sync(FULL, l[h], off);
+                if (!EXACT) continue;                                 // no sums over centres: it only brings NaN
 #pragma unroll
-                for (int off = 4; off < 32; off <<= 1) {
-                    l[j][h] += __shfl_xor_sync(FULL, l[j][h], off);
-                    if (!EXACT) continue;                                 // no sums over centres: it only brings NaN
-#pragma unroll
-                    for (int i = 0; i < NG; ++i) oc[j][i][h] += __shfl_xor_sync(FULL, oc[j][i][h], off);
-                }
+                for (int i = 0; i < NG; ++i) oc[i][h] += __shfl_xor_sync(FULL, oc[i][h], off);
             }
+        }
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) poisoned |= __shfl_xor_sync(FULL, poisoned, off);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int i = 0; i < NG; ++i)
 #pragma unroll
-            for (int i = 0; i < NG; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (poisoned >> (2 * (j * NG + i) + h) & 1u) oc[j][i][h] = CUDART_NAN_F;
+            for (int h = 0; h < 2; ++h)
+                if (poisoned >> (2 * i + h) & 1u) oc[i][h] = CUDART_NAN_F;
         if (SHARED && lane == 0) result_place[warp] = (int)(stage ^ 1);
         __syncwarp();
         float* mine_results = results_of(warp);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int h = 0; h < 2; ++h) {
+            float* to = mine_results + (2 * t + h) * ROW;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float* to = mine_results + (8 * j + 2 * t + h) * ROW;
-#pragma unroll
-                for (int i = 0; i < NG; ++i)
-                    *reinterpret_cast<float4*>(to + 32 * i + 4 * g) =
-                        make_float4(o[j][i][0][h] + oc[j][i][h], o[j][i][0][h + 2] + oc[j][i][h], o[j][i][1][h] + oc[j][i][h], o[j][i][1][h + 2] + oc[j][i][h]);
-                if (g == 0) { to[32 * NG] = -below[j][h]; to[32 * NG + 1] = l[j][h]; }
-            }
+            for (int i = 0; i < NG; ++i)
+                *reinterpret_cast<float4*>(to + 32 * i + 4 * g) =
+                    make_float4(o[i][0][h] + oc[i][h], o[i][0][h + 2] + oc[i][h], o[i][1][h] + oc[i][h], o[i][1][h + 2] + oc[i][h]);
+            if (g == 0) { to[32 * NG] = -below[h]; to[32 * NG + 1] = l[h]; }
+        }
         __syncthreads();
         for (int c = warp; c < COLS && m0 + c < columns; c += WARPS) {
             const int mc = m0 + c, token = tok0 + mc / G, head = kvh * G + mc % G;
@@ -799,7 +768,7 @@ kv4_attention_kernel(const Problem a) {
         }
         if (SHARED && t_begin == 0 && threadIdx.x == 0) {
             // which blocks hold this item
-            Held* held = reinterpret_cast<Held*>(a.part + (long long)gridDim.x * 2 * part_floats<NG, NT>());
+            Held* held = reinterpret_cast<Held*>(a.part + (long long)gridDim.x * 2 * part_floats<NG>());
             const int b = (int)blockIdx.x;
             held[item] = Held{b, slot < 0 ? b + 1 : item_last / share + 1};
         }
@@ -814,16 +783,16 @@ constexpr int MERGE_THREADS = 256;
 // A block per (head, request): what several blocks hold of an item is weighted by their maxima and added.  Sets of threads, four numbers of
 // the head a thread, take every sets-th part, AHEAD parts on their way at once, with a running maximum of their own; the sets are
 // added in their order.
-template <typename TQ, int NG, int NT>
+template <typename TQ, int NG>
 __global__ void __launch_bounds__(MERGE_THREADS)
 kv4_merge_kernel(const Problem a, int blocks) {
     griddep_wait();
     griddep_launch_dependents();
-    constexpr int COLS = 8 * NT, ROW = 32 * NG + 4, SETS = MERGE_THREADS / (8 * NG), AHEAD = 8;
+    constexpr int ROW = 32 * NG + 4, SETS = MERGE_THREADS / (8 * NG), AHEAD = 8;
     __shared__ __align__(16) float sums[SETS][ROW];
     const int r = blockIdx.y, head = blockIdx.x, G = a.nq / a.nkv, kvh = head / G, m = head % G;
     const int token = a.cu_q[r], behind = a.cu_q[r + 1];
-    const Held held = reinterpret_cast<const Held*>(a.part + (long long)blocks * 2 * part_floats<NG, NT>())[(r * a.nkv + kvh) * ((G + COLS - 1) / COLS) + m / COLS];
+    const Held held = reinterpret_cast<const Held*>(a.part + (long long)blocks * 2 * part_floats<NG>())[(r * a.nkv + kvh) * ((G + COLS - 1) / COLS) + m / COLS];
     if (min((long long)behind, a.tokens) <= token) return;
     const int n = held.to - held.from;
     if (n <= 1) return;
@@ -883,15 +852,15 @@ kv4_merge_kernel(const Problem a, int blocks) {
 }
 
 // Blocks of the kernel that the device holds at once (asked of the driver once per device).
-template <typename TQ, int NG, int NT> int resident() {
+template <typename TQ, int NG> int resident() {
     static int cached[64];
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 0;
     if (cached[device] == 0) {
         int each = 0;
-        constexpr int smem = smem_bytes<NG, NT>();
-        cudaFuncSetAttribute(kv4_attention_kernel<TQ, NG, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kv4_attention_kernel<TQ, NG, NT, true>, WARPS * 32, smem) != cudaSuccess || each < 1) {
+        constexpr int smem = smem_bytes<NG>();
+        cudaFuncSetAttribute(kv4_attention_kernel<TQ, NG, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kv4_attention_kernel<TQ, NG, true>, WARPS * 32, smem) != cudaSuccess || each < 1) {
             cudaGetLastError();
             each = 1;
         }
@@ -906,10 +875,10 @@ struct Launch {
     cudaStream_t stream;
 };
 
-template <typename TQ, int NG, int NT> int run(const Launch& w) {
-    constexpr int smem = smem_bytes<NG, NT>();
+template <typename TQ, int NG> int run(const Launch& w) {
+    constexpr int smem = smem_bytes<NG>();
     const Problem& a = *w.a;
-    auto kernel = w.blocks ? kv4_attention_kernel<TQ, NG, NT, true> : kv4_attention_kernel<TQ, NG, NT, false>;
+    auto kernel = w.blocks ? kv4_attention_kernel<TQ, NG, true> : kv4_attention_kernel<TQ, NG, false>;
     FE_REQUIRE(fe_allow_smem((const void*)kernel, smem), "paged_attention_kv4: no kernel with %d bytes of shared memory", smem);
     const dim3 grid = w.blocks ? dim3((unsigned)w.blocks) : dim3((unsigned)(w.column_tiles * a.splits), (unsigned)a.nkv, (unsigned)w.requests);
     if (!w.blocks && a.splits > 1) {
@@ -931,7 +900,7 @@ template <typename TQ, int NG, int NT> int run(const Launch& w) {
         fe::launch(kernel, grid, WARPS * 32, smem, w.stream, a);
     if (const int rc = fe_check_launch("paged_attention_kv4")) return rc;
     if (!w.blocks) return 0;
-    fe::launch_as(FE_PDL_ELEMENTWISE, kv4_merge_kernel<TQ, NG, NT>, dim3((unsigned)a.nq, (unsigned)w.requests), MERGE_THREADS, 0, w.stream, a, w.blocks);
+    fe::launch_as(FE_PDL_ELEMENTWISE, kv4_merge_kernel<TQ, NG>, dim3((unsigned)a.nq, (unsigned)w.requests), MERGE_THREADS, 0, w.stream, a, w.blocks);
     return fe_check_launch("paged_attention_kv4 merge");
 }
 
@@ -965,7 +934,7 @@ extern "C" int fe_kv4_attention_plan(int requests, int tiles, int nq, int nkv, i
     if (!head_size_ok(d) || requests <= 0 || nq <= 0 || nkv <= 0) return -1;
     const long long items = (long long)requests * nkv * ((nq / nkv + 7) / 8), all = items * tiles;
     if (tiles <= 2 * WARPS * PAIR) return -1;
-    const long long most = dtype == FE_F32 ? with_groups(d, [](auto n) { return resident<float, n.value, 1>(); }) : with_groups(d, [](auto n) { return resident<bf16, n.value, 1>(); });
+    const long long most = dtype == FE_F32 ? with_groups(d, [](auto n) { return resident<float, n.value>(); }) : with_groups(d, [](auto n) { return resident<bf16, n.value>(); });
     const int sms = fe_sm_count(), round = WARPS * PAIR;
     const double tile = kv4_groups(d) / 4.0 * (dtype == FE_F32 ? 1.1 : 1.0);
     auto walk = [&](long long blocks, long long each) {          // of so many tiles by each of the blocks on the device
@@ -1016,5 +985,5 @@ extern "C" int fe_paged_attention_kv4(const void* q, long long q_stride, void* o
     const Problem a{q, q_stride, out, out_stride, (const unsigned char*)cache, block_table, bt_stride, cu_q, q_start, requests, nq, nkv, d, ps, num_pages,
                     scale * LOG2E, window, keep, sink, splits, (float*)scratch, tokens, status, fe_waits()};
     const Launch w{&a, requests, (int)(((long long)max_q_len * (nq / nkv) + 7) / 8), blocks, stream};
-    return dtype == FE_F32 ? with_groups(d, [&](auto n) { return run<float, n.value, 1>(w); }) : with_groups(d, [&](auto n) { return run<bf16, n.value, 1>(w); });
+    return dtype == FE_F32 ? with_groups(d, [&](auto n) { return run<float, n.value>(w); }) : with_groups(d, [&](auto n) { return run<bf16, n.value>(w); });
 }
