@@ -7,7 +7,7 @@
 //     o_g = sum_t (p_t s_tg) n_tg + sum_t p_t c_tg ,
 // so the codes themselves go through the tensor cores, as whole numbers that half precision holds exactly.  Of keys, scales are applied to
 // the groups' partial scores in 32 bits, centres as one more product of (c_g) with the sums of q_g.  What is rounded is the query to half precision (exact for
-// bfloat16 but for numbers 2^-24 of the row's largest).  Of values under 16-bit queries, scale and centre go into the decoded
+// bfloat16 from 2^-17 of the row's largest number on; what is smaller is off by up to 2^-25 of it).  Of values under 16-bit queries, scale and centre go into the decoded
 // numbers (one multiply-add for two, rounded to half precision: 2^-11 of a number, where bfloat16 results have 2^-8) and the weights p into half
 // precision; under 32-bit queries scales go to the weights in 32 bits and centres into sums of p_t c_tg, and query and weights are taken in two
 // parts, high and low: 22 bits of what is near the largest, and no step below 2^-24 where that is one (a weight of 2^-11 keeps 14 bits).
@@ -28,10 +28,11 @@
 // The reference point m is the largest score met, and moves only when it has grown by more than 2^8 (weights stay below that: in half's range).  Under 32-bit
 // queries a weight p s has to keep its place in half precision whatever the scale of the values, so there m is a maximum of score +
 // exponent of the token's largest value scale: 2^(score - m) s is then at most 2, and the sum of 2^(score - m) is kept in 32 bits, where
-// small scales may make it large.
+// small scales may make it large.  A NaN score never moves it: who has met no other has a NaN sum beside a maximum of -inf, and a merge passes it on.
 //
-// Bound by the instructions that decode and by the loads' latency: 16 requests of up to 32,768 keys, 40/8 heads of 128, 93 us for 396 MB of cache (4.3 TB/s; the copies
-// alone, nothing computed, 74); 64 of up to 8,191, 28/4 heads, 63; 8 of 2,049 14; a call of a few keys 7.
+// Long rows are bound by the instructions that decode: 16 requests of up to 32,768 keys, 40/8 heads of 128, 93 us for 396 MB of cache (4.3 TB/s; the copies
+// alone, nothing computed, 74); 64 of up to 8,191, 28/4 heads, 63.  Short ones by latency: 8 of 2,049 13; a call of a few keys 7.6.  The kernels of head size 128 under
+// 16-bit queries are held to 128 registers for four blocks an SM and spill 44 and 68 bytes a thread; 32-bit ones of head size 256 28 and 140.
 #include <type_traits>
 
 #define FE_PDL_CLASS 2      // FE_PDL_DECODE_ATTENTION
@@ -370,8 +371,9 @@ kv4_attention_kernel(const Problem a) {
 
         // ---- the queries as B operands, a column each; thread (g, t) holds numbers 32 i + 8 t .. + 7 of column g
         // Keys' codes are multiplied raised (by 1024 or 64: kv4_raise) where queries are 16-bit; ``lift`` is what that adds to a group's partial
-        // score, and eight codes' worth more, with the sign turned: the sums begin there.  That costs their last bits: with |q| in [1, 2)
-        // they are off by about 2^-24 8,000, a thousandth of what rounding the query to bfloat16 did.  (Values are summed over all keys,
+        // score, and eight codes' worth more, with the sign turned: the sums begin there.  That costs their last bits: with |q| in [1, 2) a sum
+        // reaches some 10,000 where signs are mixed and 66,000 where 32 numbers have one sign, in steps of 2^-10 and 2^-7.  Results are then off by
+        // 0.00168 of their norm where rounding them to bfloat16 is 0.00160 (one sign, scores tens apart; otherwise by less).  (Values are summed over all keys,
         // where the part of 1024 would grow: they are decoded in full, and so are keys under 32-bit queries.)
         constexpr bool RAISED = PARTS == 1;
         unsigned qsum[2];                                // (high, low) of the sums over group t, and over group t + 4
@@ -929,7 +931,8 @@ bool head_size_ok(int d) { return d >= 16 && d % 16 == 0 && d <= KV4_MAX_DIM; }
 // sums over the requests, pieces of two items in a block, a second kernel) and 0.12 for each request, and is no faster where all requests are as long as the longest, but
 // lengths that differ leave no block without work: its tiles are taken as three quarters of that.  28/4 heads of 128, microseconds, one block, clusters of 2, 4
 // and 8, shared: 64 requests of 512 keys 11 15 23 42 21; 64 of 1,101 19 22 32 52 34; 48 of 2,101 29 25 33 46 34; 8 of 2,049 23 17 14 14 19; 1 of
-// 8,301 70 40 25 18 17; 64 of 8,192 92 84 91 106 87; 64 of 1,024 to 8,191 84 74 71 88 64.
+// 8,301 70 40 25 18 17; 64 of 8,192 92 84 91 106 87; 64 of 1,024 to 8,191 84 74 71 88 64.  Head sizes other than 128 are taken in proportion to their groups of 32.
+// A captured step keeps the plan of the length it was captured for: at 32,768, 64 requests of 512 keys take 20 instead of 10.4.
 extern "C" int fe_kv4_attention_plan(int requests, int tiles, int nq, int nkv, int d, int dtype) {
     if (!head_size_ok(d) || requests <= 0 || nq <= 0 || nkv <= 0) return -1;
     const long long items = (long long)requests * nkv * ((nq / nkv + 7) / 8), all = items * tiles;

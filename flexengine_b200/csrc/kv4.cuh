@@ -36,7 +36,8 @@ __device__ __forceinline__ int kv4_key_at(int g, int p, int groups) { return ((p
 __device__ __forceinline__ int kv4_value_at(int g, int p, int groups) { return (p * groups + g) * 2; }
 
 // Eight codes of a word as four pairs of half-precision numbers: pair i holds the codes at bits 4 i and 16 + 4 i, as KV4_RAISED_EVEN + code
-// (i even: four bits under the exponent of 1024) or KV4_RAISED_ODD + code (i odd: four bits higher, under that of 64).
+// (i even: four bits under the exponent of 1024) or KV4_RAISED_ODD + code (i odd: four bits higher, under that of 64).  Integers put under an exponent
+// by bit operations: Kim et al., "Who Says Elephants Can't Run", 2022.
 constexpr float KV4_RAISED_EVEN = 1024.f, KV4_RAISED_ODD = 64.f;
 __device__ __forceinline__ void kv4_raise(unsigned w, unsigned* out) {
     const unsigned v = w >> 8;

@@ -16,9 +16,10 @@
 // takes (equal logits, as 16-bit ones often are) is taken apart by the bits of the logits.  The masses that stay are added up by
 // segments of the row, in the walk of the cut or one of their own, and the segment in which the target falls is gone through once more.
 //
-// Bound by the walks' integer work and, for one row, by the chain of barriers and trips between blocks.  64 rows of 152,064 (39 MB, read once 5.9 us), by what
+// Bound by the walks' integer work and, for one row, by the chain of barriers and trips between blocks; 1,024 threads have 64 registers each, and 1,344 bytes
+// a thread are spilled (2,064 of loads).  64 rows of 152,064 (39 MB, read once 5.9 us), by what
 // the rows ask for: the maximum alone 8 us, no limits 32, k = 50 46, top-p 0.9 75 to 88, k = 20,000 and top-p 119, a mixture 86; one row of the mixture
-// 37 to 39 in a cluster of 8 blocks.
+// 38 in a cluster of 8 blocks.
 #include <math_constants.h>
 
 #define FE_PDL_CLASS 8      // FE_PDL_SAMPLING

@@ -1875,7 +1875,7 @@ def kv4_portions(lengths, starts, nq: int, nkv: int, d: int, window: int = 0, te
     single tokens in clusters of S blocks.  What either takes, in microseconds (28/4 heads of 128; a tile is 16 keys, an item 256 rows): the
     one of single tokens 7 and 1 for 1,600 (tile of eight rows, key tile) pairs, or 0.13 for each key tile that one block walks; tcgen05 16 and 1.3 for each 64 keys of
     an item, all items shared out over the multiprocessors.  32 portions of 4 tokens after 2,000 take 43 and 56, 8 of 32 after 1,000 45 and 26, one of 2,048 292
-    and 60."""
+    and 60.  ``d`` is not looked at: at 14/2 heads of 64 the three take 19 and 32, 17 and 19, 94 and 51."""
     group = nq // nkv
     pairs = item_tiles = blocks = longest = 0
     for n, s in zip(lengths, starts):
@@ -1915,7 +1915,8 @@ def paged_attention_kv4(q, cache, block_table, ctx, nq, nkv, d, page_size, scale
     bfloat16 or float32, holds the turned queries in its first nq d columns; returns [T, nq d] of its type.  ``ctx``: the step
     (``cu_q``, ``q_start``, ``max_q_len``, ``max_ctx_len``).  ``window`` > 0: the last so many keys are seen, and with ``keep_first`` the sequence's first
     so many too; ``sink``: 1 is added to the softmax's denominator.  Codes are multiplied as whole numbers; queries and weights go through the
-    products in half precision (csrc/attention_kv4.cu), float32 ones in two parts of it: 22 bits of those near the row's largest."""
+    products in half precision (csrc/attention_kv4.cu), float32 ones in two parts of it: 22 bits of those near the row's largest.  A NaN among a row's
+    scores makes NaN of the row, one in a visible value of its group of 32 numbers."""
     what = "paged_attention_kv4"
     with _on(what, q, cache, block_table, ctx.cu_q, ctx.q_start):
         T, requests, pages, code = q.shape[0], ctx.cu_q.numel() - 1, block_table.shape[-1], _code(q.dtype)
