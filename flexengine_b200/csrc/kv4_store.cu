@@ -2,9 +2,10 @@
 // the queries beside them; and reading rows back.
 //
 // Rotation of the first ``rot`` entries of every query and key head by angle = position * inv_freq[j]: entries j and j + rot / 2 (halves)
-// or 2j and 2j + 1 (interleaved) turn together, a' = (a cos - b sin) gain, b' = (b cos + a sin) gain.  The angle is taken in 64 bits and
-// brought to within a quarter turn there: at position 100,000 a 32-bit product alone is off by up to 0.004, as much as bfloat16
-// rounds a query by, and enough to move every twentieth 4-bit code of a fast pair.  A token has rot / 2 angles, shared by its heads.
+// or 2j and 2j + 1 (interleaved) turn together, a' = (a cos - b sin) gain, b' = (b cos + a sin) gain.  The angle, its sine and its
+// cosine are taken in 64 bits: at position 100,000 a 32-bit product alone is off by up to 0.004, as much as bfloat16
+// rounds a query by, and enough to move every twentieth 4-bit code of a fast pair.  A token has rot / 2 angles, shared by its heads.  From there on every operation is rounded by itself
+// to 32 bits, up to the pair of scale and centre and the codes: next to the border of two codes the one that is taken is the formula's.
 //
 // A warp takes a row of d numbers (one head of one token), four neighbouring numbers a lane, so that a group of 32 is eight lanes: its
 // smallest and largest number are three shuffles away, and each lane's four codes are two neighbouring bytes of the row.  What bounds
@@ -19,18 +20,15 @@ namespace {
 
 constexpr int MAX_ROT = 256;
 
+// sine and cosine of the exact angle (31 and 24 bits make a product of 55 at most, rounded to 53), rounded to 32 bits once
 __device__ __forceinline__ void angle_of(int pos, float freq, float* sn, float* cs) {
-    const double a = (double)pos * (double)freq;                 // exact: 31 and 24 bits
-    const double turns = rint(a * 0.63661977236758134308);       // of a quarter: a 2 / pi
-    const float r = (float)fma(turns, -1.57079632679489661923, a);
-    const int quarter = (int)(long long)turns & 3;
-    float s, c;
-    sincosf(r, &s, &c);
-    *sn = quarter & 1 ? c : s;
-    *cs = quarter & 1 ? s : c;
-    if (quarter & 2) *sn = -*sn;
-    if ((quarter + 1) & 2) *cs = -*cs;
+    double s, c;
+    sincos((double)pos * (double)freq, &s, &c);
+    *sn = (float)s;
+    *cs = (float)c;
 }
+// a cos + b sin, each product rounded by itself: next to the border of two codes the one that is taken does not hang on which product the compiler fuses
+__device__ __forceinline__ float turn_by(float a, float cs, float b, float sn) { return __fadd_rn(__fmul_rn(a, cs), __fmul_rn(b, sn)); }
 
 // Four numbers from ``p``; VEC: from a boundary of four.
 template <typename T, bool VEC> __device__ __forceinline__ void load4(const T* p, float* v);
@@ -101,14 +99,25 @@ __device__ __forceinline__ void put_group(float* v, bool real, int u, int units,
     const float s = __half2float(scale);
     const __half centre = __float2half_rn(fmaf(8.f, s, low));
     // A code is 8 + (x - centre) / scale to the nearest whole number, 8 where the scale is 0 or NaN: adding 1.5 2^23 rounds and leaves it in the lowest
-    // bits.  The hardware's reciprocal (1 ulp) moves a code only within 2^-22 of the border to the next.
+    // bits.  The quotient by the hardware's reciprocal (1 ulp) is within 2^-20 of the rounded one, which is asked for next to a border only: without, one
+    // code in a million was another than the formula's, a whole step away.
     const float c = bad ? 0.f : __half2float(centre);
-    float each;
+    float each, off[4];
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(each) : "f"(s));
     each = s > 0.f ? each : 0.f;
+    bool close = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        off[e] = (v[e] - c) * each;
+        close |= fabsf(off[e] - __fsub_rn(__fadd_rn(off[e], 12582912.f), 12582912.f)) > 0.5f - 0x1p-18f;
+    }
+    if (close && s > 0.f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) off[e] = __fdiv_rn(v[e] - c, s);
+    }
     unsigned codes = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) codes |= (__float_as_uint(fminf(fmaxf(fmaf(v[e] - c, each, 8.f), 0.f), 15.f) + 12582912.f) & 15u) << (4 * e);
+    for (int e = 0; e < 4; ++e) codes |= ((__float_as_uint(fminf(fmaxf(off[e], -8.f), 7.f) + 12582912.f) + 8u) & 15u) << (4 * e);
     *reinterpret_cast<unsigned short*>(tile + into.codes + row_codes) = (unsigned short)codes;
     if ((u & 7) == 0) *reinterpret_cast<__half2*>(tile + into.pair + row_pairs) = __halves2half2(scale, centre);
 }
@@ -176,8 +185,8 @@ kv4_store_kernel(const TI* __restrict__ src, long long ld, const float* __restri
                         if (i + e >= turn.rot) break;
                         const int j = (i + e) / 2;
                         const float a = v[e], c = v[e + 1];
-                        v[e] = a * cosine[j] - c * sine[j];
-                        v[e + 1] = c * cosine[j] + a * sine[j];
+                        v[e] = turn_by(a, cosine[j], c, -sine[j]);
+                        v[e + 1] = turn_by(c, cosine[j], a, sine[j]);
                     }
                 } else {
                     // the entries these four turn with, half the rotated part away
@@ -202,7 +211,7 @@ kv4_store_kernel(const TI* __restrict__ src, long long ld, const float* __restri
                     for (int e = 0; e < 4; ++e) {
                         if (i + e >= turn.rot) break;
                         const int j = i + e < half ? i + e : i + e - half;
-                        v[e] = v[e] * cosine[j] + (i + e < half ? -o[e] : o[e]) * sine[j];
+                        v[e] = turn_by(v[e], cosine[j], i + e < half ? -o[e] : o[e], sine[j]);
                     }
                 }
             }
@@ -316,7 +325,7 @@ kv4_store_many_kernel(const TI* __restrict__ src, long long ld, const float* __r
                     for (int e = 0; e < 4; ++e) o[e] += w[e];
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = v[e] * cs[e] + o[e] * sn[e];
+                for (int e = 0; e < 4; ++e) v[e] = turn_by(v[e], cs[e], o[e], sn[e]);
             };
             // keys and values first: they take the longest; then the queries
             if (to.tile)

@@ -721,3 +721,34 @@ def test_special_numbers_leave_nan_where_they_were_and_nowhere_else(gen):
     bad[0, 4, 0, 32:] = bad[1, 5, 0, :32] = bad[1, 6, 0, 32:] = True
     assert torch.equal(keys.isnan(), bad[0]) and torch.equal(values.isnan(), bad[1])
     assert q.isnan().nonzero().tolist() == [[3, 64 + 7]]
+
+
+@pytest.mark.parametrize("T,pairs,d,rot", [(2048, "halves", 128, 128), (100, "halves", 128, 128), (1500, "interleaved", 64, 32), (700, "halves", 80, 20)])
+def test_codes_next_to_a_border_are_the_formula_s(T, pairs, d, rot, gen):
+    """Bias, rotation and rounding step by step in 32 bits, every operation rounded by itself, sines and cosines from 64 bits: the same pairs and the same
+    codes, all of them (some three million; a border is met within 2^-22 of a step a few times)."""
+    nq, nkv, page = 8, 8, 16
+    width = (nq + 2 * nkv) * d
+    projected = normal(gen, T, width) * torch.where(torch.rand(width, generator=gen, device=DEV) < 0.05, 6.0, 1.0)
+    bias = normal(gen, width)
+    positions = torch.arange(T, device=DEV, dtype=torch.int32) * 13
+    inv_freq = (1e6 ** (-torch.arange(rot // 2, dtype=torch.float64) * 2 / rot)).float().to(DEV)
+    cache = torch.zeros(kv4_shape(-(-T // page), nkv, page, d), dtype=torch.uint8, device=DEV)
+    slots = torch.arange(T, device=DEV, dtype=torch.int32)
+    q = ops().qkv_rope_kv4(projected, bias, positions, inv_freq, rot, slots, cache, nq, nkv, d, page, pairs=pairs)
+    x = (projected.cpu() + bias.cpu()).view(T, nq + 2 * nkv, d)
+    angle = positions.cpu().double()[:, None, None] * inv_freq.cpu().double()
+    cos, sin = angle.cos().float(), angle.sin().float()
+    i = torch.arange(rot // 2)
+    a, b = (i, i + rot // 2) if pairs == "halves" else (2 * i, 2 * i + 1)
+    turned = x[:, :nq + nkv].clone()
+    turned[..., a], turned[..., b] = x[:, :nq + nkv, a] * cos - x[:, :nq + nkv, b] * sin, x[:, :nq + nkv, b] * cos + x[:, :nq + nkv, a] * sin
+    assert torch.equal(q.cpu(), turned[:, :nq].flatten(1))
+    for got, want in zip(kv4_refs.read_rows(cache, slots, d), (turned[:, nq:], x[:, nq + nkv:])):
+        for first in range(0, d, 32):
+            w = want[..., first:first + 32]
+            low, high = w.amin(-1, keepdim=True), w.amax(-1, keepdim=True)
+            scale = ((high - low) * torch.tensor(1 / 15)).half().float()          # by a fifteenth as 32 bits hold it
+            centre = (low + 8 * scale).half().float()
+            code = (torch.round((w - centre) / scale) + 8).clamp(0, 15)
+            assert torch.equal(got[..., first:first + 32], centre.double() + (code.double() - 8) * scale.double())
